@@ -68,6 +68,13 @@ from mpgcn_amd.ops.functional import (  # noqa: E402,F401
     mode1_proj,
     mode2_bias_act,
 )
+from mpgcn_amd.ops.sequence import (  # noqa: E402,F401
+    norm_gate_residual,
+    selective_scan,
+    selective_scan_step,
+    short_conv,
+    short_conv_step,
+)
 
 __all__ = [
     "has_ext",
@@ -81,4 +88,9 @@ __all__ = [
     "linear_act",
     "mode1_proj",
     "mode2_bias_act",
+    "norm_gate_residual",
+    "selective_scan",
+    "selective_scan_step",
+    "short_conv",
+    "short_conv_step",
 ]

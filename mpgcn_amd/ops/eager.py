@@ -118,3 +118,86 @@ def lstm_forward_eager(
         h = o * torch.tanh(c)
         outs.append(h)
     return torch.stack(outs, dim=1), h, c
+
+
+# ---- sequence operators -----------------------------------------------------
+# The definitions of mpgcn_amd/ops/sequence.py in elementary operations: f32
+# (f64 for f64 inputs) inside, rounded once to the output's type.
+
+
+def _wide(*tensors):
+    dt = torch.float64 if any(t is not None and t.dtype == torch.float64 for t in tensors) else torch.float32
+    return [None if t is None else t.to(dt) for t in tensors]
+
+
+def valid_tokens(lengths: torch.Tensor | None, L: int) -> torch.Tensor | None:
+    """(B, L, 1) truth values of the tokens before each sequence's end."""
+    if lengths is None:
+        return None
+    return (torch.arange(L, device=lengths.device) < lengths.unsqueeze(1)).unsqueeze(-1)
+
+
+def short_conv_eager(x, weight, bias, state, lengths, silu):
+    """-> (y (B, L, D), final state (B, K-1, D)), both of x's type."""
+    B, L, D = x.shape
+    K = weight.shape[1]
+    xw, w, b, s = _wide(x, weight, bias, state)
+    zero = xw.new_zeros(())
+    ok = valid_tokens(lengths, L)
+    if ok is not None:
+        xw = torch.where(ok, xw, zero)
+    xp = torch.cat([xw.new_zeros(B, K - 1, D) if s is None else s, xw], dim=1)
+    acc = sum(xp[:, k:k + L] * w[:, k] for k in range(K))
+    if b is not None:
+        acc = acc + b
+    y = acc * torch.sigmoid(acc) if silu else acc
+    if ok is not None:
+        y = torch.where(ok, y, zero)
+    if lengths is None:
+        last = xp[:, L:]
+    else:
+        at = lengths.clamp(0, L).long().unsqueeze(1) + torch.arange(K - 1, device=x.device)
+        last = xp.gather(1, at.unsqueeze(-1).expand(B, K - 1, D))
+    return y.to(x.dtype), last.to(x.dtype).contiguous()
+
+
+def selective_scan_eager(u, delta, A, B, C, skip, delta_bias, softplus, state, lengths):
+    """B, C: (batch, L, G, N) -> (y (batch, L, D) of u's type, final state (batch, D, N))."""
+    nb, L, D = u.shape
+    G, N = B.shape[2], B.shape[3]
+    uw, dw, Aw, Bw, Cw, sk, db, h = _wide(u, delta, A, B, C, skip, delta_bias, state)
+    zero = uw.new_zeros(())
+    step = dw if db is None else dw + db
+    if softplus:
+        step = step.clamp(min=0) + torch.log1p(torch.exp(-step.abs()))
+    ok = valid_tokens(lengths, L)
+    if ok is not None:
+        step, uw = torch.where(ok, step, zero), torch.where(ok, uw, zero)
+        Bw, Cw = (torch.where(ok.unsqueeze(-1), t, zero) for t in (Bw, Cw))
+    h = uw.new_zeros(nb, D, N) if h is None else h.clone()
+    ys = []
+    for t in range(L):
+        dt = step[:, t].unsqueeze(-1)
+        Bt, Ct = (v[:, t].repeat_interleave(D // G, dim=1) for v in (Bw, Cw))
+        h = torch.exp(dt * Aw) * h + dt * uw[:, t].unsqueeze(-1) * Bt
+        ys.append((h * Ct).sum(-1))
+    y = torch.stack(ys, dim=1) if ys else uw.new_zeros(nb, 0, D)
+    if sk is not None:
+        y = y + sk * uw
+    return y.to(u.dtype), h
+
+
+def norm_gate_residual_eager(x, gate, post_weight, residual, scale, pre_weight, eps):
+    """-> (y or None, h or None)."""
+    p, g, w1, r, s, w2 = _wide(x, gate, post_weight, residual, scale, pre_weight)
+    if g is not None:
+        p = p * (g * torch.sigmoid(g))
+    if w1 is not None:
+        p = p * torch.rsqrt((p * p).mean(-1, keepdim=True) + eps) * w1
+    if r is None:
+        return p.to(x.dtype), None
+    h = r + (p if s is None else p * s)
+    y = None
+    if w2 is not None:
+        y = (h * torch.rsqrt((h * h).mean(-1, keepdim=True) + eps) * w2).to(x.dtype)
+    return y, h.to(residual.dtype)

@@ -1240,7 +1240,10 @@ std::vector<torch::Tensor> relu_bwd_colsum(torch::Tensor dH, torch::Tensor Y,
     return {dY, colsum};
 }
 
+void bind_sequence(pybind11::module_& m);  // ext_seq.hip
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_sequence(m);
     m.def("bdgcn_mode1", &bdgcn_mode1, "origin-axis graph product (K1)",
           py::arg("X"), py::arg("GT"), py::arg("id_skip") = false,
           py::arg("no_fill") = false);

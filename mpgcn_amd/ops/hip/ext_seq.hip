@@ -1,0 +1,431 @@
+// Torch bindings of the sequence operators: short causal convolution, selective
+// scan, norms around a block. mpgcn_amd/ops/sequence.py checks the arguments
+// for its users; what the kernels rely on for their bounds is checked here too.
+#include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPException.h>
+#include <c10/hip/HIPStream.h>
+
+#include "params.hpp"
+
+namespace {
+
+using torch::Tensor;
+using Opt = c10::optional<Tensor>;
+
+bool has(const Opt& t) { return t.has_value() && t->defined(); }
+void* ptr(const Opt& t) { return has(t) ? t->data_ptr() : nullptr; }
+const float* fptr(const Opt& t) { return has(t) ? t->data_ptr<float>() : nullptr; }
+
+int f32(const Tensor& t) { return t.scalar_type() == torch::kFloat ? 1 : 0; }
+
+hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+void check_data(const Tensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type());
+    TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+    TORCH_CHECK(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, name, " must be contiguous in its last axis");
+}
+
+void check_like(const Opt& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
+    if (!has(t)) return;
+    check_data(*t, like, shape, name);
+    TORCH_CHECK(t->is_contiguous(), name, " must be contiguous");
+}
+
+void check_f32(const Opt& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
+    if (!has(t)) return;
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), name, " must be on ", like.device());
+    TORCH_CHECK(t->scalar_type() == torch::kFloat, name, " must be f32");
+    TORCH_CHECK(t->sizes() == shape && t->is_contiguous(), name, " must be contiguous with shape ", shape);
+}
+
+int check_lens(const Opt& t, const Tensor& like, long B) {
+    if (!has(t)) return 0;
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), "lengths must be on ", like.device());
+    TORCH_CHECK(t->scalar_type() == torch::kInt || t->scalar_type() == torch::kLong,
+                "lengths must be int32 or int64");
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == B && t->is_contiguous(), "lengths must have shape (B,)");
+    return t->scalar_type() == torch::kLong ? 1 : 0;
+}
+
+void check_main(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be on GPU");
+    TORCH_CHECK(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat, name,
+                " must be bf16 or f32");
+    for (long s : t.sizes()) TORCH_CHECK(s <= INT_MAX / 2, name, ": extent too large");
+}
+
+// Rows of `t` can be read `elems` channels at a time, in pieces of 16 bytes at most.
+bool aligned(const Tensor& t, long elems) {
+    const long es = t.element_size(), step = elems * es < 16 ? elems * es : 16;
+    if ((uintptr_t)t.data_ptr() % step) return false;
+    for (long i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) * es % step) return false;
+    return true;
+}
+bool aligned(const Opt& t, long elems) { return !has(t) || aligned(*t, elems); }
+
+Tensor empty_f32(const Tensor& like, at::IntArrayRef shape) {
+    return torch::empty(shape, like.options().dtype(torch::kFloat));
+}
+
+// ---- short convolution ------------------------------------------------------
+
+ShortConvParams conv_params(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& s0,
+                            const Opt& lens, bool silu) {
+    check_main(x, "x");
+    TORCH_CHECK(x.dim() == 3, "x must be (B, L, D)");
+    const long B = x.size(0), L = x.size(1), D = x.size(2);
+    TORCH_CHECK(w.dim() == 2 && w.size(0) == D && w.size(1) >= 2 && w.size(1) <= 4, "weight must be (D, K), K in 2..4");
+    const long K = w.size(1);
+    check_data(x, x, x.sizes(), "x");
+    check_f32(w, x, {D, K}, "weight");
+    check_f32(bias, x, {D}, "bias");
+    check_like(s0, x, {B, K - 1, D}, "state");
+    ShortConvParams p{};
+    p.lens64 = check_lens(lens, x, B);
+    p.x = x.data_ptr();
+    p.w = w.data_ptr<float>();
+    p.bias = fptr(bias);
+    p.s0 = ptr(s0);
+    p.lens = ptr(lens);
+    p.x_b = x.stride(0);
+    p.x_t = x.stride(1);
+    p.B = (int)B;
+    p.L = (int)L;
+    p.D = (int)D;
+    p.silu = silu ? 1 : 0;
+    return p;
+}
+
+std::vector<Tensor> short_conv_fwd(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state) {
+    at::DeviceGuard guard(x.device());
+    auto p = conv_params(x, w, bias, s0, lens, silu);
+    const long K = w.size(1);
+    auto y = torch::empty({p.B, p.L, p.D}, x.options());
+    auto s1 = want_state ? torch::empty({p.B, K - 1, p.D}, x.options()) : Tensor();
+    if (p.B && p.D && (p.L || want_state)) {
+        p.y = y.data_ptr();
+        p.s1 = want_state ? s1.data_ptr() : nullptr;
+        const int vec = p.D % 8 == 0 && aligned(x, 8) && aligned(s0, 8);
+        short_conv_fwd_launch(p, (int)K, f32(x), vec, stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return {y, s1};
+}
+
+// {dx, dw (D, K), db (D,), dstate or undefined}
+std::vector<Tensor> short_conv_bwd(Tensor dy, Opt ds1, Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu,
+                                   bool want_state) {
+    at::DeviceGuard guard(x.device());
+    auto p = conv_params(x, w, bias, s0, lens, silu);
+    const long K = w.size(1), D = p.D;
+    check_like(dy, x, {p.B, p.L, p.D}, "dy");
+    check_like(ds1, x, {p.B, K - 1, p.D}, "dstate");
+    auto dx = torch::empty({p.B, p.L, p.D}, x.options());
+    auto ds0 = want_state ? torch::empty({p.B, K - 1, p.D}, x.options()) : Tensor();
+    if (!p.B || !p.D) {
+        auto z = torch::zeros({D * (K + 1)}, w.options());
+        return {dx, z.narrow(0, 0, D * K).view({D, K}), z.narrow(0, D * K, D), ds0};
+    }
+    p.slots = short_conv_bwd_slots(p.B, p.L, D);
+    auto ws = empty_f32(x, {p.slots, D * (K + 1)});
+    auto sums = empty_f32(x, {D * (K + 1)});
+    p.dy = dy.data_ptr();
+    p.ds1 = ptr(ds1);
+    p.dx = dx.data_ptr();
+    p.ds0 = want_state ? ds0.data_ptr() : nullptr;
+    p.ws = ws.data_ptr<float>();
+    const int vec = D % 8 == 0 && aligned(x, 8) && aligned(s0, 8) && aligned(dy, 8) && aligned(ds1, 8);
+    short_conv_bwd_launch(p, (int)K, f32(x), vec, stream());
+    seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, D * (K + 1), stream());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    return {dx, sums.narrow(0, 0, D * K).view({D, K}), sums.narrow(0, D * K, D), ds0};
+}
+
+Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt bias, bool silu) {
+    at::DeviceGuard guard(x.device());
+    check_main(x, "x");
+    TORCH_CHECK(x.dim() == 2, "x must be (B, D)");
+    const long B = x.size(0), D = x.size(1);
+    TORCH_CHECK(w.dim() == 2 && w.size(1) >= 2 && w.size(1) <= 4, "weight must be (D, K), K in 2..4");
+    const long K = w.size(1);
+    check_data(x, x, x.sizes(), "x");
+    check_f32(w, x, {D, K}, "weight");
+    check_f32(bias, x, {D}, "bias");
+    check_like(state, x, {B, K - 1, D}, "state");
+    check_like(state_out, x, {B, K - 1, D}, "state_out");
+    auto y = torch::empty({B, D}, x.options());
+    if (B && D) {
+        const int vec = D % 8 == 0 && aligned(x, 8) && aligned(state, 8) && aligned(state_out, 8);
+        short_conv_step_launch(x.data_ptr(), x.stride(0), state.data_ptr(), state_out.data_ptr(),
+                               w.data_ptr<float>(), fptr(bias), y.data_ptr(), B, (int)D, (int)K, silu,
+                               f32(x), vec, stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return y;
+}
+
+// ---- selective scan ---------------------------------------------------------
+
+ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                       const Opt& skip, const Opt& dbias, const Opt& h0, const Opt& lens, bool softplus) {
+    check_main(u, "u");
+    TORCH_CHECK(u.dim() == 3, "u must be (B, L, D)");
+    const long B = u.size(0), L = u.size(1), D = u.size(2);
+    TORCH_CHECK(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be (D, N), N in 1..64");
+    const long N = A.size(1);
+    TORCH_CHECK(Bm.dim() == 4 && Bm.size(2) >= 1 && D % Bm.size(2) == 0, "B must be (B, L, G, N), G a divisor of D");
+    const long G = Bm.size(2);
+    check_data(u, u, u.sizes(), "u");
+    check_data(delta, u, {B, L, D}, "delta");
+    check_data(Bm, u, {B, L, G, N}, "B");
+    check_data(Cm, u, {B, L, G, N}, "C");
+    check_f32(A, u, {D, N}, "A");
+    check_f32(skip, u, {D}, "skip");
+    check_f32(dbias, u, {D}, "delta_bias");
+    check_f32(h0, u, {B, D, N}, "state");
+    ScanParams p{};
+    p.lens64 = check_lens(lens, u, B);
+    p.u = u.data_ptr();
+    p.delta = delta.data_ptr();
+    p.Bm = Bm.data_ptr();
+    p.Cm = Cm.data_ptr();
+    p.A = A.data_ptr<float>();
+    p.skip = fptr(skip);
+    p.dbias = fptr(dbias);
+    p.h0 = fptr(h0);
+    p.lens = ptr(lens);
+    p.u_b = u.stride(0); p.u_t = u.stride(1);
+    p.d_b = delta.stride(0); p.d_t = delta.stride(1);
+    p.B_b = Bm.stride(0); p.B_t = Bm.stride(1); p.B_g = Bm.stride(2);
+    p.C_b = Cm.stride(0); p.C_t = Cm.stride(1); p.C_g = Cm.stride(2);
+    p.B = (int)B; p.L = (int)L; p.D = (int)D; p.N = (int)N; p.G = (int)G;
+    p.softplus = softplus ? 1 : 0;
+    p.bvec = aligned(Bm, 16) && aligned(Cm, 16);
+    return p;
+}
+
+// {y, final state, states entering every chunk or undefined}
+std::vector<Tensor> selective_scan_fwd(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias,
+                                       Opt h0, Opt lens, bool softplus, bool want_state, bool train) {
+    at::DeviceGuard guard(u.device());
+    auto p = scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus);
+    auto y = torch::empty({p.B, p.L, p.D}, u.options());
+    auto h1 = want_state ? empty_f32(u, {p.B, p.D, p.N}) : Tensor();
+    const long chunks = (p.L + scan_chunk() - 1) / scan_chunk();
+    // one chunk starts from the state given: nothing to keep
+    auto ck = train && chunks > 1 ? empty_f32(u, {p.B, chunks, p.D, p.N}) : Tensor();
+    if (p.B && p.D && (p.L || want_state)) {
+        p.y = y.data_ptr();
+        p.h1 = want_state ? h1.data_ptr<float>() : nullptr;
+        p.ckpt = ck.defined() ? ck.data_ptr<float>() : nullptr;
+        scan_fwd_launch(p, f32(u), stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return {y, h1, ck};
+}
+
+// {du, ddelta, dA, dB, dC, dskip, ddelta_bias, dstate or undefined}
+std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm,
+                                       Opt skip, Opt dbias, Opt h0, Opt lens, Opt ck, bool softplus,
+                                       bool want_state) {
+    at::DeviceGuard guard(u.device());
+    auto p = scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus);
+    const long B = p.B, L = p.L, D = p.D, N = p.N, G = p.G;
+    const long chunks = (L + scan_chunk() - 1) / scan_chunk();
+    check_like(dy, u, {B, L, D}, "dy");
+    check_f32(dh1, u, {B, D, N}, "dstate");
+    check_f32(ck, u, {B, chunks, D, N}, "chunk states");
+    TORCH_CHECK(has(ck) || chunks <= 1, "the forward kept no chunk states");
+    auto du = torch::empty({B, L, D}, u.options());
+    auto dd = torch::empty({B, L, D}, u.options());
+    auto dB = torch::empty({B, L, G, N}, u.options());
+    auto dC = torch::empty({B, L, G, N}, u.options());
+    auto dh0 = want_state ? empty_f32(u, {B, D, N}) : Tensor();
+    auto split = [&](const Tensor& s) {
+        return std::vector<Tensor>{du, dd, s.narrow(0, 0, D * N).view({D, N}), dB, dC, s.narrow(0, D * N, D),
+                                   s.narrow(0, D * N + D, D), dh0};
+    };
+    if (!B || !D) return split(torch::zeros({D * (N + 2)}, A.options()));
+    p.slots = scan_bwd_slots(B, D, G, N);
+    const long cb = scan_cblocks(D, G, N);
+    auto ws = empty_f32(u, {p.slots, D * (N + 2)});
+    auto sums = empty_f32(u, {D * (N + 2)});
+    auto dbc = empty_f32(u, {cb, B, L, G, 2, N});
+    p.dy = ptr(dy);
+    p.dh1 = fptr(dh1);
+    p.du = du.data_ptr();
+    p.ddelta = dd.data_ptr();
+    p.ckpt = has(ck) ? ck->data_ptr<float>() : nullptr;
+    p.dbc = dbc.data_ptr<float>();
+    p.ws = ws.data_ptr<float>();
+    p.dh0 = want_state ? dh0.data_ptr<float>() : nullptr;
+    scan_bwd_launch(p, f32(u), stream());
+    seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, D * (N + 2), stream());
+    if (L) scan_bc_reduce_launch(p.dbc, dB.data_ptr(), dC.data_ptr(), cb, B * L * G, p.N, f32(u), stream());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    return split(sums);
+}
+
+Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state, Tensor state_out,
+                           Opt skip, Opt dbias, bool softplus) {
+    at::DeviceGuard guard(u.device());
+    check_main(u, "u");
+    TORCH_CHECK(u.dim() == 2, "u must be (B, D)");
+    const long B = u.size(0), D = u.size(1);
+    TORCH_CHECK(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be (D, N), N in 1..64");
+    const long N = A.size(1);
+    TORCH_CHECK(Bm.dim() == 3 && Bm.size(1) >= 1 && D % Bm.size(1) == 0, "B must be (B, G, N), G a divisor of D");
+    const long G = Bm.size(1);
+    check_data(u, u, u.sizes(), "u");
+    check_data(delta, u, {B, D}, "delta");
+    check_data(Bm, u, {B, G, N}, "B");
+    check_data(Cm, u, {B, G, N}, "C");
+    check_f32(A, u, {D, N}, "A");
+    check_f32(skip, u, {D}, "skip");
+    check_f32(dbias, u, {D}, "delta_bias");
+    check_f32(state, u, {B, D, N}, "state");
+    check_f32(state_out, u, {B, D, N}, "state_out");
+    auto y = torch::empty({B, D}, u.options());
+    if (B && D) {
+        ScanStepParams p{};
+        p.u = u.data_ptr(); p.delta = delta.data_ptr(); p.Bm = Bm.data_ptr(); p.Cm = Cm.data_ptr();
+        p.A = A.data_ptr<float>(); p.skip = fptr(skip); p.dbias = fptr(dbias);
+        p.h = state.data_ptr<float>(); p.h_out = state_out.data_ptr<float>(); p.y = y.data_ptr();
+        p.u_b = u.stride(0); p.d_b = delta.stride(0);
+        p.B_b = Bm.stride(0); p.B_g = Bm.stride(1); p.C_b = Cm.stride(0); p.C_g = Cm.stride(1);
+        p.B = (int)B; p.D = (int)D; p.N = (int)N; p.G = (int)G;
+        p.softplus = softplus ? 1 : 0;
+        p.bvec = N % 4 == 0 && aligned(Bm, 4) && aligned(Cm, 4) && aligned(A, 4) && aligned(state, 4) &&
+                 aligned(state_out, 4);
+        scan_step_launch(p, f32(u), stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return y;
+}
+
+// ---- norms around a block ---------------------------------------------------
+
+BlockNormParams norm_params(const Tensor& x, const Opt& gate, const Opt& post, const Opt& res, const Opt& scale,
+                            const Opt& pre, double eps) {
+    check_main(x, "x");
+    TORCH_CHECK(x.dim() == 2, "x must be (R, D)");
+    const long R = x.size(0), D = x.size(1);
+    TORCH_CHECK(D <= 16384, "D must be at most 16384");
+    check_data(x, x, x.sizes(), "x");
+    if (has(gate)) check_data(*gate, x, {R, D}, "gate");
+    if (has(res)) {
+        check_main(*res, "residual");
+        check_data(*res, *res, {R, D}, "residual");
+        TORCH_CHECK(res->device() == x.device(), "residual must be on ", x.device());
+    }
+    TORCH_CHECK(has(post) || has(pre), "a norm's weight is needed");
+    TORCH_CHECK(has(res) || !(has(scale) || has(pre)), "scale and pre need a residual");
+    check_f32(post, x, {D}, "post_weight");
+    check_f32(scale, x, {D}, "scale");
+    check_f32(pre, x, {D}, "pre_weight");
+    BlockNormParams p{};
+    p.x = x.data_ptr();
+    p.gate = ptr(gate);
+    p.post = fptr(post);
+    p.res = ptr(res);
+    p.scale = fptr(scale);
+    p.pre = fptr(pre);
+    p.x_r = x.stride(0);
+    p.g_r = has(gate) ? gate->stride(0) : 0;
+    p.r_r = has(res) ? res->stride(0) : 0;
+    p.R = R;
+    p.D = (int)D;
+    p.eps = (float)eps;
+    p.vec = D % 8 == 0 && aligned(x, 8) && aligned(gate, 8) && aligned(res, 8);
+    return p;
+}
+
+// {y, h, inv1, inv2}, those that there are
+std::vector<Tensor> block_norm_fwd(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps,
+                                   bool train) {
+    at::DeviceGuard guard(x.device());
+    auto p = norm_params(x, gate, post, res, scale, pre, eps);
+    const long R = p.R, D = p.D;
+    auto y = has(pre) || !has(res) ? torch::empty({R, D}, x.options()) : Tensor();
+    auto h = has(res) ? torch::empty({R, D}, res->options()) : Tensor();
+    auto i1 = train && has(post) ? empty_f32(x, {R}) : Tensor();
+    auto i2 = train && has(pre) ? empty_f32(x, {R}) : Tensor();
+    if (R && D) {
+        p.y = y.defined() ? y.data_ptr() : nullptr;
+        p.h = h.defined() ? h.data_ptr() : nullptr;
+        p.inv1 = i1.defined() ? i1.data_ptr<float>() : nullptr;
+        p.inv2 = i2.defined() ? i2.data_ptr<float>() : nullptr;
+        block_norm_fwd_launch(p, f32(x), has(res) ? f32(*res) : f32(x), stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return {y, h, i1, i2};
+}
+
+// {dx, dgate, dpost, dresidual, dscale, dpre}, those that there are
+std::vector<Tensor> block_norm_bwd(Opt dy, Opt dh, Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre,
+                                   Opt inv1, Opt inv2, double eps) {
+    at::DeviceGuard guard(x.device());
+    auto p = norm_params(x, gate, post, res, scale, pre, eps);
+    const long R = p.R, D = p.D;
+    check_like(dy, x, {R, D}, "dy");
+    if (has(res)) check_like(dh, *res, {R, D}, "dh");
+    check_f32(inv1, x, {R}, "inv1");
+    check_f32(inv2, x, {R}, "inv2");
+    TORCH_CHECK(has(inv1) == has(post) && has(inv2) == has(pre), "the forward kept no row statistics");
+    auto dx = torch::empty({R, D}, x.options());
+    auto dg = has(gate) ? torch::empty({R, D}, x.options()) : Tensor();
+    auto dr = has(res) ? torch::empty({R, D}, res->options()) : Tensor();
+    const long nw = has(post) + has(scale) + has(pre);
+    Tensor sums;
+    if (R && D) {
+        p.slots = block_norm_slots(R, D);
+        auto ws = empty_f32(x, {p.slots, nw * D});
+        sums = empty_f32(x, {nw, D});
+        p.inv1 = (float*)fptr(inv1);
+        p.inv2 = (float*)fptr(inv2);
+        p.dy = ptr(dy);
+        p.dh = has(res) ? ptr(dh) : nullptr;
+        p.dx = dx.data_ptr();
+        p.dgate = ptr(dg);
+        p.dres = ptr(dr);
+        p.ws = ws.data_ptr<float>();
+        p.vec = p.vec && aligned(dy, 8) && aligned(dh, 8);
+        block_norm_bwd_launch(p, f32(x), has(res) ? f32(*res) : f32(x), stream());
+        seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, nw * D, stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    } else {
+        sums = torch::zeros({nw, D}, x.options().dtype(torch::kFloat));
+    }
+    long at = 0;
+    auto next = [&](const Opt& w) { return has(w) ? sums.select(0, at++) : Tensor(); };
+    auto dpost = next(post), dscale = next(scale), dpre = next(pre);
+    return {dx, dg, dpost, dr, dscale, dpre};
+}
+
+}  // namespace
+
+// A leaf whose gradient an eager graph, still alive, accumulates on another
+// stream: a backward captured now would wait for that stream and break the capture.
+bool accumulates_elsewhere(Tensor leaf) {
+    auto acc = torch::autograd::impl::try_get_grad_accumulator(leaf);
+    if (!acc) return false;
+    const auto s = acc->stream();
+    return s.has_value() && *s != c10::impl::VirtualGuardImpl(s->device_type()).getStream(s->device());
+}
+
+void bind_sequence(pybind11::module_& m) {
+    m.def("accumulates_elsewhere", &accumulates_elsewhere, "leaf has a live accumulator on another stream");
+    m.def("short_conv_fwd", &short_conv_fwd, "short causal convolution");
+    m.def("short_conv_bwd", &short_conv_bwd, "backward of short_conv_fwd");
+    m.def("short_conv_step", &short_conv_step, "short causal convolution of one new token");
+    m.def("selective_scan_fwd", &selective_scan_fwd, "selective state space scan");
+    m.def("selective_scan_bwd", &selective_scan_bwd, "backward of selective_scan_fwd");
+    m.def("selective_scan_step", &selective_scan_step, "selective state space scan of one new token");
+    m.def("block_norm_fwd", &block_norm_fwd, "norms around a block with gate and residual scale");
+    m.def("block_norm_bwd", &block_norm_bwd, "backward of block_norm_fwd");
+}

@@ -177,3 +177,105 @@ void cheby_seed_launch(const float* A, const float* d, float* OUT, long B,
 void rwd_norm_t_launch(const float* A, const float* d, float* OUT, long B,
                        int N, long sOUT, hipStream_t s);
 }
+
+// ---- sequence operators (ext_seq.hip) ---------------------------------------
+// Strides count elements; the channel axis is contiguous in every tensor.
+
+struct ShortConvParams {
+    const void* x;       // (B, L, D)
+    const float* w;      // (D, K) taps, w[:, K-1] on the newest input
+    const float* bias;   // (D,) or null
+    const void* s0;      // (B, K-1, D) inputs before the first, or null (zeros)
+    const void* lens;    // (B,) int32/int64 valid lengths, or null (all L)
+    void* y;             // (B, L, D) contiguous
+    void* s1;            // (B, K-1, D) the last K-1 valid inputs, or null
+    const void* dy;      // (B, L, D) contiguous
+    const void* ds1;     // (B, K-1, D) gradient of s1, or null
+    void* dx;            // (B, L, D) contiguous
+    void* ds0;           // (B, K-1, D) or null
+    float* ws;           // (slots, D*K + D) partial dw | db
+    long x_b, x_t;
+    int B, L, D;
+    int lens64, silu;
+    int slots;           // backward: blocks that share one channel group
+};
+
+struct ScanParams {
+    const void *u, *delta, *Bm, *Cm;  // (B, L, D) x2, (B, L, G, N) x2
+    const float* A;      // (D, N)
+    const float* skip;   // (D,) or null
+    const float* dbias;  // (D,) or null
+    const float* h0;     // (B, D, N) or null (zeros)
+    const void* lens;    // (B,) or null
+    void* y;             // (B, L, D) contiguous
+    float* h1;           // (B, D, N) final state, or null
+    float* ckpt;         // (B, chunks, D, N) state entering every chunk, or null
+    // backward
+    const void* dy;      // (B, L, D) contiguous, or null (zeros)
+    const float* dh1;    // (B, D, N) or null
+    void *du, *ddelta;   // (B, L, D) contiguous
+    float* dbc;          // (cblocks, B, L, G, 2, N) partial dB | dC
+    float* ws;           // (slots, D*N + 2*D) partial dA | dskip | dbias
+    float* dh0;          // (B, D, N) or null
+    long u_b, u_t, d_b, d_t, B_b, B_t, B_g, C_b, C_t, C_g;
+    int B, L, D, N, G;
+    int softplus, lens64;
+    int bvec;            // rows of Bm/Cm can be read 16 bytes at a time
+    int slots;
+};
+
+struct ScanStepParams {
+    const void *u, *delta, *Bm, *Cm;  // (B, D) x2, (B, G, N) x2
+    const float *A, *skip, *dbias;
+    const float* h;      // (B, D, N)
+    float* h_out;        // (B, D, N), may be h itself
+    void* y;             // (B, D) contiguous
+    long u_b, d_b, B_b, B_g, C_b, C_g;
+    int B, D, N, G;
+    int softplus;
+    int bvec;            // N a multiple of 4 and every row of Bm/Cm, A, h aligned for it
+};
+
+struct BlockNormParams {
+    const void* x;       // (R, D) rows x_r apart
+    const void* gate;    // (R, D) or null
+    const float* post;   // (D,) or null
+    const void* res;     // (R, D) or null
+    const float* scale;  // (D,) or null
+    const float* pre;    // (D,) or null
+    void* y;             // (R, D) contiguous, or null
+    void* h;             // (R, D) contiguous, or null
+    float *inv1, *inv2;  // (R,) reciprocal rms of the two norms, or null
+    // backward
+    const void* dy;      // (R, D) contiguous, or null (zeros)
+    const void* dh;      // (R, D) contiguous, or null (zeros)
+    void *dx, *dgate, *dres;
+    float* ws;           // (slots, weights*D) partial dpost | dscale | dpre, those there are
+    long x_r, g_r, r_r;
+    long R;
+    int D;
+    float eps;
+    int vec;             // every row of every tensor can be read 16 bytes at a time
+    int slots;
+};
+
+extern "C" {
+void seq_colsum_launch(const float* ws, float* out, long nb, long E, hipStream_t s);
+void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
+int short_conv_bwd_slots(long B, long L, long D);
+void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
+void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out, const float* w,
+                            const float* bias, void* y, long B, int D, int K, int silu, int is_f32,
+                            int vec, hipStream_t s);
+int scan_chunk();
+int scan_cblocks(long D, long G, long N);
+int scan_bwd_slots(long B, long D, long G, long N);
+void scan_fwd_launch(const ScanParams& p, int is_f32, hipStream_t s);
+void scan_bwd_launch(const ScanParams& p, int is_f32, hipStream_t s);
+void scan_bc_reduce_launch(const float* dbc, void* dB, void* dC, long cblocks, long rows, int N,
+                           int is_f32, hipStream_t s);
+void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s);
+int block_norm_slots(long R, long D);
+void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);
+void block_norm_bwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);
+}
