@@ -199,13 +199,18 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     p.dbias = fptr(dbias);
     p.h0 = fptr(h0);
     p.lens = ptr(lens);
-    p.u_b = u.stride(0); p.u_t = u.stride(1);
-    p.d_b = delta.stride(0); p.d_t = delta.stride(1);
-    p.B_b = Bm.stride(0); p.B_t = Bm.stride(1); p.B_g = Bm.stride(2);
-    p.C_b = Cm.stride(0); p.C_t = Cm.stride(1); p.C_g = Cm.stride(2);
+    auto step = [](const Tensor& t) {
+        if (t.size(1) < 2) return 0;
+        TORCH_CHECK(t.stride(1) <= INT_MAX, "the stride between tokens must be below 2^31");
+        return (int)t.stride(1);
+    };
+    p.u_b = u.stride(0); p.u_t = step(u);
+    p.d_b = delta.stride(0); p.d_t = step(delta);
+    p.B_b = Bm.stride(0); p.B_t = step(Bm); p.B_g = Bm.stride(2);
+    p.C_b = Cm.stride(0); p.C_t = step(Cm); p.C_g = Cm.stride(2);
     p.B = (int)B; p.L = (int)L; p.D = (int)D; p.N = (int)N; p.G = (int)G;
     p.softplus = softplus ? 1 : 0;
-    p.bvec = aligned(Bm, 16) && aligned(Cm, 16);
+    p.bvec = aligned(Bm, 4) && aligned(Cm, 4);
     return p;
 }
 
@@ -216,14 +221,22 @@ std::vector<Tensor> selective_scan_fwd(Tensor u, Tensor delta, Tensor A, Tensor 
     auto p = scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus);
     auto y = torch::empty({p.B, p.L, p.D}, u.options());
     auto h1 = want_state ? empty_f32(u, {p.B, p.D, p.N}) : Tensor();
-    const long chunks = (p.L + scan_chunk() - 1) / scan_chunk();
-    // one chunk starts from the state given: nothing to keep
-    auto ck = train && chunks > 1 ? empty_f32(u, {p.B, chunks, p.D, p.N}) : Tensor();
+    Tensor ck, seg_h, seg_s;
     if (p.B && p.D && (p.L || want_state)) {
+        const ScanPlan l = scan_plan(p, f32(u));
+        const long tasks = l.groups * p.G * l.cb;
+        // one chunk starts from the state given: nothing to keep
+        if (train && l.chunks > 1) ck = empty_f32(u, {tasks, l.chunks, l.state});
+        if (l.nseg > 1) {
+            seg_h = empty_f32(u, {tasks, l.nseg, l.state});
+            seg_s = empty_f32(u, {tasks, l.nseg, 64});
+            p.seg_h = seg_h.data_ptr<float>();
+            p.seg_s = seg_s.data_ptr<float>();
+        }
         p.y = y.data_ptr();
         p.h1 = want_state ? h1.data_ptr<float>() : nullptr;
         p.ckpt = ck.defined() ? ck.data_ptr<float>() : nullptr;
-        scan_fwd_launch(p, f32(u), stream());
+        scan_fwd_launch(p, l, f32(u), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return {y, h1, ck};
@@ -236,11 +249,8 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     at::DeviceGuard guard(u.device());
     auto p = scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus);
     const long B = p.B, L = p.L, D = p.D, N = p.N, G = p.G;
-    const long chunks = (L + scan_chunk() - 1) / scan_chunk();
     check_like(dy, u, {B, L, D}, "dy");
     check_f32(dh1, u, {B, D, N}, "dstate");
-    check_f32(ck, u, {B, chunks, D, N}, "chunk states");
-    TORCH_CHECK(has(ck) || chunks <= 1, "the forward kept no chunk states");
     auto du = torch::empty({B, L, D}, u.options());
     auto dd = torch::empty({B, L, D}, u.options());
     auto dB = torch::empty({B, L, G, N}, u.options());
@@ -251,12 +261,24 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
                                    s.narrow(0, D * N + D, D), dh0};
     };
     if (!B || !D) return split(torch::zeros({D * (N + 2)}, A.options()));
-    p.slots = scan_bwd_slots(B, D, G, N);
-    const long cb = scan_cblocks(D, G, N);
-    auto ws = empty_f32(u, {p.slots, D * (N + 2)});
+    const ScanPlan l = scan_plan(p, f32(u));
+    const long tasks = l.groups * G * l.cb;
+    if (l.chunks > 1) {
+        TORCH_CHECK(has(ck), "the forward kept no chunk states");
+        check_f32(ck, u, {tasks, l.chunks, l.state}, "chunk states");
+    }
+    auto ws = empty_f32(u, {l.slots, D * (N + 2)});
     auto sums = empty_f32(u, {D * (N + 2)});
-    auto dbc = empty_f32(u, {cb, B, L, G, 2, N});
-    p.dy = ptr(dy);
+    auto dbc = empty_f32(u, {l.cb, B, L, G, 2, N});
+    Tensor seg_h, seg_s;
+    if (l.nseg > 1) {
+        seg_h = empty_f32(u, {tasks, l.nseg, l.state});
+        seg_s = empty_f32(u, {tasks, l.nseg, 64});
+        p.seg_h = seg_h.data_ptr<float>();
+        p.seg_s = seg_s.data_ptr<float>();
+    }
+    const Tensor dyt = has(dy) ? *dy : torch::zeros({B, L, D}, u.options());
+    p.dy = dyt.data_ptr();
     p.dh1 = fptr(dh1);
     p.du = du.data_ptr();
     p.ddelta = dd.data_ptr();
@@ -264,9 +286,9 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     p.dbc = dbc.data_ptr<float>();
     p.ws = ws.data_ptr<float>();
     p.dh0 = want_state ? dh0.data_ptr<float>() : nullptr;
-    scan_bwd_launch(p, f32(u), stream());
-    seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, D * (N + 2), stream());
-    if (L) scan_bc_reduce_launch(p.dbc, dB.data_ptr(), dC.data_ptr(), cb, B * L * G, p.N, f32(u), stream());
+    scan_bwd_launch(p, l, f32(u), stream());
+    seq_colsum_launch(p.ws, sums.data_ptr<float>(), l.slots, D * (N + 2), stream());
+    if (L) scan_bc_reduce_launch(p.dbc, dB.data_ptr(), dC.data_ptr(), l.cb, B * L * G, p.N, f32(u), stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return split(sums);
 }

@@ -209,19 +209,32 @@ struct ScanParams {
     const void* lens;    // (B,) or null
     void* y;             // (B, L, D) contiguous
     float* h1;           // (B, D, N) final state, or null
-    float* ckpt;         // (B, chunks, D, N) state entering every chunk, or null
+    float* ckpt;         // (tasks, chunks, state) state entering every chunk, or null
+    float* seg_h;        // (tasks, nseg, state) a segment's own end state, then its start's
+    float* seg_s;        // (tasks, nseg, 64) its summed step sizes
     // backward
-    const void* dy;      // (B, L, D) contiguous, or null (zeros)
+    const void* dy;      // (B, L, D) contiguous
     const float* dh1;    // (B, D, N) or null
     void *du, *ddelta;   // (B, L, D) contiguous
     float* dbc;          // (cblocks, B, L, G, 2, N) partial dB | dC
     float* ws;           // (slots, D*N + 2*D) partial dA | dskip | dbias
     float* dh0;          // (B, D, N) or null
-    long u_b, u_t, d_b, d_t, B_b, B_t, B_g, C_b, C_t, C_g;
+    long u_b, d_b, B_b, B_g, C_b, C_g;
+    int u_t, d_t, B_t, C_t;  // under 2^31 (checked)
     int B, L, D, N, G;
     int softplus, lens64;
-    int bvec;            // rows of Bm/Cm can be read 16 bytes at a time
-    int slots;
+    int bvec;            // rows of Bm/Cm are aligned for four states at a time
+};
+
+// How a scan is laid over the card. A task is one wave's channels and
+// sequences: channel block, group, group of sequences, the first fastest.
+struct ScanPlan {
+    int cw, rw, cb;      // channels and sequences a wave, channel blocks a group
+    long groups;         // groups of rw sequences
+    int chunks;          // of 8 steps
+    int nseg, seg_chunks;
+    int state;           // floats of a task's state
+    int fslots, slots;   // waves that share the same channels, forward and backward
 };
 
 struct ScanStepParams {
@@ -267,11 +280,9 @@ void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
 void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out, const float* w,
                             const float* bias, void* y, long B, int D, int K, int silu, int is_f32,
                             int vec, hipStream_t s);
-int scan_chunk();
-int scan_cblocks(long D, long G, long N);
-int scan_bwd_slots(long B, long D, long G, long N);
-void scan_fwd_launch(const ScanParams& p, int is_f32, hipStream_t s);
-void scan_bwd_launch(const ScanParams& p, int is_f32, hipStream_t s);
+ScanPlan scan_plan(const ScanParams& p, int is_f32);
+void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
+void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bc_reduce_launch(const float* dbc, void* dB, void* dC, long cblocks, long rows, int N,
                            int is_f32, hipStream_t s);
 void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s);
