@@ -23,7 +23,8 @@
 // sequences of a wave lie too far apart for that a wave takes one sequence.
 #include "seq.hpp"
 
-#define SCAN_CH 8  // steps loaded at a time; the backward holds their states
+#define SCAN_CH 8  // steps of a chunk: the backward holds their states
+#define SCAN_PF 4  // steps that loads run ahead in the forward
 
 namespace {
 
@@ -145,10 +146,16 @@ struct Place {
     __device__ __forceinline__ bool state(const ScanParams& p, int c, int i) const { return c < nd && n0 + i < p.N; }
 };
 
+// A uniform base and a lane's bytes from there. The offset is kept from being
+// widened outside the loops: the load then adds the two by itself.
+__device__ __forceinline__ unsigned here(unsigned off) {
+    asm volatile("" : "+v"(off));
+    return off;
+}
 template <typename T>
-__device__ __forceinline__ T at(const T* base, unsigned off) { return *(const T*)((const char*)base + off); }
+__device__ __forceinline__ T at(const T* base, unsigned off) { return *(const T*)((const char*)base + here(off)); }
 template <typename T>
-__device__ __forceinline__ void put(T* base, unsigned off, T v) { *(T*)((char*)base + off) = v; }
+__device__ __forceinline__ void put(T* base, unsigned off, T v) { *(T*)((char*)base + here(off)) = v; }
 
 template <typename T, int NQ>
 struct alignas(NQ * sizeof(T) < 16 ? NQ * sizeof(T) : 16) Row { T v[NQ]; };
@@ -157,7 +164,7 @@ struct alignas(NQ * sizeof(T) < 16 ? NQ * sizeof(T) : 16) Row { T v[NQ]; };
 template <typename T, int NQ, bool VB>
 __device__ __forceinline__ Row<T, NQ> row_at(const T* base, unsigned off, int n) {
     if constexpr (VB) {
-        return *(const Row<T, NQ>*)((const char*)base + off);
+        return *(const Row<T, NQ>*)((const char*)base + here(off));
     } else {
         Row<T, NQ> r;
 #pragma unroll
@@ -333,11 +340,11 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanParams p, ScanPlan l)
     const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
 
     const int nseg = MAIN ? l.nseg : l.nseg - 1;  // the last segment's end is no start
-    const long items = l.groups * nseg;
-    for (long it = slot; it < items; it += l.fslots) {
-        const int seg = (int)(it % nseg);
-        const long grp = it / nseg, b0 = grp * l.rw;
-        const long id = (grp * p.G + g) * l.cb + cblk;
+    const int items = (int)(l.groups * nseg);
+    for (int it = slot; it < items; it += l.fslots) {
+        const int seg = it % nseg, grp = it / nseg;
+        const long b0 = (long)grp * l.rw;
+        const long id = ((long)grp * p.G + g) * l.cb + cblk;
         const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
         f32x4 h[NQ];
         load_states<NQ>(p, q, MAIN && l.nseg == 1 ? p.h0 : nullptr, h);
@@ -348,36 +355,43 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanParams p, ScanPlan l)
         if (t0 < t1) {
             Walk<T, NQ, KQ, VB> in(p, q, g, b0, t0);
             T* y = (T*)p.y + (b0 * p.L + t0) * p.D;
-            // two steps ahead of the arithmetic
-            Step<T, NQ> s0 = in.template read<true, false, true, MAIN>();
-            in.forth(p);
-            Step<T, NQ> s1 = in.template read<true, false, true, MAIN>();
-#pragma unroll 4
-            for (int t = t0; t < t1; ++t, y += p.D) {
-                const Step<T, NQ> cur = s0;
-                s0 = s1;
+            // SCAN_PF steps ahead of the arithmetic
+            Step<T, NQ> ring[SCAN_PF];
+#pragma unroll
+            for (int j = 0; j < SCAN_PF; ++j) {
+                ring[j] = in.template read<true, false, true, MAIN>();
                 in.forth(p);
-                s1 = in.template read<true, false, true, MAIN>();
-                if (MAIN && p.ckpt && t % SCAN_CH == 0) store_lanes<NQ>(p.ckpt, id * l.chunks + t / SCAN_CH, lane, h);
-                const bool on = t < q.len;
-                const float dt = step_size(p, on, to_f32(cur.de) + dbias);
-                const float uv = on ? to_f32(cur.u) : 0.f;
-                float dts[4], dus[4], Bv[NQ], Cv[NQ], acc[4] = {};
-                quad_spread(dt, dts);
-                quad_spread(dt * uv, dus);
-                widen<T, NQ>(cur.B, t < q.slen, Bv);
-                if (MAIN) widen<T, NQ>(cur.C, t < q.slen, Cv);
-                else total += dt;
+            }
+            for (int tc = t0; tc < t1; tc += SCAN_CH) {
+                if (MAIN && p.ckpt) store_lanes<NQ>(p.ckpt, id * l.chunks + tc / SCAN_CH, lane, h);
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int j = 0; j < SCAN_CH; ++j) {
+                    const int t = tc + j;
+                    if (t >= t1) break;
+                    const Step<T, NQ> cur = ring[j % SCAN_PF];
+                    const bool on = t < q.len;
+                    const float x = to_f32(cur.de) + dbias, uv = on ? to_f32(cur.u) : 0.f;
+                    float dts[4], dus[4], Bv[NQ], Cv[NQ], acc[4] = {};
+                    widen<T, NQ>(cur.B, t < q.slen, Bv);
+                    if (MAIN) widen<T, NQ>(cur.C, t < q.slen, Cv);
+                    ring[j % SCAN_PF] = in.template read<true, false, true, MAIN>();
+                    in.forth(p);
+                    const float dt = step_size(p, on, x);
+                    quad_spread(dt, dts);
+                    quad_spread(dt * uv, dus);
+                    if (!MAIN) total += dt;
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-                        h[i][c] = fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), h[i][c], dus[c] * Bv[i]);
-                        if (MAIN) acc[c] = fmaf(Cv[i], h[i][c], acc[c]);
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) {
+                            h[i][c] = fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), h[i][c], dus[c] * Bv[i]);
+                            if (MAIN) acc[c] = fmaf(Cv[i], h[i][c], acc[c]);
+                        }
+                    if (MAIN) {
+                        const float s = states_sum<KQ>(acc, lane);
+                        if (q.own) put(y, in.oy, from_f32<T>(on ? fmaf(skip, uv, s) : 0.f));
+                        y += p.D;
                     }
-                if (MAIN) {
-                    const float s = states_sum<KQ>(acc, lane);
-                    if (q.own) put(y, in.oy, from_f32<T>(on ? fmaf(skip, uv, s) : 0.f));
                 }
             }
         }
@@ -458,11 +472,11 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanParams p, ScanPla
     f32x4 A2[NQ];
     load_decay<NQ, KQ>(p, q0, A2);
     const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
-    const long items = l.groups * (l.nseg - 1);
-    for (long it = slot; it < items; it += l.fslots) {
-        const int seg = (int)(it % (l.nseg - 1)) + 1;
-        const long grp = it / (l.nseg - 1), b0 = grp * l.rw;
-        const long id = (grp * p.G + g) * l.cb + cblk;
+    const int items = (int)(l.groups * (l.nseg - 1));
+    for (int it = slot; it < items; it += l.fslots) {
+        const int seg = it % (l.nseg - 1) + 1, grp = it / (l.nseg - 1);
+        const long b0 = (long)grp * l.rw;
+        const long id = ((long)grp * p.G + g) * l.cb + cblk;
         const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
         f32x4 gs[NQ];
 #pragma unroll
@@ -471,27 +485,34 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanParams p, ScanPla
         const int t0 = seg * l.seg_chunks * SCAN_CH;
         const int t1 = t0 + l.seg_chunks * SCAN_CH < p.L ? t0 + l.seg_chunks * SCAN_CH : p.L;
         Walk<T, NQ, KQ, VB> in(p, q, g, b0, t1 - 1);
-        Step<T, NQ> s0 = in.template read<false, true, false, true>();
-        in.back(p, t1 - 1);
-        Step<T, NQ> s1 = in.template read<false, true, false, true>();
-#pragma unroll 4
-        for (int t = t1 - 1; t >= t0; --t) {
-            const Step<T, NQ> cur = s0;
-            s0 = s1;
-            in.back(p, t - 1);
-            s1 = in.template read<false, true, false, true>();
-            const bool on = t < q.len;
-            const float dt = step_size(p, on, to_f32(cur.de) + dbias);
-            float dts[4], dys[4], Cv[NQ];
-            quad_spread(dt, dts);
-            quad_spread(on ? to_f32(cur.dy) : 0.f, dys);
-            widen<T, NQ>(cur.C, t < q.slen, Cv);
-            total += dt;
+        Step<T, NQ> ring[SCAN_PF];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+        for (int j = 0; j < SCAN_PF; ++j) {
+            ring[j] = in.template read<false, true, false, true>();
+            in.back(p, t1 - 1 - j);
+        }
+        for (int tc = t1 - 1; tc >= t0; tc -= SCAN_PF) {
 #pragma unroll
-                for (int i = 0; i < NQ; ++i)
-                    gs[i][c] = fmaf(Cv[i], dys[c], gs[i][c]) * __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
+            for (int j = 0; j < SCAN_PF; ++j) {
+                const int t = tc - j;
+                if (t < t0) break;
+                const Step<T, NQ> cur = ring[j];
+                const bool on = t < q.len;
+                const float x = to_f32(cur.de) + dbias, dyv = on ? to_f32(cur.dy) : 0.f;
+                float dts[4], dys[4], Cv[NQ];
+                widen<T, NQ>(cur.C, t < q.slen, Cv);
+                ring[j] = in.template read<false, true, false, true>();
+                in.back(p, t - SCAN_PF);
+                const float dt = step_size(p, on, x);
+                quad_spread(dt, dts);
+                quad_spread(dyv, dys);
+                total += dt;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i)
+                        gs[i][c] = fmaf(Cv[i], dys[c], gs[i][c]) * __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
+            }
         }
         store_lanes<NQ>(p.seg_h, id * l.nseg + seg, lane, gs);
         p.seg_s[(id * l.nseg + seg) * 64 + lane] = total;
@@ -514,17 +535,17 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanParams p, ScanPlan
     for (int i = 0; i < NQ; ++i) dA[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float skip = p.skip ? p.skip[q0.d] : 0.f;
     const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
-    int idx, dup, left;  // left > 1 leaves no duplicates
+    int idx, dup, left;  // one value a lane is left, or two and no duplicates
     reduced_place<2 * NQ, 4 * KQ>(l.cw * KQ, lane, idx, dup, left);
     const int n1 = q0.n0 + (idx & (NQ - 1));  // the first state whose dB or dC this lane stores
 
-    const long items = l.groups * l.nseg;
-    for (long it = slot; it < items; it += l.slots) {
-        const int seg = (int)(it % l.nseg);
-        const long grp = it / l.nseg, b0 = grp * l.rw;
-        const long id = (grp * p.G + g) * l.cb + cblk;
+    const int items = (int)(l.groups * l.nseg);
+    for (int it = slot; it < items; it += l.slots) {
+        const int seg = it % l.nseg, grp = it / l.nseg;
+        const long b0 = (long)grp * l.rw;
+        const long id = ((long)grp * p.G + g) * l.cb + cblk;
         const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
-        const bool keeps = q.okb && !(lane & dup) && n1 < N;
+        const bool keeps = q.okb && !(lane & dup) && n1 < N, keeps2 = q.okb && n1 + 1 < N;
         const unsigned obc = (unsigned)(((long)q.rs * p.L * p.G * 2 * N + (idx >= NQ ? N : 0) + n1) * sizeof(float));
 
         f32x4 gs[NQ];
@@ -614,14 +635,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanParams p, ScanPlan
                         put(dde, in.oy, from_f32<T>(dx));
                     }
                     if (keeps) put(o, obc, bc[0]);
-                    if (left > 1) {  // fewer quads than values
-                        int m1 = n1;
-                        asm volatile("" : "+v"(m1));
-#pragma unroll
-                        for (int i = 1; i < 2 * NQ; ++i)
-                            if (i < left && q.okb && m1 + (i & (NQ - 1)) < N)
-                                put(o + (i < NQ ? i : N + i - NQ), obc, bc[i]);
-                    }
+                    if (left > 1 && keeps2) put(o + 1, obc, bc[1]);
                 }
                 du -= D;
                 dde -= D;
@@ -805,14 +819,14 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32) {
     const int kq = p.N <= 16 ? 1 : p.N <= 32 ? 2 : 4, nq = p.N <= 4 ? 1 : p.N <= 8 ? 2 : 4;
     const long es = is_f32 ? 4 : 2, per = p.D / p.G;
     ScanPlan l{};
+    // All lanes, or the half of them that leaves the backward's sums over
+    // channels one value a lane: two sequences a wave where a group has 32
+    // channels or fewer and their lane offsets fit 32 bits.
     l.cw = 64 / kq;
-    if (pow2_ceil(per) < l.cw) {
-        l.cw = pow2_ceil(per) < 4 ? 4 : pow2_ceil(per);
-        // the lane offsets between a wave's sequences have 32 bits
+    if (kq == 1 && per <= 32) {
         long far = (long)p.L * p.D, bc = (long)p.L * p.G * 2 * p.N * 4;
         for (long s : {p.u_b, p.d_b, p.B_b, p.C_b}) far = s > far ? s : far;
-        const long more = 64 / (l.cw * kq) - 1;
-        if (more * far * es + (p.D + 64L) * es > 0xffffffffL || more * bc + 1024 > 0xffffffffL) l.cw = 64 / kq;
+        if ((far + p.D + 64L) * es <= 0xffffffffL && bc + 1024 <= 0xffffffffL) l.cw = 32;
     }
     l.rw = 64 / (l.cw * kq);
     l.cb = (int)((per + l.cw - 1) / l.cw);
