@@ -201,7 +201,7 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     p.lens = ptr(lens);
     auto step = [](const Tensor& t) {
         if (t.size(1) < 2) return 0;
-        TORCH_CHECK(t.stride(1) <= INT_MAX, "the stride between tokens must be below 2^31");
+        TORCH_CHECK(t.stride(1) < (1L << 26), "the stride between tokens must be below 2^26 elements");
         return (int)t.stride(1);
     };
     p.u_b = u.stride(0); p.u_t = step(u);
@@ -210,7 +210,8 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     p.C_b = Cm.stride(0); p.C_t = step(Cm); p.C_g = Cm.stride(2);
     p.B = (int)B; p.L = (int)L; p.D = (int)D; p.N = (int)N; p.G = (int)G;
     p.softplus = softplus ? 1 : 0;
-    p.bvec = aligned(Bm, 4) && aligned(Cm, 4);
+    p.rvec = D / G % 8 == 0 && aligned(u, 8) && aligned(delta, 8) && aligned(Bm, 8) && aligned(Cm, 8);
+    p.svec = aligned(h0, 4);
     return p;
 }
 
@@ -269,7 +270,7 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     }
     auto ws = empty_f32(u, {l.slots, D * (N + 2)});
     auto sums = empty_f32(u, {D * (N + 2)});
-    auto dbc = empty_f32(u, {l.cb, B, L, G, 2, N});
+    auto dbc = empty_f32(u, {l.cb, B, G, l.chunks, 8, 2, l.state / (4 * l.cw * l.rw) * 4});
     Tensor seg_h, seg_s;
     if (l.nseg > 1) {
         seg_h = empty_f32(u, {tasks, l.nseg, l.state});
@@ -280,6 +281,8 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     const Tensor dyt = has(dy) ? *dy : torch::zeros({B, L, D}, u.options());
     p.dy = dyt.data_ptr();
     p.dh1 = fptr(dh1);
+    p.svec = p.svec && aligned(dh1, 4);
+    p.rvec = p.rvec && aligned(dyt, 8);
     p.du = du.data_ptr();
     p.ddelta = dd.data_ptr();
     p.ckpt = has(ck) ? ck->data_ptr<float>() : nullptr;
@@ -288,7 +291,7 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     p.dh0 = want_state ? dh0.data_ptr<float>() : nullptr;
     scan_bwd_launch(p, l, f32(u), stream());
     seq_colsum_launch(p.ws, sums.data_ptr<float>(), l.slots, D * (N + 2), stream());
-    if (L) scan_bc_reduce_launch(p.dbc, dB.data_ptr(), dC.data_ptr(), l.cb, B * L * G, p.N, f32(u), stream());
+    if (L) scan_bc_reduce_launch(p, l, dB.data_ptr(), dC.data_ptr(), f32(u), stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return split(sums);
 }

@@ -216,14 +216,15 @@ struct ScanParams {
     const void* dy;      // (B, L, D) contiguous
     const float* dh1;    // (B, D, N) or null
     void *du, *ddelta;   // (B, L, D) contiguous
-    float* dbc;          // (cblocks, B, L, G, 2, N) partial dB | dC
+    float* dbc;          // (cblocks, B, G, chunks, 8, 2, N padded) partial dB | dC
     float* ws;           // (slots, D*N + 2*D) partial dA | dskip | dbias
     float* dh0;          // (B, D, N) or null
     long u_b, d_b, B_b, B_g, C_b, C_g;
-    int u_t, d_t, B_t, C_t;  // under 2^31 (checked)
+    int u_t, d_t, B_t, C_t;  // under 2^26 (checked: 8 of them are a lane's offset)
     int B, L, D, N, G;
     int softplus, lens64;
-    int bvec;            // rows of Bm/Cm are aligned for four states at a time
+    int rvec;            // 16-byte pieces of u, delta, Bm, Cm are whole and aligned
+    int svec;            // and of h0, dh1
 };
 
 // How a scan is laid over the card. A task is one wave's channels and
@@ -283,8 +284,7 @@ void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_o
 ScanPlan scan_plan(const ScanParams& p, int is_f32);
 void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
-void scan_bc_reduce_launch(const float* dbc, void* dB, void* dC, long cblocks, long rows, int N,
-                           int is_f32, hipStream_t s);
+void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32, hipStream_t s);
 void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s);
 int block_norm_slots(long R, long D);
 void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);

@@ -23,8 +23,7 @@
 // sequences of a wave lie too far apart for that a wave takes one sequence.
 #include "seq.hpp"
 
-#define SCAN_CH 8  // steps of a chunk: the backward holds their states
-#define SCAN_PF 4  // steps that loads run ahead in the forward
+#define SCAN_CH 8  // steps of a chunk: staged together, their states held by the backward
 
 namespace {
 
@@ -116,99 +115,60 @@ __device__ __forceinline__ void reduced_place(int span, int lane, int& idx, int&
 
 // ---- a lane's place ---------------------------------------------------------
 
-template <typename T, int NQ, int KQ>
+// Where a lane stands in its wave: its sequence, the channel it loads and
+// stores, the four channels and NQ states it computes.
+template <int NQ, int KQ>
 struct Place {
-    int lane, rs, b, d, n0;   // sequence in the wave, sequence, own channel, first state
-    int d4, nd;               // the quad's first channel, how many of its four there are
-    bool okb, ok, own;        // the sequence exists; and the channel; and this lane stores it
-    int slen, len;            // valid steps of the sequence, of the own channel (0: no such channel)
+    static constexpr int CH = 64 / KQ;       // channels of a wave, over its sequences
+    static constexpr int NP = 4 * NQ * KQ;   // states, padded
+    int rs, col, d, n0, d4, nd;
+    bool okc;
 
-    __device__ __forceinline__ Place(const ScanParams& p, const ScanPlan& l, int lane_, int g, int cblk, long b0) {
-        lane = lane_;
+    __device__ __forceinline__ Place(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk) {
         const int per = p.D / p.G;
         const int quad = (lane / (4 * KQ)) & (l.cw / 4 - 1);
         const int kq = (lane >> 2) & (KQ - 1);
         rs = lane / (l.cw * KQ);
-        okb = b0 + rs < p.B;
-        rs = okb ? rs : 0;
-        b = (int)b0 + rs;
         const int c4 = cblk * l.cw + quad * 4, c = c4 + (lane & 3);
+        col = rs * l.cw + quad * 4 + (lane & 3);
         nd = per - c4 < 0 ? 0 : per - c4 > 4 ? 4 : per - c4;
-        const bool okc = c < per;
+        okc = c < per;
         d = g * per + (okc ? c : 0);
         d4 = g * per + (nd ? c4 : 0);
         n0 = (kq * 4 + (lane & 3)) * NQ;
-        ok = okb && okc;
-        own = ok && kq == 0;
-        slen = okb ? seq_len(p.lens, p.lens64, b, p.L) : 0;
-        len = ok ? slen : 0;
     }
     __device__ __forceinline__ bool state(const ScanParams& p, int c, int i) const { return c < nd && n0 + i < p.N; }
 };
 
-// A uniform base and a lane's bytes from there. The offset is kept from being
-// widened outside the loops: the load then adds the two by itself.
-__device__ __forceinline__ unsigned here(unsigned off) {
-    asm volatile("" : "+v"(off));
-    return off;
-}
-template <typename T>
-__device__ __forceinline__ T at(const T* base, unsigned off) { return *(const T*)((const char*)base + here(off)); }
-template <typename T>
-__device__ __forceinline__ void put(T* base, unsigned off, T v) { *(T*)((char*)base + here(off)) = v; }
-
-template <typename T, int NQ>
-struct alignas(NQ * sizeof(T) < 16 ? NQ * sizeof(T) : 16) Row { T v[NQ]; };
-
-// NQ entries of a row of B or C; VB: all rows whole and aligned.
-template <typename T, int NQ, bool VB>
-__device__ __forceinline__ Row<T, NQ> row_at(const T* base, unsigned off, int n) {
-    if constexpr (VB) {
-        return *(const Row<T, NQ>*)((const char*)base + here(off));
-    } else {
-        Row<T, NQ> r;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) r.v[i] = i < n ? ((const T*)((const char*)base + off))[i] : (T)0.f;
-        return r;
-    }
-}
-
-// to f32; zeros where the step is past the sequence's end
-template <typename T, int NQ>
-__device__ __forceinline__ void widen(const Row<T, NQ>& r, bool on, float (&v)[NQ]) {
-    if constexpr (sizeof(r) >= 4) {
-        int w[sizeof(r) / 4];
-        __builtin_memcpy(w, &r, sizeof(r));
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(r) / 4); ++i) w[i] = on ? w[i] : 0;
-        Row<T, NQ> z;
-        __builtin_memcpy(&z, w, sizeof(r));
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) v[i] = to_f32(z.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) v[i] = on ? to_f32(r.v[i]) : 0.f;
-    }
-}
-
-// log(1 + e^x). e^-|x| with the argument's rounding put right, the logarithm of
-// 1 + e with that sum's: a few 2^-24 of the result over the whole range.
-__device__ __forceinline__ float softplus_s(float x) {
+// log(1 + e^x) and its slope. e^-|x| with the argument's rounding put right,
+// the logarithm of 1 + e with that sum's: a few 2^-24 of the result over the
+// whole range.
+__device__ __forceinline__ float softplus_s(float x, float& slope) {
     const float a = -fabsf(x), hi = a * LOG2E, lo = fmaf(a, LOG2E, -hi);
     float e = __builtin_amdgcn_exp2f(hi);
     e = fmaf(e * lo, LN2, e);
-    const float s = 1.f + e;
+    const float s = 1.f + e, r = __builtin_amdgcn_rcpf(s);
+    slope = x < 0.f ? e * r : r;
     return fmaxf(x, 0.f) + fmaf(__builtin_amdgcn_logf(s), LN2, e - (s - 1.f));
+}
+
+// the step size, 0 past the sequence's end, and its slope in delta
+__device__ __forceinline__ float step_size(bool softplus, bool on, float x, float& slope) {
+    float s = softplus_s(x, slope);
+    asm volatile("" : "+v"(s));  // no branch around it: the steps stay one block
+    s = softplus ? s : x;
+    slope = softplus ? slope : 1.f;
+    return on ? s : 0.f;
 }
 
 // s[i] where ok, else 0: read without a branch
 __device__ __forceinline__ float pick(const float* __restrict__ s, bool ok, long i) {
-    const float v = s[ok ? i : 0];
+    const float v = ((gmem<const float>)s)[ok ? i : 0];
     return ok ? v : 0.f;
 }
 
-template <int NQ, int KQ, typename P>
-__device__ __forceinline__ void load_decay(const ScanParams& p, const P& q, f32x4 (&A2)[NQ]) {
+template <int NQ, int KQ>
+__device__ __forceinline__ void load_decay(const ScanParams& p, const Place<NQ, KQ>& q, f32x4 (&A2)[NQ]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -216,191 +176,404 @@ __device__ __forceinline__ void load_decay(const ScanParams& p, const P& q, f32x
             A2[i][c] = pick(p.A, q.state(p, c, i), (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
 }
 
-// (B, D, N) states of the lane, or zeros
-template <int NQ, typename P>
-__device__ __forceinline__ void load_states(const ScanParams& p, const P& q, const float* s, f32x4 (&h)[NQ]) {
-    const bool some = s != nullptr && q.okb;
-    s = s ? s : p.A;  // anything that can be read
+// The lane's states of sequence b in a (B, D, N) tensor, or zeros. VS: a
+// channel's four are one aligned piece.
+template <bool VS, int NQ, int KQ>
+__device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ, KQ>& q, const float* s, long b,
+                                            f32x4 (&h)[NQ]) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) h[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!s) return;
     // addresses and masks are formed here, not kept over the loop around
     int d4 = q.d4, nd = q.nd, n0 = q.n0;
     asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
+    nd = b < p.B ? nd : 0;
+    s += b < p.B ? (b * p.D + d4) * p.N : 0;
+    if (VS && NQ == 4 && p.svec) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+            const f32x4 v = *(gmem<const f32x4>)(s + (c < nd ? c * p.N + n0 : 0));
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-            h[i][c] = pick(s, some && c < nd && n0 + i < p.N, ((long)q.b * p.D + d4 + c) * p.N + n0 + i);
+            for (int i = 0; i < NQ; ++i) h[i][c] = c < nd ? v[i & 3] : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, c < nd && n0 + i < p.N, (long)c * p.N + n0 + i);
+    }
 }
-template <int NQ, typename P>
-__device__ __forceinline__ void store_states(const ScanParams& p, const P& q, float* s, const f32x4 (&h)[NQ]) {
+template <bool VS, int NQ, int KQ>
+__device__ __forceinline__ void store_states(const ScanParams& p, const Place<NQ, KQ>& q, float* s, long b,
+                                             const f32x4 (&h)[NQ]) {
     int d4 = q.d4, nd = q.nd, n0 = q.n0;
     asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
+    if (b >= p.B) return;
+    s += (b * p.D + d4) * p.N + n0;
+    if (VS && NQ == 4) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+            f32x4 v;
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-            if (q.okb && c < nd && n0 + i < p.N) s[((long)q.b * p.D + d4 + c) * p.N + n0 + i] = h[i][c];
+            for (int i = 0; i < 4; ++i) v[i] = h[i & (NQ - 1)][c];
+            if (c < nd) *(gmem<f32x4>)(s + c * p.N) = v;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+                if (c < nd && n0 + i < p.N) ((gmem<float>)s)[c * p.N + i] = h[i][c];
+    }
 }
 // the same in the order of a wave's lanes: 16 bytes a lane, NQ rows of them
 template <int NQ>
 __device__ __forceinline__ void load_lanes(const float* s, long slot, int lane, f32x4 (&h)[NQ]) {
-    const f32x4* v = (const f32x4*)s + slot * NQ * 64 + lane;
+    const auto v = (gmem<const f32x4>)s + slot * NQ * 64 + lane;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) h[i] = v[i * 64];
 }
 template <int NQ>
 __device__ __forceinline__ void store_lanes(float* s, long slot, int lane, const f32x4 (&h)[NQ]) {
-    f32x4* v = (f32x4*)s + slot * NQ * 64 + lane;
+    const auto v = (gmem<f32x4>)s + slot * NQ * 64 + lane;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) v[i * 64] = h[i];
 }
 
+struct ScanArgs {
+    ScanParams p;
+    ScanPlan l;
+};
+
+// The kernel's arguments read anew from where the launch put them: kept over
+// the loops they would not fit the scalar registers.
+__device__ __forceinline__ ScanArgs args() {
+    auto k = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    int w[sizeof(ScanArgs) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(ScanArgs) / 4); ++i) w[i] = k[i];
+    ScanArgs a;
+    __builtin_memcpy(&a, w, sizeof(a));
+    return a;
+}
+
+// The lane, so that what follows from it is worked out where it is used and
+// not kept over the loops.
+__device__ __forceinline__ int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// One step's inputs as they are in memory.
-template <typename T, int NQ>
-struct Step { T u, de, dy; Row<T, NQ> B, C; };
+// ---- a chunk's inputs, by way of LDS ----------------------------------------
+//
+// A wave reads a chunk of 8 steps in 16-byte pieces, one or two a lane and
+// tensor, into registers while it works on the chunk before, and puts them into
+// LDS of its own when it gets there. B and C are widened to f32 on the way;
+// what is past a sequence's end goes in as zeros, whatever it holds. Outputs
+// take the same way back over the inputs' place. LDS operations of one wave
+// run in order, so no barrier is needed, only that the compiler keeps them so.
 
-// Walks the inputs step by step: uniform pointers that stop at the ends of the
-// sequence, so that a step past them reads what is there and counts as nothing.
-template <typename T, int NQ, int KQ, bool VB>
-struct Walk {
-    const T *u, *de, *Bm, *Cm, *dy;
-    unsigned ou, od, oB, oC, oy;  // this lane's bytes from there
-    int nB;                       // entries of a row this lane may read
-    int t;
+template <typename T, int NQ, int KQ>
+struct Tile {
+    static constexpr int CH = 64 / KQ, NP = 4 * NQ * KQ, RW = KQ == 1 ? 2 : 1;
+    T u[SCAN_CH][CH], de[SCAN_CH][CH];
+    float bc[SCAN_CH][RW][2][NP];
+};
+template <typename T, int NQ, int KQ>
+struct TileBack : Tile<T, NQ, KQ> {
+    using B = Tile<T, NQ, KQ>;
+    T dy[SCAN_CH][B::CH];
+    float step[SCAN_CH][64][2];  // step size and its slope
+    float dbc[B::RW][SCAN_CH][2][B::NP];
+};
 
-    template <typename P>
-    __device__ __forceinline__ Walk(const ScanParams& p, const P& q, int g, long b0, int t0) {
-        t = t0 < p.L ? t0 : p.L - 1;
-        u = (const T*)p.u + b0 * p.u_b + (long)t * p.u_t;
-        de = (const T*)p.delta + b0 * p.d_b + (long)t * p.d_t;
-        Bm = (const T*)p.Bm + b0 * p.B_b + g * p.B_g + (long)t * p.B_t;
-        Cm = (const T*)p.Cm + b0 * p.C_b + g * p.C_g + (long)t * p.C_t;
-        dy = (const T*)p.dy + (b0 * p.L + t) * p.D;
-        ou = (unsigned)((q.rs * p.u_b + q.d) * sizeof(T));
-        od = (unsigned)((q.rs * p.d_b + q.d) * sizeof(T));
-        nB = p.N - q.n0 < 0 ? 0 : p.N - q.n0;
-        const int n0 = nB ? q.n0 : 0;
-        oB = (unsigned)((q.rs * p.B_b + n0) * sizeof(T));
-        oC = (unsigned)((q.rs * p.C_b + n0) * sizeof(T));
-        oy = (unsigned)(((long)q.rs * p.L * p.D + q.d) * sizeof(T));
+__device__ __forceinline__ void lds_order() {
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A piece of a row, 16 bytes or a whole shorter row, n elements of it there. V: at once.
+template <typename T, int E, bool V>
+__device__ __forceinline__ void read_piece(const T* base, unsigned off, int n, T (&v)[E]) {
+    const auto s = (gmem<const T>)((gmem<const char>)base + off);
+    if constexpr (V && E * sizeof(T) == 16) {
+        *(i32x4*)v = *(gmem<const i32x4>)s;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = e < n ? s[e] : (T)0.f;
     }
-    template <bool U, bool DY, bool B, bool C>
-    __device__ __forceinline__ Step<T, NQ> read() const {
-        Step<T, NQ> s;
-        s.de = at(de, od);
-        if (U) s.u = at(u, ou);
-        if (DY) s.dy = at(dy, oy);
-        if (B) s.B = row_at<T, NQ, VB>(Bm, oB, nB);
-        if (C) s.C = row_at<T, NQ, VB>(Cm, oC, nB);
-        return s;
+}
+
+// One (8 steps) x (the wave's channels) tensor.
+template <typename T, int KQ, bool V>
+struct Rows {
+    static constexpr int CH = 64 / KQ, E = 16 / sizeof(T), PR = CH / E, P = SCAN_CH * PR;
+    static constexpr int K = (P + 63) / 64;  // pieces a lane
+    struct Raw { alignas(16) T v[K][E]; };
+
+    // piece k of the lane: its step, sequence, first channel of the tensor, elements there
+    static __device__ __forceinline__ bool piece(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk, int k,
+                                                 int& row, int& rs, int& d, int& n) {
+        const int i = k * 64 + lane;
+        row = i / PR;
+        const int col = i % PR * E;
+        rs = col >= l.cw ? 1 : 0;
+        const int per = p.D / p.G, c = cblk * l.cw + col - rs * l.cw;
+        n = per - c > E ? E : per - c;
+        d = g * per + (n > 0 ? c : 0);
+        return (P % 64 == 0 || i < P) && n > 0;
     }
-    __device__ __forceinline__ void forth(const ScanParams& p) {
-        const bool go = t + 1 < p.L;
-        t += go ? 1 : 0;
-        u += go ? p.u_t : 0;
-        de += go ? p.d_t : 0;
-        Bm += go ? p.B_t : 0;
-        Cm += go ? p.C_t : 0;
-        dy += go ? p.D : 0;
+    // base: the wave's first sequence at the chunk's first step; last: the last step there is from it
+    static __device__ __forceinline__ void read(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk,
+                                                const T* base, long b_stride, int t_stride, int last, bool two, Raw& r) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            int row, rs, d, n;
+            const bool ok = piece(p, l, lane, g, cblk, k, row, rs, d, n);
+            row = row < last ? row : last;
+            const unsigned off =
+                ((rs && two ? (unsigned)b_stride : 0u) + (unsigned)row * (unsigned)t_stride + (unsigned)d) * (unsigned)sizeof(T);
+            read_piece<T, E, V>(base, ok ? off : 0, ok ? n : 0, r.v[k]);
+        }
     }
-    __device__ __forceinline__ void back(const ScanParams& p, int from) {  // from step `from` to the one before
-        const bool go = from < p.L && from > 0;
-        u -= go ? p.u_t : 0;
-        de -= go ? p.d_t : 0;
-        Bm -= go ? p.B_t : 0;
-        Cm -= go ? p.C_t : 0;
-        dy -= go ? p.D : 0;
+    static __device__ __forceinline__ void stage(int cw, int lane, const Raw& r, int live0, int live1, T (*tile)[CH]) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = k * 64 + lane, row = i / PR;
+            const bool on = row < (i % PR * E >= cw ? live1 : live0);
+            Chunk16 c = *(const Chunk16*)r.v[k];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c.v[j] = on ? c.v[j] : 0;
+            if (P % 64 == 0 || i < P) *(Chunk16*)((T*)tile + i * E) = c;
+        }
+    }
+    // back out: rows below `rows`, of a contiguous (B, L, D) tensor
+    static __device__ __forceinline__ void write(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk, T* base,
+                                                 int rows, bool two, const T (*tile)[CH]) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            int row, rs, d, n;
+            if (!piece(p, l, lane, g, cblk, k, row, rs, d, n) || row >= rows || (rs && !two)) continue;
+            const auto o = (gmem<T>)base + ((rs ? (long)p.L : 0) + row) * p.D + d;
+            const T* s = (const T*)tile + (k * 64 + lane) * E;
+            if constexpr (V) {
+                *(gmem<i32x4>)o = *(const i32x4*)s;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e < n) o[e] = s[e];
+            }
+        }
     }
 };
 
-__device__ __forceinline__ float step_size(const ScanParams& p, bool on, float x) {
-    float s = softplus_s(x);
-    asm volatile("" : "+v"(s));  // no branch around it: the steps stay one block
-    s = p.softplus ? s : x;
-    return on ? s : 0.f;
-}
+// The chunk's rows of B or of C, to f32.
+template <typename T, int NQ, int KQ, bool V>
+struct States {
+    static constexpr int NP = 4 * NQ * KQ, RW = KQ == 1 ? 2 : 1;
+    static constexpr int E = NP * sizeof(T) < 16 ? NP : 16 / sizeof(T), PR = NP / E, P = SCAN_CH * RW * PR;
+    static constexpr int K = (P + 63) / 64;
+    struct Raw { alignas(16) T v[K][E]; };
+
+    static __device__ __forceinline__ void read(const ScanParams& p, int lane, const T* base, long b_stride, int t_stride,
+                                                int last, bool two, Raw& r) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = k * 64 + lane, e0 = i % PR * E;
+            const int rs = RW == 2 && two ? i / PR % RW : 0;
+            int row = i / (PR * RW);
+            row = row < last ? row : last;
+            const int n = p.N - e0;
+            const unsigned off = ((rs ? (unsigned)b_stride : 0u) + (unsigned)row * (unsigned)t_stride +
+                                  (unsigned)(n > 0 ? e0 : 0)) * (unsigned)sizeof(T);
+            read_piece<T, E, V>(base, off, n, r.v[k]);
+        }
+    }
+    static __device__ __forceinline__ void stage(int lane, const Raw& r, int which, int live0, int live1,
+                                                 float (*tile)[RW][2][NP]) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = k * 64 + lane, e0 = i % PR * E, rs = i / PR % RW, row = i / (PR * RW);
+            const bool on = row < (rs ? live1 : live0);
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = on ? to_f32(r.v[k][e]) : 0.f;
+            if (P % 64 == 0 || i < P) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) *(f32x4*)&tile[row][rs][which][e0 + e] = *(const f32x4*)(v + e);
+            }
+        }
+    }
+};
+
+// What a wave works on: its channels, and one item after another of sequences
+// and a segment of their time. Uniform.
+struct Work {
+    int cblk, g, slot;
+    __device__ __forceinline__ explicit Work(const ScanArgs& a) {
+        const int w = blockIdx.x * 4 + wave_id();
+        cblk = w % a.l.cb;
+        g = w / a.l.cb % a.p.G;
+        slot = w / a.l.cb / a.p.G;
+    }
+};
+struct Item {
+    int seg, c0, c1;  // its chunks
+    long b0, id;      // first sequence, task
+    int len0, len1;   // valid lengths of the sequences; 0 for one that there is not
+    bool two;
+
+    // nseg segments from number `from` on
+    __device__ __forceinline__ Item(const ScanArgs& a, const Work& w, int it, int nseg, int from) {
+        const int grp = nseg == 1 ? it : it / nseg;
+        seg = from + (nseg == 1 ? 0 : it - grp * nseg);
+        b0 = (long)grp * a.l.rw;
+        id = (long)(grp * a.p.G + w.g) * a.l.cb + w.cblk;
+        c0 = seg * a.l.seg_chunks;
+        c1 = c0 + a.l.seg_chunks < a.l.chunks ? c0 + a.l.seg_chunks : a.l.chunks;
+        two = a.l.rw == 2 && b0 + 1 < a.p.B;
+        len0 = seq_len(a.p.lens, a.p.lens64, (int)b0, a.p.L);
+        len1 = two ? seq_len(a.p.lens, a.p.lens64, (int)b0 + 1, a.p.L) : 0;
+    }
+};
+
+// A chunk's inputs on their way: of u, delta, dy, B and C those asked for.
+template <typename T, int NQ, int KQ, bool V, bool U, bool DY, bool B, bool C>
+struct Inputs {
+    using RowsT = Rows<T, KQ, V>;
+    using StatesT = States<T, NQ, KQ, V>;
+    typename RowsT::Raw u, de, dy;
+    typename StatesT::Raw Br, Cr;
+
+    __device__ __forceinline__ void read(const Work& w, const Item& m, int ck) {
+        const ScanArgs a = args();
+        const ScanParams& p = a.p;
+        const int lane = fresh_lane();
+        const long t0 = (long)ck * SCAN_CH;
+        const int last = (int)(p.L - 1 - t0);
+        if (U)
+            RowsT::read(p, a.l, lane, w.g, w.cblk, (const T*)p.u + m.b0 * p.u_b + t0 * p.u_t, p.u_b, p.u_t, last, m.two, u);
+        RowsT::read(p, a.l, lane, w.g, w.cblk, (const T*)p.delta + m.b0 * p.d_b + t0 * p.d_t, p.d_b, p.d_t, last, m.two, de);
+        if (DY)
+            RowsT::read(p, a.l, lane, w.g, w.cblk, (const T*)p.dy + (m.b0 * p.L + t0) * p.D, (long)p.L * p.D, p.D, last,
+                        m.two, dy);
+        if (B)
+            StatesT::read(p, lane, (const T*)p.Bm + m.b0 * p.B_b + w.g * p.B_g + t0 * p.B_t, p.B_b, p.B_t, last, m.two, Br);
+        if (C)
+            StatesT::read(p, lane, (const T*)p.Cm + m.b0 * p.C_b + w.g * p.C_g + t0 * p.C_t, p.C_b, p.C_t, last, m.two, Cr);
+    }
+    // dyt: where dy goes
+    template <typename Tl>
+    __device__ __forceinline__ void stage(const Item& m, int ck, int cw, Tl& tile, T (*dyt)[RowsT::CH]) {
+        const int lane = fresh_lane(), t0 = ck * SCAN_CH;
+        lds_order();
+        if (U) RowsT::stage(cw, lane, u, m.len0 - t0, m.len1 - t0, tile.u);
+        RowsT::stage(cw, lane, de, m.len0 - t0, m.len1 - t0, tile.de);
+        if (DY) RowsT::stage(cw, lane, dy, m.len0 - t0, m.len1 - t0, dyt);
+        if (B) StatesT::stage(lane, Br, 0, m.len0 - t0, m.len1 - t0, tile.bc);
+        if (C) StatesT::stage(lane, Cr, 1, m.len0 - t0, m.len1 - t0, tile.bc);
+        lds_order();
+    }
+};
 
 // ---- forward ----------------------------------------------------------------
 
 // MAIN: outputs, chunk states, final state. Otherwise the end state of a
-// segment from zero and its summed step size. A wave keeps its channels and
-// takes one (sequences, segment) after another.
-template <typename T, int NQ, int KQ, bool VB, bool MAIN>
-__launch_bounds__(256) __global__ void scan_fwd_kernel(ScanParams p, ScanPlan l) {
+// segment from zero and its summed step size.
+template <typename T, int NQ, int KQ, bool V, bool MAIN>
+__launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
+    __shared__ Tile<T, NQ, KQ> tiles[4];
+    Tile<T, NQ, KQ>& tile = tiles[wave_id()];
     const int lane = threadIdx.x & 63;
-    const int w = blockIdx.x * 4 + wave_id();
-    const int cblk = w % l.cb, g = w / l.cb % p.G, slot = w / l.cb / p.G;
-    if (slot >= l.fslots) return;
-    const Place<T, NQ, KQ> q0(p, l, lane, g, cblk, 0);
     f32x4 A2[NQ];
-    load_decay<NQ, KQ>(p, q0, A2);
-    const float skip = p.skip ? p.skip[q0.d] : 0.f;
-    const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
-
-    const int nseg = MAIN ? l.nseg : l.nseg - 1;  // the last segment's end is no start
-    const int items = (int)(l.groups * nseg);
-    for (int it = slot; it < items; it += l.fslots) {
-        const int seg = it % nseg, grp = it / nseg;
-        const long b0 = (long)grp * l.rw;
-        const long id = ((long)grp * p.G + g) * l.cb + cblk;
-        const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
+    float skip, dbias;
+    int items, nseg, step, L, cw;
+    bool softplus, keep;
+    const ScanArgs a0 = args();
+    const Work w(a0);
+    const Place<NQ, KQ> q(a0.p, a0.l, lane, w.g, w.cblk);
+    {
+        nseg = MAIN ? a0.l.nseg : a0.l.nseg - 1;  // the last segment's end is no start
+        items = (int)(a0.l.groups * nseg);
+        step = a0.l.fslots;
+        if (w.slot >= step || w.slot >= items) return;
+        L = a0.p.L;
+        cw = a0.l.cw;
+        softplus = a0.p.softplus;
+        keep = MAIN && a0.p.ckpt;
+        load_decay(a0.p, q, A2);
+        skip = a0.p.skip ? ((gmem<const float>)a0.p.skip)[q.d] : 0.f;
+        dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
+    }
+    Inputs<T, NQ, KQ, V, true, false, true, MAIN> in;
+    Item m(a0, w, w.slot, nseg, 0);
+    if (m.c0 < m.c1) in.read(w, m, m.c0);
+    for (int it = w.slot; it < items; it += step) {
+        const int len = q.okc ? (q.rs ? m.len1 : m.len0) : 0;
         f32x4 h[NQ];
-        load_states<NQ>(p, q, MAIN && l.nseg == 1 ? p.h0 : nullptr, h);
-        if (MAIN && l.nseg > 1) load_lanes<NQ>(p.seg_h, id * l.nseg + seg, lane, h);
+        {
+            const ScanArgs a = args();
+            if (MAIN && nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, h);
+            else load_states<V>(a.p, q, MAIN ? a.p.h0 : nullptr, m.b0 + q.rs, h);
+        }
         float total = 0.f;
-        const int t0 = seg * l.seg_chunks * SCAN_CH;
-        const int t1 = t0 + l.seg_chunks * SCAN_CH < p.L ? t0 + l.seg_chunks * SCAN_CH : p.L;
-        if (t0 < t1) {
-            Walk<T, NQ, KQ, VB> in(p, q, g, b0, t0);
-            T* y = (T*)p.y + (b0 * p.L + t0) * p.D;
-            // SCAN_PF steps ahead of the arithmetic
-            Step<T, NQ> ring[SCAN_PF];
-#pragma unroll
-            for (int j = 0; j < SCAN_PF; ++j) {
-                ring[j] = in.template read<true, false, true, MAIN>();
-                in.forth(p);
+        for (int ck = m.c0; ck < m.c1; ++ck) {
+            const int t0 = ck * SCAN_CH;
+            in.stage(m, ck, cw, tile, tile.u);
+            if (ck + 1 < m.c1) in.read(w, m, ck + 1);
+            else if (it + step < items) {
+                const Item n(args(), w, it + step, nseg, 0);
+                in.read(w, n, n.c0);
             }
-            for (int tc = t0; tc < t1; tc += SCAN_CH) {
-                if (MAIN && p.ckpt) store_lanes<NQ>(p.ckpt, id * l.chunks + tc / SCAN_CH, lane, h);
+            if (keep) {
+                const ScanArgs a = args();
+                store_lanes<NQ>(a.p.ckpt, m.id * a.l.chunks + ck, lane, h);
+            }
 #pragma unroll
-                for (int j = 0; j < SCAN_CH; ++j) {
-                    const int t = tc + j;
-                    if (t >= t1) break;
-                    const Step<T, NQ> cur = ring[j % SCAN_PF];
-                    const bool on = t < q.len;
-                    const float x = to_f32(cur.de) + dbias, uv = on ? to_f32(cur.u) : 0.f;
-                    float dts[4], dus[4], Bv[NQ], Cv[NQ], acc[4] = {};
-                    widen<T, NQ>(cur.B, t < q.slen, Bv);
-                    if (MAIN) widen<T, NQ>(cur.C, t < q.slen, Cv);
-                    ring[j % SCAN_PF] = in.template read<true, false, true, MAIN>();
-                    in.forth(p);
-                    const float dt = step_size(p, on, x);
-                    quad_spread(dt, dts);
-                    quad_spread(dt * uv, dus);
-                    if (!MAIN) total += dt;
+            for (int j = 0; j < SCAN_CH; ++j) {
+                if (t0 + j >= L) break;
+                const bool on = t0 + j < len;
+                const float uv = to_f32(tile.u[j][q.col]);
+                float slope, dts[4], dus[4], acc[4] = {};
+                const float dt = step_size(softplus, on, to_f32(tile.de[j][q.col]) + dbias, slope);
+                quad_spread(dt, dts);
+                quad_spread(dt * uv, dus);
+                if (!MAIN) total += dt;
+                const float* Bv = &tile.bc[j][q.rs][0][q.n0];
+                const float* Cv = &tile.bc[j][q.rs][1][q.n0];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < NQ; ++i) {
+                    const float Bi = Bv[i], Ci = MAIN ? Cv[i] : 0.f;
 #pragma unroll
-                        for (int i = 0; i < NQ; ++i) {
-                            h[i][c] = fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), h[i][c], dus[c] * Bv[i]);
-                            if (MAIN) acc[c] = fmaf(Cv[i], h[i][c], acc[c]);
-                        }
-                    if (MAIN) {
-                        const float s = states_sum<KQ>(acc, lane);
-                        if (q.own) put(y, in.oy, from_f32<T>(on ? fmaf(skip, uv, s) : 0.f));
-                        y += p.D;
+                    for (int c = 0; c < 4; ++c) {
+                        h[i][c] = fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), h[i][c], dus[c] * Bi);
+                        if (MAIN) acc[c] = fmaf(Ci, h[i][c], acc[c]);
                     }
                 }
+                if (MAIN) {
+                    const float s = states_sum<KQ>(acc, lane);
+                    tile.u[j][q.col] = from_f32<T>(on ? fmaf(skip, uv, s) : 0.f);
+                }
+            }
+            if (MAIN) {
+                const ScanArgs a = args();
+                lds_order();
+                Rows<T, KQ, V>::write(a.p, a.l, fresh_lane(), w.g, w.cblk, (T*)a.p.y + (m.b0 * L + t0) * a.p.D, L - t0,
+                                      m.two, tile.u);
             }
         }
+        const ScanArgs a = args();
         if (!MAIN) {
-            store_lanes<NQ>(p.seg_h, id * l.nseg + seg, lane, h);
-            p.seg_s[(id * l.nseg + seg) * 64 + lane] = total;
-        } else if (p.h1 && seg == l.nseg - 1) {
-            store_states<NQ>(p, q, p.h1, h);
+            store_lanes<NQ>(a.p.seg_h, m.id * a.l.nseg + m.seg, lane, h);
+            ((gmem<float>)a.p.seg_s)[(m.id * a.l.nseg + m.seg) * 64 + lane] = total;
+        } else if (a.p.h1 && m.seg == a.l.nseg - 1) {
+            store_states<V>(a.p, q, a.p.h1, m.b0 + q.rs, h);
         }
+        if (it + step < items) m = Item(a, w, it + step, nseg, 0);
     }
 }
 
@@ -414,14 +587,15 @@ __launch_bounds__(256) __global__ void scan_carry_kernel(ScanParams p, ScanPlan 
     if (w >= waves) return;
     const int i = (int)(w % NQ);
     const long id = w / NQ;
-    const Place<float, NQ, KQ> q(p, l, lane, (int)(id / l.cb % p.G), (int)(id % l.cb), id / l.cb / p.G * l.rw);
+    const Place<NQ, KQ> q(p, l, lane, (int)(id / l.cb % p.G), (int)(id % l.cb));
+    const long b = id / l.cb / p.G * l.rw + q.rs;
     const float* first = BACK ? p.dh1 : p.h0;
     f32x4 A2, carry;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const bool on = q.state(p, c, i);
         A2[c] = pick(p.A, on, (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
-        carry[c] = first ? pick(first, on && q.okb, ((long)q.b * p.D + q.d4 + c) * p.N + q.n0 + i) : 0.f;
+        carry[c] = first ? pick(first, on && b < p.B, (b * p.D + q.d4 + c) * p.N + q.n0 + i) : 0.f;
     }
     f32x4* seg_h = (f32x4*)p.seg_h + (id * l.nseg * NQ + i) * 64 + lane;
     const float* seg_s = p.seg_s + id * l.nseg * 64 + lane;
@@ -462,189 +636,202 @@ __launch_bounds__(256) __global__ void scan_carry_kernel(ScanParams p, ScanPlan 
 // one the forward kept at its start and held in registers.
 
 // The adjoint that a segment hands to the one before it, from zero at its end.
-template <typename T, int NQ, int KQ, bool VB>
-__launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanParams p, ScanPlan l) {
+template <typename T, int NQ, int KQ, bool V>
+__launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
+    __shared__ Tile<T, NQ, KQ> tiles[4];
+    Tile<T, NQ, KQ>& tile = tiles[wave_id()];
     const int lane = threadIdx.x & 63;
-    const int w = blockIdx.x * 4 + wave_id();
-    const int cblk = w % l.cb, g = w / l.cb % p.G, slot = w / l.cb / p.G;
-    if (slot >= l.fslots) return;
-    const Place<T, NQ, KQ> q0(p, l, lane, g, cblk, 0);
+    const ScanArgs a0 = args();
+    const Work w(a0);
+    const Place<NQ, KQ> q(a0.p, a0.l, lane, w.g, w.cblk);
+    const int nseg = a0.l.nseg - 1, items = (int)(a0.l.groups * nseg), step = a0.l.fslots, cw = a0.l.cw;
+    const bool softplus = a0.p.softplus;
+    if (w.slot >= step || w.slot >= items) return;
     f32x4 A2[NQ];
-    load_decay<NQ, KQ>(p, q0, A2);
-    const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
-    const int items = (int)(l.groups * (l.nseg - 1));
-    for (int it = slot; it < items; it += l.fslots) {
-        const int seg = it % (l.nseg - 1) + 1, grp = it / (l.nseg - 1);
-        const long b0 = (long)grp * l.rw;
-        const long id = ((long)grp * p.G + g) * l.cb + cblk;
-        const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
+    load_decay(a0.p, q, A2);
+    const float dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
+
+    Inputs<T, NQ, KQ, V, false, true, false, true> in;
+    Item m(a0, w, w.slot, nseg, 1);
+    in.read(w, m, m.c1 - 1);
+    for (int it = w.slot; it < items; it += step) {
+        const int len = q.okc ? (q.rs ? m.len1 : m.len0) : 0;
         f32x4 gs[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i) gs[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         float total = 0.f;
-        const int t0 = seg * l.seg_chunks * SCAN_CH;
-        const int t1 = t0 + l.seg_chunks * SCAN_CH < p.L ? t0 + l.seg_chunks * SCAN_CH : p.L;
-        Walk<T, NQ, KQ, VB> in(p, q, g, b0, t1 - 1);
-        Step<T, NQ> ring[SCAN_PF];
+        for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
+            const int t0 = ck * SCAN_CH;
+            in.stage(m, ck, cw, tile, tile.u);
+            if (ck > m.c0) in.read(w, m, ck - 1);
+            else if (it + step < items) {
+                const Item n(args(), w, it + step, nseg, 1);
+                in.read(w, n, n.c1 - 1);
+            }
 #pragma unroll
-        for (int j = 0; j < SCAN_PF; ++j) {
-            ring[j] = in.template read<false, true, false, true>();
-            in.back(p, t1 - 1 - j);
-        }
-        for (int tc = t1 - 1; tc >= t0; tc -= SCAN_PF) {
-#pragma unroll
-            for (int j = 0; j < SCAN_PF; ++j) {
-                const int t = tc - j;
-                if (t < t0) break;
-                const Step<T, NQ> cur = ring[j];
-                const bool on = t < q.len;
-                const float x = to_f32(cur.de) + dbias, dyv = on ? to_f32(cur.dy) : 0.f;
-                float dts[4], dys[4], Cv[NQ];
-                widen<T, NQ>(cur.C, t < q.slen, Cv);
-                ring[j] = in.template read<false, true, false, true>();
-                in.back(p, t - SCAN_PF);
-                const float dt = step_size(p, on, x);
+            for (int j = SCAN_CH - 1; j >= 0; --j) {
+                float slope, dts[4], dys[4];
+                const float dt = step_size(softplus, t0 + j < len, to_f32(tile.de[j][q.col]) + dbias, slope);
                 quad_spread(dt, dts);
-                quad_spread(dyv, dys);
+                quad_spread(to_f32(tile.u[j][q.col]), dys);
                 total += dt;
+                const float* Cv = &tile.bc[j][q.rs][1][q.n0];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < NQ; ++i) {
+                    const float Ci = Cv[i];
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i)
-                        gs[i][c] = fmaf(Cv[i], dys[c], gs[i][c]) * __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
+                    for (int c = 0; c < 4; ++c)
+                        gs[i][c] = fmaf(Ci, dys[c], gs[i][c]) * __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
+                }
             }
         }
-        store_lanes<NQ>(p.seg_h, id * l.nseg + seg, lane, gs);
-        p.seg_s[(id * l.nseg + seg) * 64 + lane] = total;
+        const ScanArgs a = args();
+        store_lanes<NQ>(a.p.seg_h, m.id * a.l.nseg + m.seg, lane, gs);
+        ((gmem<float>)a.p.seg_s)[(m.id * a.l.nseg + m.seg) * 64 + lane] = total;
+        if (it + step < items) m = Item(a, w, it + step, nseg, 1);
     }
 }
 
-template <typename T, int NQ, int KQ, bool VB>
-__launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanParams p, ScanPlan l) {
+template <typename T, int NQ, int KQ, bool V>
+__launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
+    using RowsT = Rows<T, KQ, V>;
+    using TileT = TileBack<T, NQ, KQ>;
+    constexpr int NP = TileT::B::NP;
+    __shared__ TileT tiles[4];
+    TileT& tile = tiles[wave_id()];
     const int lane = threadIdx.x & 63;
-    const int w = blockIdx.x * 4 + wave_id();
-    const int cblk = w % l.cb, g = w / l.cb % p.G, slot = w / l.cb / p.G;
-    if (slot >= l.slots) return;
-    const int N = p.N, D = p.D;
-    const Place<T, NQ, KQ> q0(p, l, lane, g, cblk, 0);
+    const ScanArgs a0 = args();
+    const Work w(a0);
+    const Place<NQ, KQ> q(a0.p, a0.l, lane, w.g, w.cblk);
+    const int items = (int)(a0.l.groups * a0.l.nseg), nseg = a0.l.nseg, step = a0.l.slots, L = a0.p.L, cw = a0.l.cw;
+    const bool softplus = a0.p.softplus;
+    if (w.slot >= step) return;
 
     f32x4 A2[NQ], dA[NQ];
     float dskip = 0.f, ddb = 0.f;
-    load_decay<NQ, KQ>(p, q0, A2);
+    load_decay(a0.p, q, A2);
 #pragma unroll
     for (int i = 0; i < NQ; ++i) dA[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float skip = p.skip ? p.skip[q0.d] : 0.f;
-    const float dbias = p.dbias ? p.dbias[q0.d] : 0.f;
-    int idx, dup, left;  // one value a lane is left, or two and no duplicates
-    reduced_place<2 * NQ, 4 * KQ>(l.cw * KQ, lane, idx, dup, left);
-    const int n1 = q0.n0 + (idx & (NQ - 1));  // the first state whose dB or dC this lane stores
+    const float skip = a0.p.skip ? ((gmem<const float>)a0.p.skip)[q.d] : 0.f;
+    const float dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
+    int idx, dup, keeps;  // where the sums over channels end up: one value a lane, or two
+    reduced_place<2 * NQ, 4 * KQ>(cw * KQ, lane, idx, dup, keeps);
+    const int obc = q.rs * (SCAN_CH * 2 * NP) + (idx >= NQ ? NP : 0) + q.n0 + (idx & (NQ - 1));
 
-    const int items = (int)(l.groups * l.nseg);
-    for (int it = slot; it < items; it += l.slots) {
-        const int seg = it % l.nseg, grp = it / l.nseg;
-        const long b0 = (long)grp * l.rw;
-        const long id = ((long)grp * p.G + g) * l.cb + cblk;
-        const Place<T, NQ, KQ> q(p, l, lane, g, cblk, b0);
-        const bool keeps = q.okb && !(lane & dup) && n1 < N, keeps2 = q.okb && n1 + 1 < N;
-        const unsigned obc = (unsigned)(((long)q.rs * p.L * p.G * 2 * N + (idx >= NQ ? N : 0) + n1) * sizeof(float));
-
+    Inputs<T, NQ, KQ, V, true, true, true, true> in;
+    Item m(a0, w, w.slot, nseg, 0);
+    if (m.c0 < m.c1) in.read(w, m, m.c1 - 1);
+    for (int it = w.slot; it < items; it += step) {
+        const int len = q.okc ? (q.rs ? m.len1 : m.len0) : 0;
         f32x4 gs[NQ];
-        load_states<NQ>(p, q, l.nseg == 1 ? p.dh1 : nullptr, gs);
-        if (l.nseg > 1) load_lanes<NQ>(p.seg_h, id * l.nseg + seg, lane, gs);
-
-        const int c0 = seg * l.seg_chunks;
-        const int c1 = c0 + l.seg_chunks < l.chunks ? c0 + l.seg_chunks : l.chunks;
-        for (int ck = c1 - 1; ck >= c0; --ck) {
+        {
+            const ScanArgs a = args();
+            if (nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, gs);
+            else load_states<V>(a.p, q, a.p.dh1, m.b0 + q.rs, gs);
+        }
+        for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
             const int t0 = ck * SCAN_CH;
             f32x4 hist[SCAN_CH + 1][NQ];
-            if (p.ckpt) load_lanes<NQ>(p.ckpt, id * l.chunks + ck, lane, hist[0]);
-            else load_states<NQ>(p, q, p.h0, hist[0]);
-            Walk<T, NQ, KQ, VB> in(p, q, g, b0, t0);
-            Step<T, NQ> next = in.template read<true, false, true, false>();
+            {
+                const ScanArgs a = args();
+                if (a.p.ckpt) load_lanes<NQ>(a.p.ckpt, m.id * a.l.chunks + ck, lane, hist[0]);
+                else load_states<V>(a.p, q, a.p.h0, m.b0 + q.rs, hist[0]);
+            }
+            in.stage(m, ck, cw, tile, tile.dy);
 #pragma unroll
             for (int j = 0; j < SCAN_CH; ++j) {
-                const Step<T, NQ> cur = next;
-                if (j + 1 < SCAN_CH) {
-                    in.forth(p);
-                    next = in.template read<true, false, true, false>();
-                }
-                const bool on = t0 + j < q.len;
-                const float dt = step_size(p, on, to_f32(cur.de) + dbias);
-                float dts[4], dus[4], Bv[NQ];
+                float slope, dts[4], dus[4];
+                const float dt = step_size(softplus, t0 + j < len, to_f32(tile.de[j][q.col]) + dbias, slope);
+                tile.step[j][lane][0] = dt;
+                tile.step[j][lane][1] = slope;
                 quad_spread(dt, dts);
-                quad_spread(on ? dt * to_f32(cur.u) : 0.f, dus);
-                widen<T, NQ>(cur.B, t0 + j < q.slen, Bv);
+                quad_spread(dt * to_f32(tile.u[j][q.col]), dus);
+                const float* Bv = &tile.bc[j][q.rs][0][q.n0];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < NQ; ++i) {
+                    const float Bi = Bv[i];
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i)
+                    for (int c = 0; c < 4; ++c)
                         hist[j + 1][i][c] =
-                            fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), hist[j][i][c], dus[c] * Bv[i]);
-                __builtin_amdgcn_sched_barrier(0);
+                            fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), hist[j][i][c], dus[c] * Bi);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // one step at a time: no registers for more
             }
-            // The walk back reads its inputs anew: held from the walk forward they
-            // would take the registers of the states.
-            asm volatile("" : "+v"(in.ou), "+v"(in.od), "+v"(in.oB));
-            next = in.template read<true, true, true, true>();
-            T* du = (T*)p.du + (b0 * p.L + t0 + SCAN_CH - 1) * D;
-            T* dde = (T*)p.ddelta + (b0 * p.L + t0 + SCAN_CH - 1) * D;
-            float* o = p.dbc + ((((long)cblk * p.B + b0) * p.L + t0 + SCAN_CH - 1) * p.G + g) * 2 * N;
+            lds_order();
 #pragma unroll
             for (int j = SCAN_CH - 1; j >= 0; --j) {
-                const int t = t0 + j;
-                const bool on = t < q.len;
-                const Step<T, NQ> cur = next;
-                if (j) {
-                    in.back(p, t);
-                    next = in.template read<true, true, true, true>();
+                // the next chunk's inputs, once half of the states are done with
+                if (j == SCAN_CH / 2 - 1) {
+                    if (ck > m.c0) in.read(w, m, ck - 1);
+                    else if (it + step < items) {
+                        const Item n(args(), w, it + step, nseg, 0);
+                        in.read(w, n, n.c1 - 1);
+                    }
                 }
-                const float x = to_f32(cur.de) + dbias;
-                const float dt = step_size(p, on, x);
-                const float uv = on ? to_f32(cur.u) : 0.f, dyv = on ? to_f32(cur.dy) : 0.f;
-                float dts[4], dus[4], dys[4], Bv[NQ], Cv[NQ], bc[2 * NQ] = {}, into[4] = {}, dec[4] = {};
+                if (t0 + j >= L) continue;
+                const bool on = t0 + j < len;
+                const float dt = tile.step[j][lane][0], slope = tile.step[j][lane][1];
+                const float uv = to_f32(tile.u[j][q.col]), dyv = to_f32(tile.dy[j][q.col]);
+                float dts[4], dus[4], dys[4], bc[2 * NQ] = {}, into[4] = {}, dec[4] = {};
                 quad_spread(dt, dts);
                 quad_spread(dt * uv, dus);
                 quad_spread(dyv, dys);
-                widen<T, NQ>(cur.B, t < q.slen, Bv);
-                widen<T, NQ>(cur.C, t < q.slen, Cv);
+                const float* Bv = &tile.bc[j][q.rs][0][q.n0];
+                const float* Cv = &tile.bc[j][q.rs][1][q.n0];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < NQ; ++i) {
+                    const float Bi = Bv[i], Ci = Cv[i];
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
+                    for (int c = 0; c < 4; ++c) {
                         const float a = __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
                         const float back = a * hist[j][i][c];
-                        gs[i][c] = fmaf(Cv[i], dys[c], gs[i][c]);
+                        gs[i][c] = fmaf(Ci, dys[c], gs[i][c]);
                         bc[i] = fmaf(gs[i][c], dus[c], bc[i]);
                         bc[NQ + i] = fmaf(dys[c], hist[j + 1][i][c], bc[NQ + i]);
-                        into[c] = fmaf(gs[i][c], Bv[i], into[c]);
+                        into[c] = fmaf(gs[i][c], Bi, into[c]);
                         const float gb = gs[i][c] * back;
                         dec[c] = fmaf(gb, A2[i][c], dec[c]);
                         dA[i][c] = fmaf(gb, dts[c], dA[i][c]);
                         gs[i][c] *= a;
                     }
+                }
                 const float in_n = states_sum<KQ>(into, lane);
-                float dx = fmaf(uv, in_n, states_sum<KQ>(dec, lane) * LN2);
-                if (p.softplus) dx *= fast_sigmoid(x);
+                float dx = fmaf(uv, in_n, states_sum<KQ>(dec, lane) * LN2) * slope;
                 dx = on ? dx : 0.f;
                 ddb += dx;
                 dskip = fmaf(dyv, uv, dskip);
-                reduce_quads<4 * KQ, 2 * NQ>(bc, l.cw * KQ, lane);
-                if (t < p.L) {
-                    if (q.own) {
-                        put(du, in.oy, from_f32<T>(on ? fmaf(skip, dyv, dt * in_n) : 0.f));
-                        put(dde, in.oy, from_f32<T>(dx));
-                    }
-                    if (keeps) put(o, obc, bc[0]);
-                    if (left > 1 && keeps2) put(o + 1, obc, bc[1]);
-                }
-                du -= D;
-                dde -= D;
-                o -= (long)p.G * 2 * N;
-                __builtin_amdgcn_sched_barrier(0);  // one step at a time: no registers for more
+                tile.u[j][q.col] = from_f32<T>(on ? fmaf(skip, dyv, dt * in_n) : 0.f);
+                tile.de[j][q.col] = from_f32<T>(dx);
+                reduce_quads<4 * KQ, 2 * NQ>(bc, cw * KQ, lane);
+                float* o = &tile.dbc[0][j][0][0] + obc;
+                o[0] = bc[0];
+                if (keeps > 1) o[1] = bc[1];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            lds_order();
+            const ScanArgs a = args();
+            const int ln = fresh_lane();
+            RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.du + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.u);
+            RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.ddelta + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.de);
+            const long row = (((long)w.cblk * a.p.B + m.b0) * a.p.G + w.g) * a.l.chunks + ck;
+            constexpr int PC = SCAN_CH * 2 * NP / 4;  // 16-byte pieces of a chunk
+#pragma unroll
+            for (int r = 0; r < TileT::B::RW; ++r) {
+                if (r && !m.two) break;
+                const auto o = (gmem<f32x4>)a.p.dbc + (row + (long)r * a.p.G * a.l.chunks) * PC;
+#pragma unroll
+                for (int i = 0; i < (PC + 63) / 64; ++i)
+                    if (PC % 64 == 0 || i * 64 + ln < PC) o[i * 64 + ln] = ((const f32x4*)tile.dbc[r])[i * 64 + ln];
             }
         }
-        if (p.dh0 && seg == 0) store_states<NQ>(p, q, p.dh0, gs);
+        const ScanArgs a = args();
+        if (a.p.dh0 && m.seg == 0) store_states<V>(a.p, q, a.p.dh0, m.b0 + q.rs, gs);
+        if (it + step < items) m = Item(a, w, it + step, nseg, 0);
     }
+    const ScanArgs a1 = args();
+    const ScanParams& p = a1.p;
+    const ScanPlan& l = a1.l;
+    const int N = p.N, D = p.D, slot = w.slot;
     // the wave's sequences share their channels: join them, then one row per slot
     for (int m = l.cw * KQ; m < 64; m <<= 1) {
 #pragma unroll
@@ -655,31 +842,40 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanParams p, ScanPlan
         ddb += __shfl_xor(ddb, m);
     }
     if (lane < l.cw * KQ) {
-        float* ws = p.ws + (long)slot * D * (N + 2);
+        const auto ws = (gmem<float>)p.ws + (long)slot * D * (N + 2);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
-                if (q0.state(p, c, i)) ws[(long)(q0.d4 + c) * N + q0.n0 + i] = dA[i][c];
-        if (q0.own) {
-            ws[(long)D * N + q0.d] = dskip;
-            ws[(long)D * N + D + q0.d] = ddb;
+                if (q.state(p, c, i)) ws[(long)(q.d4 + c) * N + q.n0 + i] = dA[i][c];
+        if (q.okc) {
+            ws[(long)D * N + q.d] = dskip;
+            ws[(long)D * N + D + q.d] = ddb;
         }
     }
 }
 
 // dB and dC: the channel blocks' partial sums in ascending order.
 template <typename T>
-__launch_bounds__(256) __global__ void scan_bc_reduce_kernel(const float* __restrict__ dbc,
-                                                             T* __restrict__ dB, T* __restrict__ dC,
-                                                             long cblocks, long rows, int N) {
+__launch_bounds__(256) __global__ void scan_bc_reduce_kernel(const float* __restrict__ dbc, T* __restrict__ dB,
+                                                             T* __restrict__ dC, int cblocks, long rows, int B, int L,
+                                                             int G, int N, int NP) {
+    // a thread: four padded states of one row, of dB and dC in turn
+    const int pr = 2 * NP / 4;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * 2 * N) return;
-    float s = 0.f;
-    for (long c = 0; c < cblocks; ++c) s += dbc[c * rows * 2 * N + i];
-    const long row = i / (2 * N);
-    const int n = (int)(i % (2 * N));
-    (n < N ? dB : dC)[row * N + (n < N ? n : n - N)] = from_f32<T>(s);
+    const long row = i / pr;
+    if (row >= rows) return;
+    const int k = (int)(i % pr) * 4, which = k >= NP, n0 = which ? k - NP : k;
+    const int g = (int)(row % G);
+    const long bt = row / G, b = bt / L, t = bt % L;
+    const long Lp = (L + SCAN_CH - 1) / SCAN_CH * SCAN_CH;
+    const f32x4* src = (const f32x4*)dbc + ((b * G + g) * Lp + t) * pr + k / 4;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < cblocks; ++c) s += src[(long)c * B * G * Lp * pr];
+    T* o = (which ? dC : dB) + row * N + n0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (n0 + j < N) o[j] = from_f32<T>(s[j]);
 }
 
 // One new token. Bound by the state, read and written once: 4 states (16
@@ -697,7 +893,8 @@ __launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp
     const int N = p.N;
     const float uv = to_f32(((const T*)p.u)[b * p.u_b + d]);
     float dt = to_f32(((const T*)p.delta)[b * p.d_b + d]) + (p.dbias ? p.dbias[d] : 0.f);
-    if (p.softplus) dt = softplus_s(dt);
+    float slope;
+    if (p.softplus) dt = softplus_s(dt, slope);
     const T* Bm = (const T*)p.Bm + b * p.B_b + g * p.B_g;
     const T* Cm = (const T*)p.Cm + b * p.C_b + g * p.C_g;
     const float* h = p.h + r * N;
@@ -760,10 +957,10 @@ void by_states(int N, F f) {
 template <typename F>
 struct Typed {
     F f;
-    int is_f32, bvec;
+    int is_f32;
     template <int NQ, int KQ>
     void operator()() const {
-        const bool vb = bvec && f.p.N == 4 * NQ * KQ;
+        const bool vb = f.p.rvec && f.p.N == 4 * NQ * KQ;
         if (is_f32) {
             if (vb) f.template run<float, NQ, KQ, true>();
             else f.template run<float, NQ, KQ, false>();
@@ -785,12 +982,12 @@ struct ScanFwd {
         const long tasks = l.groups * p.G * l.cb;
         if (l.nseg > 1) {
             hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, VB, false>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256),
-                               0, s, p, l);
+                               0, s, ScanArgs{p, l});
             hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, false>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
                                tasks * NQ);
         }
         hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, VB, true>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0,
-                           s, p, l);
+                           s, ScanArgs{p, l});
     }
 };
 
@@ -803,12 +1000,12 @@ struct ScanBwd {
         const long tasks = l.groups * p.G * l.cb;
         if (l.nseg > 1) {
             hipLaunchKernelGGL((scan_adjoint_kernel<T, NQ, KQ, VB>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0, s,
-                               p, l);
+                               ScanArgs{p, l});
             hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, true>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
                                tasks * NQ);
         }
-        hipLaunchKernelGGL((scan_bwd_kernel<T, NQ, KQ, VB>), wave_blocks((long)l.slots * p.G * l.cb), dim3(256), 0, s, p,
-                           l);
+        hipLaunchKernelGGL((scan_bwd_kernel<T, NQ, KQ, VB>), wave_blocks((long)l.slots * p.G * l.cb), dim3(256), 0, s,
+                           ScanArgs{p, l});
     }
 };
 
@@ -819,14 +1016,15 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32) {
     const int kq = p.N <= 16 ? 1 : p.N <= 32 ? 2 : 4, nq = p.N <= 4 ? 1 : p.N <= 8 ? 2 : 4;
     const long es = is_f32 ? 4 : 2, per = p.D / p.G;
     ScanPlan l{};
-    // All lanes, or the half of them that leaves the backward's sums over
-    // channels one value a lane: two sequences a wave where a group has 32
-    // channels or fewer and their lane offsets fit 32 bits.
+    // Two sequences a wave where a group has 32 channels or fewer and their
+    // lane offsets fit 32 bits.
     l.cw = 64 / kq;
     if (kq == 1 && per <= 32) {
-        long far = (long)p.L * p.D, bc = (long)p.L * p.G * 2 * p.N * 4;
-        for (long s : {p.u_b, p.d_b, p.B_b, p.C_b}) far = s > far ? s : far;
-        if ((far + p.D + 64L) * es <= 0xffffffffL && bc + 1024 <= 0xffffffffL) l.cw = 32;
+        long far = 0;
+        for (long s : {(long)p.L * p.D, p.u_b, p.d_b, p.B_b, p.C_b}) far = s > far ? s : far;
+        for (long s : {(long)p.D, (long)p.u_t, (long)p.d_t, (long)p.B_t, (long)p.C_t})
+            if ((far + 7 * s + p.D + 64) * es > 0xffffffffL) far = 0xffffffffL;
+        if (far < 0xffffffffL) l.cw = 32;
     }
     l.rw = 64 / (l.cw * kq);
     l.cb = (int)((per + l.cw - 1) / l.cw);
@@ -851,22 +1049,25 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32) {
 }
 
 extern "C" void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s) {
-    by_states(p.N, Typed<ScanFwd>{ScanFwd{p, l, s}, is_f32, p.bvec});
+    by_states(p.N, Typed<ScanFwd>{ScanFwd{p, l, s}, is_f32});
 }
 
 extern "C" void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s) {
-    by_states(p.N, Typed<ScanBwd>{ScanBwd{p, l, s}, is_f32, p.bvec});
+    by_states(p.N, Typed<ScanBwd>{ScanBwd{p, l, s}, is_f32});
 }
 
-extern "C" void scan_bc_reduce_launch(const float* dbc, void* dB, void* dC, long cblocks, long rows,
-                                      int N, int is_f32, hipStream_t s) {
-    const dim3 grid((unsigned)((rows * 2 * N + 255) / 256));
-    if (is_f32)
-        hipLaunchKernelGGL((scan_bc_reduce_kernel<float>), grid, dim3(256), 0, s,
-            dbc, (float*)dB, (float*)dC, cblocks, rows, N);
-    else
-        hipLaunchKernelGGL((scan_bc_reduce_kernel<__bf16>), grid, dim3(256), 0, s,
-            dbc, (__bf16*)dB, (__bf16*)dC, cblocks, rows, N);
+extern "C" void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32,
+                                      hipStream_t s) {
+    const int NP = l.state / (4 * l.cw * l.rw) * 4;
+    const long rows = (long)p.B * p.L * p.G;
+    const dim3 grid((unsigned)((rows * (2 * NP / 4) + 255) / 256));
+    if (is_f32) {
+        hipLaunchKernelGGL((scan_bc_reduce_kernel<float>), grid, dim3(256), 0, s, p.dbc, (float*)dB, (float*)dC, l.cb, rows,
+                           p.B, p.L, p.G, p.N, NP);
+    } else {
+        hipLaunchKernelGGL((scan_bc_reduce_kernel<__bf16>), grid, dim3(256), 0, s, p.dbc, (__bf16*)dB, (__bf16*)dC, l.cb,
+                           rows, p.B, p.L, p.G, p.N, NP);
+    }
 }
 
 extern "C" void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s) {

@@ -10,6 +10,12 @@
 
 #define SEQ_CH 8
 
+// Pointers that the compiler cannot trace back to the launch, named as what
+// they are: loads and stores through them are global, not generic.
+template <typename T>
+using gmem = __attribute__((address_space(1))) T*;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)[SEQ_CH]) {
     if constexpr (VEC) {
@@ -49,7 +55,7 @@ __device__ __forceinline__ void zero8(float (&v)[SEQ_CH]) {
 // Valid length of sequence b, held inside [0, L].
 __device__ __forceinline__ int seq_len(const void* lens, int is64, int b, int L) {
     if (!lens) return L;
-    const long n = is64 ? ((const long*)lens)[b] : (long)((const int*)lens)[b];
+    const long n = is64 ? ((gmem<const long>)lens)[b] : (long)((gmem<const int>)lens)[b];
     return n < 0 ? 0 : n > L ? L : (int)n;
 }
 
