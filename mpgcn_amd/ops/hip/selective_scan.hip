@@ -176,11 +176,12 @@ __device__ __forceinline__ void load_decay(const ScanParams& p, const Place<NQ, 
             A2[i][c] = pick(p.A, q.state(p, c, i), (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
 }
 
-// The lane's states of sequence b in a (B, D, N) tensor, or zeros. VS: a
-// channel's four are one aligned piece.
+// The lane's states in a (B, D, N) tensor, or zeros, for a wave whose first
+// sequence is b0. VS: a channel's four are one aligned piece.
 template <bool VS, int NQ, int KQ>
-__device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ, KQ>& q, const float* s, long b,
+__device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ, KQ>& q, const float* s, long b0,
                                             f32x4 (&h)[NQ]) {
+    const long b = b0 + q.rs;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) h[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (!s) return;
@@ -188,19 +189,22 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
     int d4 = q.d4, nd = q.nd, n0 = q.n0;
     asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
     nd = b < p.B ? nd : 0;
-    s += b < p.B ? (b * p.D + d4) * p.N : 0;
     if (VS && NQ == 4 && p.svec) {
+        // Unmasked, so that nothing waits for the loads here. VS has all four
+        // channels or none, and one there is not reads the first sequence's of
+        // the wave: states that meet only zeros and are not stored.
+        s += ((b < p.B ? b : b0) * p.D + d4) * p.N + n0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const f32x4 v = *(gmem<const f32x4>)(s + (c < nd ? c * p.N + n0 : 0));
+            const f32x4 v = *(gmem<const f32x4>)(s + (long)c * p.N);
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) h[i][c] = c < nd ? v[i & 3] : 0.f;
+            for (int i = 0; i < NQ; ++i) h[i][c] = v[i & 3];
         }
     } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, c < nd && n0 + i < p.N, (long)c * p.N + n0 + i);
+            for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, c < nd && n0 + i < p.N, (b * p.D + d4 + c) * p.N + n0 + i);
     }
 }
 template <bool VS, int NQ, int KQ>
@@ -518,7 +522,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
         {
             const ScanArgs a = args();
             if (MAIN && nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, h);
-            else load_states<V>(a.p, q, MAIN ? a.p.h0 : nullptr, m.b0 + q.rs, h);
+            else load_states<V>(a.p, q, MAIN ? a.p.h0 : nullptr, m.b0, h);
         }
         float total = 0.f;
         for (int ck = m.c0; ck < m.c1; ++ck) {
@@ -718,25 +722,32 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
     reduced_place<2 * NQ, 4 * KQ>(cw * KQ, lane, idx, dup, keeps);
     const int obc = q.rs * (SCAN_CH * 2 * NP) + (idx >= NQ ? NP : 0) + q.n0 + (idx & (NQ - 1));
 
+    // what the next chunk starts from: its inputs and the state before it
     Inputs<T, NQ, KQ, V, true, true, true, true> in;
+    f32x4 next_h[NQ];
+    auto read_h = [&](const Item& m, int ck) {
+        const ScanArgs a = args();
+        if (a.p.ckpt) load_lanes<NQ>(a.p.ckpt, m.id * a.l.chunks + ck, lane, next_h);
+        else load_states<V>(a.p, q, a.p.h0, m.b0, next_h);
+    };
     Item m(a0, w, w.slot, nseg, 0);
-    if (m.c0 < m.c1) in.read(w, m, m.c1 - 1);
+    if (m.c0 < m.c1) {
+        in.read(w, m, m.c1 - 1);
+        read_h(m, m.c1 - 1);
+    }
     for (int it = w.slot; it < items; it += step) {
         const int len = q.okc ? (q.rs ? m.len1 : m.len0) : 0;
-        f32x4 gs[NQ];
+        f32x4 gs[NQ];  // needed only after the first chunk's walk forward
         {
             const ScanArgs a = args();
             if (nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, gs);
-            else load_states<V>(a.p, q, a.p.dh1, m.b0 + q.rs, gs);
+            else load_states<V>(a.p, q, a.p.dh1, m.b0, gs);
         }
         for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
             const int t0 = ck * SCAN_CH;
-            f32x4 hist[SCAN_CH + 1][NQ];
-            {
-                const ScanArgs a = args();
-                if (a.p.ckpt) load_lanes<NQ>(a.p.ckpt, m.id * a.l.chunks + ck, lane, hist[0]);
-                else load_states<V>(a.p, q, a.p.h0, m.b0 + q.rs, hist[0]);
-            }
+            f32x4 hist[SCAN_CH][NQ];  // before every step; the state after it follows from its decay again
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) hist[0][i] = next_h[i];
             in.stage(m, ck, cw, tile, tile.dy);
 #pragma unroll
             for (int j = 0; j < SCAN_CH; ++j) {
@@ -744,6 +755,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                 const float dt = step_size(softplus, t0 + j < len, to_f32(tile.de[j][q.col]) + dbias, slope);
                 tile.step[j][lane][0] = dt;
                 tile.step[j][lane][1] = slope;
+                if (j + 1 == SCAN_CH) continue;
                 quad_spread(dt, dts);
                 quad_spread(dt * to_f32(tile.u[j][q.col]), dus);
                 const float* Bv = &tile.bc[j][q.rs][0][q.n0];
@@ -752,22 +764,14 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                     const float Bi = Bv[i];
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        hist[j + 1][i][c] =
+                        hist[(j + 1) % SCAN_CH][i][c] =
                             fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), hist[j][i][c], dus[c] * Bi);
                 }
-                __builtin_amdgcn_sched_barrier(0);  // one step at a time: no registers for more
+                __builtin_amdgcn_sched_barrier(4);  // one step at a time: no registers for more
             }
             lds_order();
 #pragma unroll
             for (int j = SCAN_CH - 1; j >= 0; --j) {
-                // the next chunk's inputs, once half of the states are done with
-                if (j == SCAN_CH / 2 - 1) {
-                    if (ck > m.c0) in.read(w, m, ck - 1);
-                    else if (it + step < items) {
-                        const Item n(args(), w, it + step, nseg, 0);
-                        in.read(w, n, n.c1 - 1);
-                    }
-                }
                 if (t0 + j >= L) continue;
                 const bool on = t0 + j < len;
                 const float dt = tile.step[j][lane][0], slope = tile.step[j][lane][1];
@@ -787,7 +791,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                         const float back = a * hist[j][i][c];
                         gs[i][c] = fmaf(Ci, dys[c], gs[i][c]);
                         bc[i] = fmaf(gs[i][c], dus[c], bc[i]);
-                        bc[NQ + i] = fmaf(dys[c], hist[j + 1][i][c], bc[NQ + i]);
+                        bc[NQ + i] = fmaf(dys[c], fmaf(dus[c], Bi, back), bc[NQ + i]);
                         into[c] = fmaf(gs[i][c], Bi, into[c]);
                         const float gb = gs[i][c] * back;
                         dec[c] = fmaf(gb, A2[i][c], dec[c]);
@@ -806,7 +810,16 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                 float* o = &tile.dbc[0][j][0][0] + obc;
                 o[0] = bc[0];
                 if (keeps > 1) o[1] = bc[1];
-                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_sched_barrier(4);
+            }
+            // the next chunk's inputs are on their way while this one's outputs leave
+            if (ck > m.c0) {
+                in.read(w, m, ck - 1);
+                read_h(m, ck - 1);
+            } else if (it + step < items) {
+                const Item n(args(), w, it + step, nseg, 0);
+                in.read(w, n, n.c1 - 1);
+                read_h(n, n.c1 - 1);
             }
             lds_order();
             const ScanArgs a = args();
