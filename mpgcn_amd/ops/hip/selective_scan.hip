@@ -293,6 +293,7 @@ struct TileBack : Tile<T, NQ, KQ> {
     T dy[SCAN_CH][B::CH];
     float step[SCAN_CH][64][2];  // step size and its slope
     float dbc[B::RW][SCAN_CH][2][B::NP];
+    f32x4 A2[NQ][64];            // the decays of the lanes, out of their registers
 };
 
 __device__ __forceinline__ void lds_order() {
@@ -711,9 +712,14 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
     const bool softplus = a0.p.softplus;
     if (w.slot >= step) return;
 
-    f32x4 A2[NQ], dA[NQ];
+    f32x4 dA[NQ];
     float dskip = 0.f, ddb = 0.f;
-    load_decay(a0.p, q, A2);
+    {
+        f32x4 A2[NQ];
+        load_decay(a0.p, q, A2);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) tile.A2[i][lane] = A2[i];
+    }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) dA[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float skip = a0.p.skip ? ((gmem<const float>)a0.p.skip)[q.d] : 0.f;
@@ -759,15 +765,17 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                 quad_spread(dt, dts);
                 quad_spread(dt * to_f32(tile.u[j][q.col]), dus);
                 const float* Bv = &tile.bc[j][q.rs][0][q.n0];
+                const int ln = fresh_lane();
 #pragma unroll
                 for (int i = 0; i < NQ; ++i) {
                     const float Bi = Bv[i];
+                    const f32x4 A2 = tile.A2[i][ln];
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         hist[(j + 1) % SCAN_CH][i][c] =
-                            fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[i][c]), hist[j][i][c], dus[c] * Bi);
+                            fmaf(__builtin_amdgcn_exp2f(dts[c] * A2[c]), hist[j][i][c], dus[c] * Bi);
                 }
-                __builtin_amdgcn_sched_barrier(4);  // one step at a time: no registers for more
+                __builtin_amdgcn_sched_barrier(260);  // one step at a time: no registers for more
             }
             lds_order();
 #pragma unroll
@@ -782,19 +790,21 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                 quad_spread(dyv, dys);
                 const float* Bv = &tile.bc[j][q.rs][0][q.n0];
                 const float* Cv = &tile.bc[j][q.rs][1][q.n0];
+                const int ln = fresh_lane();
 #pragma unroll
                 for (int i = 0; i < NQ; ++i) {
                     const float Bi = Bv[i], Ci = Cv[i];
+                    const f32x4 A2 = tile.A2[i][ln];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const float a = __builtin_amdgcn_exp2f(dts[c] * A2[i][c]);
+                        const float a = __builtin_amdgcn_exp2f(dts[c] * A2[c]);
                         const float back = a * hist[j][i][c];
                         gs[i][c] = fmaf(Ci, dys[c], gs[i][c]);
                         bc[i] = fmaf(gs[i][c], dus[c], bc[i]);
                         bc[NQ + i] = fmaf(dys[c], fmaf(dus[c], Bi, back), bc[NQ + i]);
                         into[c] = fmaf(gs[i][c], Bi, into[c]);
                         const float gb = gs[i][c] * back;
-                        dec[c] = fmaf(gb, A2[i][c], dec[c]);
+                        dec[c] = fmaf(gb, A2[c], dec[c]);
                         dA[i][c] = fmaf(gb, dts[c], dA[i][c]);
                         gs[i][c] *= a;
                     }
@@ -810,7 +820,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                 float* o = &tile.dbc[0][j][0][0] + obc;
                 o[0] = bc[0];
                 if (keeps > 1) o[1] = bc[1];
-                __builtin_amdgcn_sched_barrier(4);
+                __builtin_amdgcn_sched_barrier(260);
             }
             // the next chunk's inputs are on their way while this one's outputs leave
             if (ck > m.c0) {
