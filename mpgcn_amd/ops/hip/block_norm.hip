@@ -32,55 +32,116 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* lds, int& slot
     return s;
 }
 
+// Eight weights of a row's chunk; ones where there is no such weight.
+template <bool VEC>
 __device__ __forceinline__ void param8(const float* w, int c, int n, float (&v)[SEQ_CH]) {
 #pragma unroll
-    for (int j = 0; j < SEQ_CH; ++j) v[j] = (w && j < n) ? w[c + j] : 1.f;
+    for (int j = 0; j < SEQ_CH; ++j) v[j] = 1.f;
+    if (w && n > 0) load8<float, VEC>(w + c, n, v);
 }
 
-template <typename T, typename TR, int VPT, bool VEC>
+// Eight elements as they are in memory.
+template <typename T>
+struct alignas(16) Raw8 { T v[SEQ_CH]; };
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void raw8(const void* base, long at, int n, Raw8<T>& r) {
+    if (n <= 0) {
+#pragma unroll
+        for (int j = 0; j < SEQ_CH; ++j) r.v[j] = (T)0.f;
+        return;
+    }
+    const T* p = (const T*)base + at;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(r) / 16); ++i) ((Chunk16*)r.v)[i] = ((const Chunk16*)p)[i];
+    } else {
+#pragma unroll
+        for (int j = 0; j < SEQ_CH; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+    }
+}
+
+// The weights of a thread's columns: kept over its rows where it has one chunk,
+// else read where they are used, to leave the registers to the row.
+template <int VPT, bool VEC, bool RES>
+struct Weights {
+    static constexpr bool KEEP = VPT == 1;
+    float w[KEEP ? 3 : 1][SEQ_CH];
+
+    __device__ __forceinline__ Weights(const BlockNormParams& p, int c) {
+        if (!KEEP) return;
+        param8<VEC>(p.post, c, p.D - c, w[0]);
+        if (RES) param8<VEC>(p.scale, c, p.D - c, w[KEEP ? 1 : 0]);
+        if (RES) param8<VEC>(p.pre, c, p.D - c, w[KEEP ? 2 : 0]);
+    }
+    // which: 0 post, 1 scale, 2 pre
+    template <int WHICH>
+    __device__ __forceinline__ void get(const float* from, int c, int D, float (&v)[SEQ_CH]) const {
+        if (KEEP) {
+#pragma unroll
+            for (int j = 0; j < SEQ_CH; ++j) v[j] = w[KEEP ? WHICH : 0][j];
+        } else {
+            param8<VEC>(from, c, D - c, v);
+        }
+    }
+};
+
+// A thread keeps its columns and takes one row after another; with one chunk a
+// thread a row's loads are in flight while the row before is worked on.
+template <typename T, typename TR, int VPT, bool VEC, bool RES>
 __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, int tpr) {
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr;
     const float rd = 1.f / (float)p.D;
-    const long rounds = (p.R + (long)gridDim.x * rpb - 1) / ((long)gridDim.x * rpb);
-    for (long k = 0; k < rounds; ++k) {
-        const long r = (k * gridDim.x + blockIdx.x) * rpb + threadIdx.x / tpr;
-        const bool live = r < p.R;
-        float v[VPT][SEQ_CH], hv[VPT][SEQ_CH];
-        float ss = 0.f;
+    const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
+    long r = (long)blockIdx.x * rpb + threadIdx.x / tpr;
+
+    const Weights<VPT, VEC, RES> wt(p, lane * SEQ_CH);
+    constexpr bool AHEAD = VPT == 1;
+    Raw8<T> xr[VPT], gr[VPT];
+    Raw8<TR> rr[VPT];
+    auto read = [&](long row) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            const int n = live ? p.D - c : 0;
-            zero8(v[i]);
-            zero8(hv[i]);
-            if (n <= 0) continue;
-            load8<T, VEC>((const T*)p.x + r * p.x_r + c, n, v[i]);
-            if (p.res) load8<TR, VEC>((const TR*)p.res + r * p.r_r + c, n, hv[i]);
-            if (p.gate) {
-                float g[SEQ_CH];
-                load8<T, VEC>((const T*)p.gate + r * p.g_r + c, n, g);
-#pragma unroll
-                for (int j = 0; j < SEQ_CH; ++j) v[i][j] *= g[j] * fast_sigmoid(g[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < SEQ_CH; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+            const int n = row < p.R ? p.D - c : 0;
+            raw8<T, VEC>(p.x, row * p.x_r + c, n, xr[i]);
+            if (p.gate) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
+            if (RES) raw8<TR, VEC>(p.res, row * p.r_r + c, n, rr[i]);
         }
+    };
+    if (AHEAD) read(r);
+    for (long k = 0; k < rounds; ++k, r += stride) {
+        const bool live = r < p.R;
+        float v[VPT][SEQ_CH], hv[VPT][SEQ_CH];
+        float ss = 0.f;
+        if (!AHEAD) read(r);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int j = 0; j < SEQ_CH; ++j) {
+                v[i][j] = to_f32(xr[i].v[j]);
+                if (p.gate) {
+                    const float g = to_f32(gr[i].v[j]);
+                    v[i][j] *= g * fast_sigmoid(g);
+                }
+                if (RES) hv[i][j] = to_f32(rr[i].v[j]);
+                ss = fmaf(v[i][j], v[i][j], ss);
+            }
+        if (AHEAD && k + 1 < rounds) read(r + stride);
         if (p.post) {
             const float inv = 1.f / sqrtf(row_sum(ss, tpr, lds, slot) * rd + p.eps);
             if (live && lane == 0 && p.inv1) p.inv1[r] = inv;
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
-                const int c = (i * tpr + lane) * SEQ_CH;
-                if (c >= p.D) continue;
-                float w[SEQ_CH];
-                param8(p.post, c, p.D - c, w);
+                float w1[SEQ_CH];
+                wt.template get<0>(p.post, (i * tpr + lane) * SEQ_CH, p.D, w1);
 #pragma unroll
-                for (int j = 0; j < SEQ_CH; ++j) v[i][j] *= inv * w[j];
+                for (int j = 0; j < SEQ_CH; ++j) v[i][j] *= inv * w1[j];
             }
         }
-        if (!p.res) {
+        if (!RES) {
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * tpr + lane) * SEQ_CH;
@@ -92,15 +153,14 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (!live || c >= p.D) continue;
-            float w[SEQ_CH];
-            param8(p.scale, c, p.D - c, w);
+            float ws[SEQ_CH];
+            wt.template get<1>(p.scale, c, p.D, ws);
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                hv[i][j] = fmaf(w[j], v[i][j], hv[i][j]);
-                if (VEC || c + j < p.D) ss = fmaf(hv[i][j], hv[i][j], ss);
+                hv[i][j] = fmaf(ws[j], v[i][j], hv[i][j]);  // zeros past the row's end
+                ss = fmaf(hv[i][j], hv[i][j], ss);
             }
-            store8<TR, VEC>((TR*)p.h + r * p.D + c, p.D - c, hv[i]);
+            if (live && c < p.D) store8<TR, VEC>((TR*)p.h + r * p.D + c, p.D - c, hv[i]);
         }
         if (p.pre) {
             const float inv = 1.f / sqrtf(row_sum(ss, tpr, lds, slot) * rd + p.eps);
@@ -108,12 +168,11 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * tpr + lane) * SEQ_CH;
-                if (!live || c >= p.D) continue;
-                float w[SEQ_CH];
-                param8(p.pre, c, p.D - c, w);
+                float w2[SEQ_CH];
+                wt.template get<2>(p.pre, c, p.D, w2);
 #pragma unroll
-                for (int j = 0; j < SEQ_CH; ++j) hv[i][j] *= inv * w[j];
-                store8<T, VEC>((T*)p.y + r * p.D + c, p.D - c, hv[i]);
+                for (int j = 0; j < SEQ_CH; ++j) hv[i][j] *= inv * w2[j];
+                if (live && c < p.D) store8<T, VEC>((T*)p.y + r * p.D + c, p.D - c, hv[i]);
             }
         }
     }
@@ -126,64 +185,81 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 //   dp0 = inv1 (q - n1 mean(q n1));  dx, dgate by the product and silu'
 // Column gradients stay in registers over a thread's rows, are joined in LDS
 // over the block's row groups and written once per block.
-template <typename T, typename TR, int VPT, bool VEC>
+template <typename T, typename TR, int VPT, bool VEC, bool RES>
 __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
     extern __shared__ float dyn[];  // [rpb][VPT * tpr * SEQ_CH] when rpb > 1
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr, rg = threadIdx.x / tpr;
     const float rd = 1.f / (float)p.D;
+    const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
+    long r = (long)blockIdx.x * rpb + rg;
+
+    const Weights<VPT, VEC, RES> wt(p, lane * SEQ_CH);
+    constexpr bool AHEAD = VPT == 1;
     float dpost[VPT][SEQ_CH] = {}, dscale[VPT][SEQ_CH] = {}, dpre[VPT][SEQ_CH] = {};
-    const long rounds = (p.R + (long)gridDim.x * rpb - 1) / ((long)gridDim.x * rpb);
-    for (long k = 0; k < rounds; ++k) {
-        const long r = (k * gridDim.x + blockIdx.x) * rpb + rg;
-        const bool live = r < p.R;
-        float v[VPT][SEQ_CH], hv[VPT][SEQ_CH], d[VPT][SEQ_CH], gt[VPT][SEQ_CH], xv[VPT][SEQ_CH];
-        const float inv1 = (p.post && live) ? p.inv1[r] : 1.f;
-        const float inv2 = (p.pre && live) ? p.inv2[r] : 1.f;
-        float sum2 = 0.f;
+    Raw8<T> xr[VPT], gr[VPT], yr[VPT];
+    Raw8<TR> rr[VPT], hr[VPT];
+    float i1 = 1.f, i2 = 1.f;
+    // absent gradients count as zeros: n is 0 for them
+    auto read = [&](long row) {
+        const bool there = row < p.R;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            const int n = live ? p.D - c : 0;
-            zero8(xv[i]);
-            zero8(gt[i]);
-            zero8(v[i]);
-            zero8(hv[i]);
-            zero8(d[i]);
-            if (n <= 0) continue;
-            load8<T, VEC>((const T*)p.x + r * p.x_r + c, n, xv[i]);
-            if (p.gate) load8<T, VEC>((const T*)p.gate + r * p.g_r + c, n, gt[i]);
-            if (p.res) {
-                if (p.pre) load8<TR, VEC>((const TR*)p.res + r * p.r_r + c, n, hv[i]);
-                if (p.dh) load8<TR, VEC>((const TR*)p.dh + r * p.D + c, n, d[i]);
-            } else if (p.dy) {
-                load8<T, VEC>((const T*)p.dy + r * p.D + c, n, d[i]);
-            }
-            // v: the normed row without its weight, n1
+            const int n = there ? p.D - c : 0;
+            raw8<T, VEC>(p.x, row * p.x_r + c, n, xr[i]);
+            if (p.gate) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
+            if (!RES || p.pre) raw8<T, VEC>(p.dy, row * p.D + c, p.dy ? n : 0, yr[i]);
+            if (RES && p.pre) raw8<TR, VEC>(p.res, row * p.r_r + c, n, rr[i]);
+            if (RES) raw8<TR, VEC>(p.dh, row * p.D + c, p.dh ? n : 0, hr[i]);
+        }
+        if (p.post && there) i1 = p.inv1[row];
+        if (RES && p.pre && there) i2 = p.inv2[row];
+    };
+    if (AHEAD) read(r);
+    for (long k = 0; k < rounds; ++k, r += stride) {
+        const bool live = r < p.R;
+        // v: the normed row without its weight; d: the gradient on its way down
+        float v[VPT][SEQ_CH], d[VPT][SEQ_CH], hv[VPT][SEQ_CH], t[VPT][SEQ_CH];
+        Raw8<T> xk[VPT], gk[VPT];
+        if (!AHEAD) read(r);
+        const float inv1 = i1, inv2 = i2;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            xk[i] = xr[i];
+            gk[i] = gr[i];
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                const float sg = p.gate ? gt[i][j] * fast_sigmoid(gt[i][j]) : 1.f;
-                v[i][j] = xv[i][j] * sg * inv1;
-            }
-            if (p.pre) {
-                float wp[SEQ_CH], ws[SEQ_CH], w2[SEQ_CH], t[SEQ_CH];
-                zero8(t);
-                param8(p.post, c, n, wp);
-                param8(p.scale, c, n, ws);
-                param8(p.pre, c, n, w2);
-                if (p.dy) load8<T, VEC>((const T*)p.dy + r * p.D + c, n, t);
-#pragma unroll
-                for (int j = 0; j < SEQ_CH; ++j) {
-                    hv[i][j] = fmaf(ws[j] * wp[j], v[i][j], hv[i][j]) * inv2;  // y / pre
-                    dpre[i][j] = fmaf(t[j], hv[i][j], dpre[i][j]);
-                    t[j] *= w2[j];
-                    sum2 = fmaf(t[j], hv[i][j], sum2);
-                    d[i][j] = fmaf(inv2, t[j], d[i][j]);
+                const float g = p.gate ? to_f32(gr[i].v[j]) : 0.f;
+                const float sg = p.gate ? g * fast_sigmoid(g) : 1.f;
+                v[i][j] = to_f32(xr[i].v[j]) * sg * inv1;
+                d[i][j] = RES ? to_f32(hr[i].v[j]) : to_f32(yr[i].v[j]);
+                if (RES && p.pre) {
+                    hv[i][j] = to_f32(rr[i].v[j]);
+                    t[i][j] = to_f32(yr[i].v[j]);
                 }
             }
         }
-        if (p.pre) {
+        if (AHEAD && k + 1 < rounds) read(r + stride);
+        if (RES && p.pre) {
+            float sum2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = (i * tpr + lane) * SEQ_CH;
+                float w1[SEQ_CH], ws[SEQ_CH], w2[SEQ_CH];
+                wt.template get<0>(p.post, c, p.D, w1);
+                wt.template get<1>(p.scale, c, p.D, ws);
+                wt.template get<2>(p.pre, c, p.D, w2);
+#pragma unroll
+                for (int j = 0; j < SEQ_CH; ++j) {
+                    hv[i][j] = fmaf(ws[j] * w1[j], v[i][j], hv[i][j]) * inv2;  // y / pre
+                    dpre[i][j] = fmaf(t[i][j], hv[i][j], dpre[i][j]);
+                    t[i][j] *= w2[j];
+                    sum2 = fmaf(t[i][j], hv[i][j], sum2);
+                    d[i][j] = fmaf(inv2, t[i][j], d[i][j]);
+                }
+            }
             const float m = row_sum(sum2, tpr, lds, slot) * rd * inv2;
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
@@ -194,18 +270,18 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (!live || c >= p.D) continue;
-            const int n = p.D - c;
-            float wp[SEQ_CH], ws[SEQ_CH];
-            if (p.res) store8<TR, VEC>((TR*)p.dres + r * p.D + c, n, d[i]);
-            param8(p.post, c, n, wp);
-            param8(p.scale, c, n, ws);
+            if (RES && live && c < p.D) store8<TR, VEC>((TR*)p.dres + r * p.D + c, p.D - c, d[i]);
+            float w1[SEQ_CH], ws[SEQ_CH];
+            wt.template get<0>(p.post, c, p.D, w1);
+            if (RES) wt.template get<1>(p.scale, c, p.D, ws);
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                dscale[i][j] = fmaf(d[i][j], v[i][j] * wp[j], dscale[i][j]);
-                d[i][j] *= ws[j];
+                if (RES) {
+                    dscale[i][j] = fmaf(d[i][j], v[i][j] * w1[j], dscale[i][j]);
+                    d[i][j] *= ws[j];
+                }
                 dpost[i][j] = fmaf(d[i][j], v[i][j], dpost[i][j]);
-                d[i][j] *= wp[j];
+                d[i][j] *= w1[j];
                 sum1 = fmaf(d[i][j], v[i][j], sum1);
             }
         }
@@ -213,29 +289,26 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (!live || c >= p.D) continue;
-            const int n = p.D - c;
             float o[SEQ_CH], og[SEQ_CH];
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
                 const float dp = inv1 * fmaf(-m1, v[i][j], d[i][j]);
+                o[j] = dp;
                 if (p.gate) {
-                    const float sg = fast_sigmoid(gt[i][j]);
-                    const float si = gt[i][j] * sg;
+                    const float g = to_f32(gk[i].v[j]), sg = fast_sigmoid(g), si = g * sg;
                     o[j] = dp * si;
-                    og[j] = dp * xv[i][j] * (sg + si * (1.f - sg));
-                } else {
-                    o[j] = dp;
-                    og[j] = 0.f;
+                    og[j] = dp * to_f32(xk[i].v[j]) * (sg + si * (1.f - sg));
                 }
             }
-            store8<T, VEC>((T*)p.dx + r * p.D + c, n, o);
-            if (p.gate) store8<T, VEC>((T*)p.dgate + r * p.D + c, n, og);
+            if (live && c < p.D) {
+                store8<T, VEC>((T*)p.dx + r * p.D + c, p.D - c, o);
+                if (p.gate) store8<T, VEC>((T*)p.dgate + r * p.D + c, p.D - c, og);
+            }
         }
     }
     // column gradients of the weights there are, in the order post | scale | pre
     const int W = VPT * tpr * SEQ_CH;
-    float* ws = p.ws + (long)blockIdx.x * ((p.post != nullptr) + (p.scale != nullptr) + (p.pre != nullptr)) * p.D;
+    float* out = p.ws + (long)blockIdx.x * ((p.post != nullptr) + (p.scale != nullptr) + (p.pre != nullptr)) * p.D;
 #pragma unroll
     for (int a = 0; a < 3; ++a) {
         if (!(a == 0 ? p.post : a == 1 ? p.scale : p.pre)) continue;
@@ -251,7 +324,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             for (int c = threadIdx.x; c < p.D; c += blockDim.x) {
                 float s = 0.f;
                 for (int g = 0; g < rpb; ++g) s += dyn[g * W + c];
-                ws[c] = s;
+                out[c] = s;
             }
         } else {
 #pragma unroll
@@ -259,57 +332,62 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 #pragma unroll
                 for (int j = 0; j < SEQ_CH; ++j) {
                     const int c = (i * tpr + lane) * SEQ_CH + j;
-                    if (c < p.D) ws[c] = acc[i][j];
+                    if (c < p.D) out[c] = acc[i][j];
                 }
         }
-        ws += p.D;
+        out += p.D;
     }
 }
 
-// Threads a row, chunks a thread: one chunk each while a wave holds the row,
-// then two in as many whole waves as the row needs (to D = 8192), then four.
+// Threads a row, chunks a thread: a part of a wave while that holds the row,
+// then whole waves with one chunk a thread (to D = 4096), two, four. One chunk
+// leaves no thread of a row idle and registers for the next row's loads.
 inline void row_shape(long D, int* tpr, int* vpt) {
     const long chunks = (D + SEQ_CH - 1) / SEQ_CH;
-    *vpt = chunks <= 64 ? 1 : chunks <= 1024 ? 2 : 4;
+    *vpt = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
     *tpr = chunks <= 64 ? pow2_ceil(chunks) : (int)((chunks + 64 * *vpt - 1) / (64 * *vpt)) * 64;
 }
 
 // Whole rows in a block of about 256 threads.
 inline int block_threads(int tpr) { return tpr >= 256 ? tpr : 256 / tpr * tpr; }
 
+// Blocks that take the rows in turn: as many waves as stay on the card.
+inline long row_blocks(long R, int tpr, long waves) {
+    const int block = block_threads(tpr);
+    const long want = (R + block / tpr - 1) / (block / tpr), cap = (waves * 64 + block - 1) / block;
+    return want < cap ? want : cap;
+}
+
 struct NormFwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool V>
+    template <typename T, typename TR, int VPT, bool V, bool RES>
     void operator()(int tpr) const {
-        const int block = block_threads(tpr);
-        const long want = (p.R + block / tpr - 1) / (block / tpr);
-        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, V>), dim3((unsigned)(want < 65536 ? want : 65536)), dim3(block), 0, s,
-            p, tpr);
+        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, V, RES>), dim3((unsigned)row_blocks(p.R, tpr, 5120)),
+                           dim3(block_threads(tpr)), 0, s, p, tpr);
     }
 };
 
 struct NormBwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool V>
+    template <typename T, typename TR, int VPT, bool V, bool RES>
     void operator()(int tpr) const {
         const int block = block_threads(tpr);
         const size_t smem = block > tpr ? (size_t)block * VPT * SEQ_CH * sizeof(float) : 0;
-        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V>), dim3(p.slots), dim3(block), smem, s,
-            p, tpr);
+        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES>), dim3(p.slots), dim3(block), smem, s, p, tpr);
     }
 };
 
-template <typename T, typename TR, typename F>
+template <typename T, typename TR, bool RES, typename F>
 void by_shape(const BlockNormParams& p, F f) {
     int tpr, vpt;
     row_shape(p.D, &tpr, &vpt);
     auto with = [&](auto v) {
         constexpr bool V = decltype(v)::value;
-        if (vpt == 1) f.template operator()<T, TR, 1, V>(tpr);
-        else if (vpt == 2) f.template operator()<T, TR, 2, V>(tpr);
-        else f.template operator()<T, TR, 4, V>(tpr);
+        if (vpt == 1) f.template operator()<T, TR, 1, V, RES>(tpr);
+        else if (vpt == 2) f.template operator()<T, TR, 2, V, RES>(tpr);
+        else f.template operator()<T, TR, 4, V, RES>(tpr);
     };
     if (p.vec) with(std::true_type{});
     else with(std::false_type{});
@@ -317,21 +395,26 @@ void by_shape(const BlockNormParams& p, F f) {
 
 template <typename F>
 void by_type(const BlockNormParams& p, int is_f32, int res_f32, F f) {
-    if (is_f32 && res_f32) by_shape<float, float>(p, f);
-    else if (is_f32) by_shape<float, __bf16>(p, f);
-    else if (res_f32) by_shape<__bf16, float>(p, f);
-    else by_shape<__bf16, __bf16>(p, f);
+    if (!p.res) {
+        if (is_f32) by_shape<float, float, false>(p, f);
+        else by_shape<__bf16, __bf16, false>(p, f);
+    } else if (is_f32) {
+        if (res_f32) by_shape<float, float, true>(p, f);
+        else by_shape<float, __bf16, true>(p, f);
+    } else {
+        if (res_f32) by_shape<__bf16, float, true>(p, f);
+        else by_shape<__bf16, __bf16, true>(p, f);
+    }
 }
 
 }  // namespace
 
+// Blocks of the backward, each with its own row of column gradients: about
+// twelve waves a CU, what its registers allow.
 extern "C" int block_norm_slots(long R, long D) {
     int tpr, vpt;
     row_shape(D, &tpr, &vpt);
-    const int block = block_threads(tpr);
-    const long want = (R + block / tpr - 1) / (block / tpr);
-    const long cap = 1024;
-    return (int)(want < cap ? want : cap);
+    return (int)row_blocks(R, tpr, 3072);
 }
 
 extern "C" void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s) {

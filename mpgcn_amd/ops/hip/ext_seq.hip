@@ -366,7 +366,8 @@ BlockNormParams norm_params(const Tensor& x, const Opt& gate, const Opt& post, c
     p.R = R;
     p.D = (int)D;
     p.eps = (float)eps;
-    p.vec = D % 8 == 0 && aligned(x, 8) && aligned(gate, 8) && aligned(res, 8);
+    p.vec = D % 8 == 0 && aligned(x, 8) && aligned(gate, 8) && aligned(res, 8) && aligned(post, 8) &&
+            aligned(scale, 8) && aligned(pre, 8);
     return p;
 }
 
