@@ -40,24 +40,21 @@ __device__ __forceinline__ void param8(const float* w, int c, int n, float (&v)[
     if (w && n > 0) load8<float, VEC>(w + c, n, v);
 }
 
-// Eight elements as they are in memory.
+// Eight elements as they are in memory; zeros where there are none.
 template <typename T>
-struct alignas(16) Raw8 { T v[SEQ_CH]; };
+struct Raw8 {
+    static constexpr int E = Pack<T>::E;
+    Pack<T> w[SEQ_CH / E];
+    __device__ __forceinline__ float get(int j) const { return w[j / E].get(j % E); }
+};
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void raw8(const void* base, long at, int n, Raw8<T>& r) {
-    if (n <= 0) {
-#pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j) r.v[j] = (T)0.f;
-        return;
-    }
     const T* p = (const T*)base + at;
-    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(r) / 16); ++i) ((Chunk16*)r.v)[i] = ((const Chunk16*)p)[i];
-    } else {
-#pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+    for (int i = 0; i < SEQ_CH / Raw8<T>::E; ++i) {
+        if (n > 0) r.w[i].template load<VEC>(p + i * Raw8<T>::E, n - i * Raw8<T>::E);
+        else r.w[i].w = i32x4{0, 0, 0, 0};
     }
 }
 
@@ -121,12 +118,12 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                v[i][j] = to_f32(xr[i].v[j]);
+                v[i][j] = xr[i].get(j);
                 if (p.gate) {
-                    const float g = to_f32(gr[i].v[j]);
+                    const float g = gr[i].get(j);
                     v[i][j] *= g * fast_sigmoid(g);
                 }
-                if (RES) hv[i][j] = to_f32(rr[i].v[j]);
+                if (RES) hv[i][j] = rr[i].get(j);
                 ss = fmaf(v[i][j], v[i][j], ss);
             }
         if (AHEAD && k + 1 < rounds) read(r + stride);
@@ -231,13 +228,13 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             gk[i] = gr[i];
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                const float g = p.gate ? to_f32(gr[i].v[j]) : 0.f;
+                const float g = p.gate ? gr[i].get(j) : 0.f;
                 const float sg = p.gate ? g * fast_sigmoid(g) : 1.f;
-                v[i][j] = to_f32(xr[i].v[j]) * sg * inv1;
-                d[i][j] = RES ? to_f32(hr[i].v[j]) : to_f32(yr[i].v[j]);
+                v[i][j] = xr[i].get(j) * sg * inv1;
+                d[i][j] = RES ? hr[i].get(j) : yr[i].get(j);
                 if (RES && p.pre) {
-                    hv[i][j] = to_f32(rr[i].v[j]);
-                    t[i][j] = to_f32(yr[i].v[j]);
+                    hv[i][j] = rr[i].get(j);
+                    t[i][j] = yr[i].get(j);
                 }
             }
         }
@@ -295,9 +292,9 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
                 const float dp = inv1 * fmaf(-m1, v[i][j], d[i][j]);
                 o[j] = dp;
                 if (p.gate) {
-                    const float g = to_f32(gk[i].v[j]), sg = fast_sigmoid(g), si = g * sg;
+                    const float g = gk[i].get(j), sg = fast_sigmoid(g), si = g * sg;
                     o[j] = dp * si;
-                    og[j] = dp * to_f32(xk[i].v[j]) * (sg + si * (1.f - sg));
+                    og[j] = dp * xk[i].get(j) * (sg + si * (1.f - sg));
                 }
             }
             if (live && c < p.D) {

@@ -110,6 +110,7 @@ std::vector<Tensor> short_conv_fwd(Tensor x, Tensor w, Opt bias, Opt s0, Opt len
     if (p.B && p.D && (p.L || want_state)) {
         p.y = y.data_ptr();
         p.s1 = want_state ? s1.data_ptr() : nullptr;
+        short_conv_plan(&p, f32(x), 0);
         const int vec = p.D % 8 == 0 && aligned(x, 8) && aligned(s0, 8);
         short_conv_fwd_launch(p, (int)K, f32(x), vec, stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -131,7 +132,7 @@ std::vector<Tensor> short_conv_bwd(Tensor dy, Opt ds1, Tensor x, Tensor w, Opt b
         auto z = torch::zeros({D * (K + 1)}, w.options());
         return {dx, z.narrow(0, 0, D * K).view({D, K}), z.narrow(0, D * K, D), ds0};
     }
-    p.slots = short_conv_bwd_slots(p.B, p.L, D);
+    short_conv_plan(&p, f32(x), 1);
     auto ws = empty_f32(x, {p.slots, D * (K + 1)});
     auto sums = empty_f32(x, {D * (K + 1)});
     p.dy = dy.data_ptr();

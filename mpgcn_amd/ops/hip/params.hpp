@@ -197,6 +197,7 @@ struct ShortConvParams {
     long x_b, x_t;
     int B, L, D;
     int lens64, silu;
+    int tile;            // steps a thread takes at a time
     int slots;           // backward: blocks that share one channel group
 };
 
@@ -276,7 +277,7 @@ struct BlockNormParams {
 extern "C" {
 void seq_colsum_launch(const float* ws, float* out, long nb, long E, hipStream_t s);
 void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
-int short_conv_bwd_slots(long B, long L, long D);
+void short_conv_plan(ShortConvParams* p, int is_f32, int back);
 void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
 void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out, const float* w,
                             const float* bias, void* y, long B, int D, int K, int silu, int is_f32,

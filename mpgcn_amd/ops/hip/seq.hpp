@@ -64,6 +64,31 @@ __device__ __forceinline__ float softplus_f(float x) {
     return fmaxf(x, 0.f) + log1pf(__expf(-fabsf(x)));
 }
 
+// 16 bytes as they are in memory, two bf16 to a register: kept so while they
+// wait, or each of them would take a register of its own.
+template <typename T>
+struct Pack {
+    static constexpr int E = 16 / sizeof(T);
+    i32x4 w;
+
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __int_as_float(w[j]);
+        else return __int_as_float(j & 1 ? w[j >> 1] & 0xffff0000 : w[j >> 1] << 16);
+    }
+    // n of the E elements are there; VEC: all, and aligned
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* p, int n) {
+        if constexpr (VEC) {
+            w = *(const i32x4*)p;
+        } else {
+            T v[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = j < n ? p[j] : (T)0.f;
+            __builtin_memcpy(&w, v, 16);
+        }
+    }
+};
+
 static inline int pow2_ceil(long n) {
     int p = 1;
     while (p < n) p <<= 1;

@@ -2,195 +2,258 @@
 // (gfx950):  s[t] = bias + sum_k w[k] x[t - K + 1 + k],  y[t] = silu(s[t]).
 //
 // Bound by memory: 2K flops against one element read and one written. A thread
-// owns 8 channels (16 bytes of bf16) and walks the time axis with the last
-// K - 1 inputs in registers, so an input is read once per tile and again only
-// by the K - 1 outputs that the next tile shares with it.
+// owns 16 bytes of channels and walks a tile of the time axis with the last
+// K - 1 inputs in registers; a block of steps is loaded while the block before
+// is worked on. Tiles are as long as keeps the card full: each reads K - 1
+// inputs of its neighbour again.
 #include "seq.hpp"
-
-#define CONV_TT 8    // outputs a thread computes in one tile, forward
-#define CONV_BT 16   // the same, backward (each tile recomputes K - 1 gradients)
 
 namespace {
 
+template <typename T>
+constexpr int conv_e() { return 16 / sizeof(T); }  // channels a thread
+
 __device__ __forceinline__ float silu_f(float s) { return s * fast_sigmoid(s); }
 
-// Input t of sequence b: the carried state before the first, zero before that.
-template <typename T, int K, bool VEC>
-__device__ __forceinline__ void input8(const ShortConvParams& p, const T* x, const T* s0, int t,
-                                       int len, int n, float (&v)[SEQ_CH]) {
-    if (t >= 0 && t < len)
-        load8<T, VEC>(x + t * p.x_t, n, v);
-    else if (t < 0 && t >= -(K - 1) && s0)
-        load8<T, VEC>(s0 + (long)(t + K - 1) * p.D, n, v);
-    else
-        zero8(v);
+template <typename T, bool VEC>
+__device__ __forceinline__ Pack<T> row_at(const T* p, int n) {
+    Pack<T> r;
+    r.template load<VEC>(p, n);
+    return r;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void put_row(T* p, int n, const float (&v)[conv_e<T>()]) {
+    alignas(16) T r[conv_e<T>()];
+#pragma unroll
+    for (int j = 0; j < conv_e<T>(); ++j) r[j] = from_f32<T>(v[j]);
+    if constexpr (VEC) {
+        *(Chunk16*)p = *(const Chunk16*)r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < conv_e<T>(); ++j)
+            if (j < n) p[j] = r[j];
+    }
+}
+template <typename T>
+__device__ __forceinline__ Pack<T> no_row() {
+    return Pack<T>{i32x4{0, 0, 0, 0}};
 }
 
-template <int K>
-__device__ __forceinline__ void taps8(const ShortConvParams& p, int c0, int n, float (&w)[K][SEQ_CH],
-                                      float (&bias)[SEQ_CH]) {
+// Input t of a sequence: the carried state before the first, zero before that
+// and past the end.
+template <typename T, int K, bool VEC>
+__device__ __forceinline__ Pack<T> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n) {
+    if (t >= 0 && t < len) return row_at<T, VEC>(x + t * p.x_t, n);
+    if (t < 0 && t >= -(K - 1) && s0) return row_at<T, VEC>(s0 + (long)(t + K - 1) * p.D, n);
+    return no_row<T>();
+}
+
+template <int K, int E>
+__device__ __forceinline__ void taps(const float* w, const float* bias, int c0, int n, float (&wv)[K][E], float (&bv)[E]) {
 #pragma unroll
-    for (int j = 0; j < SEQ_CH; ++j) {
-        bias[j] = (p.bias && j < n) ? p.bias[c0 + j] : 0.f;
+    for (int j = 0; j < E; ++j) {
+        const int c = j < n ? c0 + j : c0;
+        bv[j] = bias ? bias[c] : 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][j] = j < n ? p.w[(long)(c0 + j) * K + k] : 0.f;
+        for (int k = 0; k < K; ++k) wv[k][j] = w[(long)c * K + k];
     }
 }
 
 template <typename T, int K, bool VEC>
-__launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv,
-                                                             int tiles) {
+__launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv, int tiles) {
+    constexpr int E = conv_e<T>(), NB = 8;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
-    const int c0 = (int)(i % dv) * SEQ_CH;
+    const int c0 = (int)(i % dv) * E;
     const long r = i / dv;
     const int tile = (int)(r % tiles), b = (int)(r / tiles);
-    const int n = p.D - c0 < SEQ_CH ? p.D - c0 : SEQ_CH;
+    const int n = p.D - c0 < E ? p.D - c0 : E;
     const int len = seq_len(p.lens, p.lens64, b, p.L);
     const T* x = (const T*)p.x + b * p.x_b + c0;
     const T* s0 = p.s0 ? (const T*)p.s0 + (long)b * (K - 1) * p.D + c0 : nullptr;
-    T* y = (T*)p.y + (long)b * p.L * p.D + c0;
+    const int t0 = tile * p.tile, t1 = t0 + p.tile < p.L ? t0 + p.tile : p.L;
+    T* y = (T*)p.y + ((long)b * p.L + t0) * p.D + c0;
 
-    const int t0 = tile * CONV_TT;
-    const int t1 = t0 + CONV_TT < p.L ? t0 + CONV_TT : p.L;
-    float w[K][SEQ_CH], bias[SEQ_CH], in[CONV_TT + K - 1][SEQ_CH];
-    // every load of the tile is in flight before the first is used
+    Pack<T> raw[NB];
+    float w[K][E], bias[E], win[K][E];
+    auto read = [&](int t) {
+        const T* s = x + t * p.x_t;
 #pragma unroll
-    for (int j = 0; j < CONV_TT + K - 1; ++j)
-        input8<T, K, VEC>(p, x, s0, t0 + j - (K - 1), len, n, in[j]);
-    taps8<K>(p, c0, n, w, bias);
-#pragma unroll
-    for (int j = 0; j < CONV_TT; ++j) {
-        if (t0 + j >= t1) break;
-        float o[SEQ_CH];
-#pragma unroll
-        for (int c = 0; c < SEQ_CH; ++c) {
-            float s = bias[c];
-#pragma unroll
-            for (int k = 0; k < K; ++k) s = fmaf(w[k][c], in[j + k][c], s);
-            o[c] = t0 + j < len ? (p.silu ? silu_f(s) : s) : 0.f;
+        for (int j = 0; j < NB; ++j) {
+            raw[j] = t + j < len ? row_at<T, VEC>(s, n) : no_row<T>();
+            s += p.x_t;
         }
-        store8<T, VEC>(y + (long)(t0 + j) * p.D, n, o);
+    };
+    Pack<T> edge[K - 1];
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K, VEC>(p, x, s0, t0 - (K - 1) + k, len, n);
+    read(t0);
+    taps<K, E>(p.w, p.bias, c0, n, w, bias);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int c = 0; c < E; ++c) win[k + 1][c] = edge[k].get(c);
+    for (int t = t0; t < t1; t += NB) {
+        Pack<T> cur[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) cur[j] = raw[j];
+        if (t + NB < t1) read(t + NB);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float o[E];
+#pragma unroll
+            for (int c = 0; c < E; ++c) {
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) win[k][c] = win[k + 1][c];
+                win[K - 1][c] = cur[j].get(c);
+                float s = bias[c];
+#pragma unroll
+                for (int k = 0; k < K; ++k) s = fmaf(w[k][c], win[k][c], s);
+                o[c] = t + j < len ? (p.silu ? silu_f(s) : s) : 0.f;
+            }
+            if (t + j < t1) put_row<T, VEC>(y, n, o);
+            y += p.D;
+        }
     }
     if (p.s1 && tile == 0) {
         T* s1 = (T*)p.s1 + (long)b * (K - 1) * p.D + c0;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            float v[SEQ_CH];
-            input8<T, K, VEC>(p, x, s0, len - (K - 1) + j, len, n, v);
-            store8<T, VEC>(s1 + (long)j * p.D, n, v);
+            const Pack<T> v = input_row<T, K, VEC>(p, x, s0, len - (K - 1) + j, len, n);
+            float o[E];
+#pragma unroll
+            for (int c = 0; c < E; ++c) o[c] = v.get(c);
+            put_row<T, VEC>(s1 + (long)j * p.D, n, o);
         }
     }
 }
 
 // Backward: ds[t] = dy[t] silu'(s[t]) with s recomputed, dx[t] = sum_k w[k]
 // ds[t + K - 1 - k], dw[k] = sum ds[t] x[t - K + 1 + k]. A thread streams one
-// tile in time order holding the last K inputs and the last K values of ds;
-// filter gradients stay in registers over all of its tiles, are joined per
-// block and written once, then summed in a fixed order (no atomics).
+// tile in time order, K - 1 steps past its end, holding the last K inputs and
+// the last K values of ds; filter gradients stay in registers over all of its
+// tiles, are joined per block and written once, then summed in a fixed order
+// (no atomics).
 template <typename T, int K, bool VEC>
-__launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, int dv, int cw,
-                                                             int tiles) {
-    extern __shared__ float lds[];  // [256][SEQ_CH * (K + 1)]
+__launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, int dv, int cw, int tiles) {
+    constexpr int E = conv_e<T>(), NB = 4;
+    constexpr int W = E * (K + 1);
+    extern __shared__ float lds[];  // [256][W]
     const int rt = threadIdx.x / cw, nrt = 256 / cw;
     const int cv = blockIdx.y * cw + threadIdx.x % cw;
-    const int c0 = cv * SEQ_CH;
-    const bool live = cv < dv;
-    const int n = p.D - c0 < SEQ_CH ? p.D - c0 : SEQ_CH;
-    float dw[K][SEQ_CH] = {}, db[SEQ_CH] = {};
-    if (live) {
-        float w[K][SEQ_CH], bias[SEQ_CH];
-        taps8<K>(p, c0, n, w, bias);
+    const int c0 = cv * E;
+    const int n = p.D - c0 < E ? p.D - c0 : E;
+    float dw[K][E] = {}, db[E] = {};
+    if (cv < dv) {
+        float w[K][E], bias[E];
+        taps<K, E>(p.w, p.bias, c0, n, w, bias);
         const long items = (long)p.B * tiles;
         for (long i = (long)blockIdx.x * nrt + rt; i < items; i += (long)p.slots * nrt) {
             const int tile = (int)(i % tiles), b = (int)(i / tiles);
             const int len = seq_len(p.lens, p.lens64, b, p.L);
+            const int t0 = tile * p.tile, t1 = t0 + p.tile < p.L ? t0 + p.tile : p.L;
             const T* x = (const T*)p.x + b * p.x_b + c0;
             const T* s0 = p.s0 ? (const T*)p.s0 + (long)b * (K - 1) * p.D + c0 : nullptr;
             const T* ds1 = p.ds1 ? (const T*)p.ds1 + (long)b * (K - 1) * p.D + c0 : nullptr;
             const T* dy = (const T*)p.dy + (long)b * p.L * p.D + c0;
             T* dx = (T*)p.dx + (long)b * p.L * p.D + c0;
             T* ds0 = p.ds0 ? (T*)p.ds0 + (long)b * (K - 1) * p.D + c0 : nullptr;
-            const int t0 = tile * CONV_BT;
-            const int t1 = t0 + CONV_BT < p.L ? t0 + CONV_BT : p.L;
-            float xw[K][SEQ_CH], gw[K][SEQ_CH];
+            Pack<T> xr[NB], yr[NB], edge[K - 1];
+            auto read = [&](int t) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                zero8(gw[k]);
-                if (k) input8<T, K, VEC>(p, x, s0, t0 - K + k, len, n, xw[k]);
-                else zero8(xw[0]);
-            }
-            // t runs K - 1 past the tile: those gradients reach back into it.
+                for (int j = 0; j < NB; ++j) {
+                    const bool on = t + j < len;
+                    xr[j] = on ? row_at<T, VEC>(x + (t + j) * p.x_t, n) : no_row<T>();
+                    yr[j] = on ? row_at<T, VEC>(dy + (long)(t + j) * p.D, n) : no_row<T>();
+                }
+            };
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K, VEC>(p, x, s0, t0 - (K - 1) + k, len, n);
+            read(t0);
+            float xw[K][E], gw[K][E];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int c = 0; c < E; ++c) {
+                    gw[k][c] = 0.f;
+                    xw[k][c] = k ? edge[k ? k - 1 : 0].get(c) : 0.f;
+                }
             // The first tile starts with the outputs whose window holds the
             // carried state, so it emits that state's gradient as it goes.
-            for (int t = t0; t < t1 + K - 1; ++t) {
-                float g[SEQ_CH];
+            for (int tb = t0; tb < t1 + K - 1; tb += NB) {
+                Pack<T> xc[NB], yc[NB];
 #pragma unroll
-                for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                    for (int c = 0; c < SEQ_CH; ++c) {
-                        xw[k][c] = xw[k + 1][c];
-                        gw[k][c] = gw[k + 1][c];
-                    }
-                input8<T, K, VEC>(p, x, s0, t, len, n, xw[K - 1]);
-                if (t < len) load8<T, VEC>(dy + (long)t * p.D, n, g);
-                else zero8(g);
-#pragma unroll
-                for (int c = 0; c < SEQ_CH; ++c) {
-                    float s = bias[c];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) s = fmaf(w[k][c], xw[k][c], s);
-                    if (p.silu) {
-                        const float sg = fast_sigmoid(s);
-                        g[c] *= sg * (1.f + s * (1.f - sg));
-                    }
-                    g[c] = t < len ? g[c] : 0.f;
-                    gw[K - 1][c] = g[c];
-                    if (t < t1) {
-                        db[c] += g[c];
-#pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][c] = fmaf(g[c], xw[k][c], dw[k][c]);
-                    }
+                for (int j = 0; j < NB; ++j) {
+                    xc[j] = xr[j];
+                    yc[j] = yr[j];
                 }
-                // ds[t - K + 1 .. t] are in gw: input t - K + 1 is complete
-                const int ti = t - (K - 1);
-                if (ti < t0 && (tile || !ds0)) continue;
-                float o[SEQ_CH];
-                zero8(o);
-                const int tail = ti - (len - (K - 1));
-                if (ds1 && tail >= 0 && tail < K - 1)
-                    load8<T, VEC>(ds1 + (long)tail * p.D, n, o);
+                if (tb + NB < t1 + K - 1) read(tb + NB);
 #pragma unroll
-                for (int c = 0; c < SEQ_CH; ++c)
+                for (int j = 0; j < NB; ++j) {
+                    const int t = tb + j;
+                    if (t >= t1 + K - 1) break;
 #pragma unroll
-                    for (int k = 0; k < K; ++k) o[c] = fmaf(w[K - 1 - k][c], gw[k][c], o[c]);
-                if (ti >= 0) {
-                    if (ti < t1) store8<T, VEC>(dx + (long)ti * p.D, n, o);
-                } else {
-                    store8<T, VEC>(ds0 + (long)(ti + K - 1) * p.D, n, o);
+                    for (int c = 0; c < E; ++c) {
+#pragma unroll
+                        for (int k = 0; k < K - 1; ++k) {
+                            xw[k][c] = xw[k + 1][c];
+                            gw[k][c] = gw[k + 1][c];
+                        }
+                        xw[K - 1][c] = xc[j].get(c);
+                        float s = bias[c], g = yc[j].get(c);
+#pragma unroll
+                        for (int k = 0; k < K; ++k) s = fmaf(w[k][c], xw[k][c], s);
+                        if (p.silu) {
+                            const float sg = fast_sigmoid(s);
+                            g *= sg * (1.f + s * (1.f - sg));
+                        }
+                        g = t < len ? g : 0.f;
+                        gw[K - 1][c] = g;
+                        g = t < t1 ? g : 0.f;  // past the tile it is another's
+                        db[c] += g;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dw[k][c] = fmaf(g, xw[k][c], dw[k][c]);
+                    }
+                    // ds[t - K + 1 .. t] are in gw: input t - K + 1 is complete
+                    const int ti = t - (K - 1);
+                    if (ti >= t1 || (ti < t0 && (tile || !ds0))) continue;
+                    float o[E];
+#pragma unroll
+                    for (int c = 0; c < E; ++c) o[c] = 0.f;
+                    const int tail = ti - (len - (K - 1));
+                    if (ds1 && tail >= 0 && tail < K - 1) {
+                        const Pack<T> v = row_at<T, VEC>(ds1 + (long)tail * p.D, n);
+#pragma unroll
+                        for (int c = 0; c < E; ++c) o[c] = v.get(c);
+                    }
+#pragma unroll
+                    for (int c = 0; c < E; ++c)
+#pragma unroll
+                        for (int k = 0; k < K; ++k) o[c] = fmaf(w[K - 1 - k][c], gw[k][c], o[c]);
+                    if (ti >= 0) put_row<T, VEC>(dx + (long)ti * p.D, n, o);
+                    else put_row<T, VEC>(ds0 + (long)(ti + K - 1) * p.D, n, o);
                 }
             }
         }
     }
-    constexpr int W = SEQ_CH * (K + 1);
     float* mine = lds + threadIdx.x * W;
 #pragma unroll
-    for (int c = 0; c < SEQ_CH; ++c) {
+    for (int c = 0; c < E; ++c) {
 #pragma unroll
         for (int k = 0; k < K; ++k) mine[c * K + k] = dw[k][c];
-        mine[SEQ_CH * K + c] = db[c];
+        mine[E * K + c] = db[c];
     }
     __syncthreads();
     float* ws = p.ws + (long)blockIdx.x * p.D * (K + 1);
     for (int i = threadIdx.x; i < cw * W; i += 256) {
         const int v = i / W, e = i % W;
-        const int c = (blockIdx.y * cw + v) * SEQ_CH;
+        const int c = (blockIdx.y * cw + v) * E;
         float s = 0.f;
         for (int r = 0; r < nrt; ++r) s += lds[(r * cw + v) * W + e];
-        if (e < SEQ_CH * K) {
+        if (e < E * K) {
             if (c + e / K < p.D) ws[(long)c * K + e] = s;
-        } else if (c + e - SEQ_CH * K < p.D) {
-            ws[(long)p.D * K + c + e - SEQ_CH * K] = s;
+        } else if (c + e - E * K < p.D) {
+            ws[(long)p.D * K + c + e - E * K] = s;
         }
     }
 }
@@ -223,6 +286,18 @@ __launch_bounds__(256) __global__ void short_conv_step_kernel(
     for (int k = 0; k < K - 1; ++k) store8<T, VEC>(s_out + (b * (K - 1) + k) * D + c0, n, in[k + 1]);
 }
 
+// Threads of a block side by side in the channels.
+inline int conv_cw(long dv) { return pow2_ceil(dv) < 64 ? pow2_ceil(dv) : 64; }
+
+// Steps of a tile, a multiple of 8: whole sequences if that leaves enough
+// threads, else as few as `threads` of them need.
+inline int conv_tile(long B, long L, long dv, long threads) {
+    long tiles = threads / (B * dv > 0 ? B * dv : 1);
+    tiles = tiles < 1 ? 1 : tiles;
+    const long t = ((L + tiles - 1) / tiles + 7) / 8 * 8;
+    return (int)(t < 16 ? (L <= 8 ? 8 : 16) : t);
+}
+
 template <typename F>
 void by_type(int K, int is_f32, int vec, F f) {
     auto with_k = [&](auto t, auto v) {
@@ -245,11 +320,11 @@ struct Fwd {
     hipStream_t s;
     template <typename T, int K, bool V>
     void operator()() const {
-        const int dv = (p.D + SEQ_CH - 1) / SEQ_CH;
-        const int tiles = p.L ? (p.L + CONV_TT - 1) / CONV_TT : 1;
+        const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
+        const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const long items = (long)p.B * tiles * dv;
-        hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, V>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s,
-            p, items, dv, tiles);
+        hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, V>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p,
+                           items, dv, tiles);
     }
 };
 
@@ -258,12 +333,12 @@ struct Bwd {
     hipStream_t s;
     template <typename T, int K, bool V>
     void operator()() const {
-        const int dv = (p.D + SEQ_CH - 1) / SEQ_CH;
-        const int cw = pow2_ceil(dv) < 64 ? pow2_ceil(dv) : 64;
-        const int tiles = p.L ? (p.L + CONV_BT - 1) / CONV_BT : 1;
-        const size_t smem = 256 * SEQ_CH * (K + 1) * sizeof(float);
-        hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3(p.slots, (dv + cw - 1) / cw), dim3(256), smem, s,
-            p, dv, cw, tiles);
+        const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
+        const int cw = conv_cw(dv);
+        const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
+        const size_t smem = 256 * conv_e<T>() * (K + 1) * sizeof(float);
+        hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3(p.slots, (dv + cw - 1) / cw), dim3(256), smem, s, p, dv,
+                           cw, tiles);
     }
 };
 
@@ -281,21 +356,21 @@ struct Step {
 
 }  // namespace
 
+// The tile of p and, for the backward, the blocks that share a channel group:
+// each writes a row of filter gradients.
+extern "C" void short_conv_plan(ShortConvParams* p, int is_f32, int back) {
+    const long e = is_f32 ? 4 : 8, dv = (p->D + e - 1) / e;
+    // 16 waves a CU forward, 8 backward: what the registers allow
+    p->tile = conv_tile(p->B, p->L, dv, back ? 256L * 8 * 64 : 256L * 16 * 64);
+    const long cw = conv_cw(dv), groups = (dv + cw - 1) / cw, rows = 256 / cw;
+    const long items = p->B * (p->L ? ((long)p->L + p->tile - 1) / p->tile : 1);
+    const long want = (items + rows - 1) / rows, cap = (512 + groups - 1) / groups;
+    p->slots = (int)(want < cap ? want : cap);
+}
+
 extern "C" void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
                                       hipStream_t s) {
     by_type(K, is_f32, vec, Fwd{p, s});
-}
-
-// Blocks per channel group in the backward: enough to fill 256 CUs a few times
-// over, no more than there are row threads with work.
-extern "C" int short_conv_bwd_slots(long B, long L, long D) {
-    const long dv = (D + SEQ_CH - 1) / SEQ_CH;
-    const long cw = pow2_ceil(dv) < 64 ? pow2_ceil(dv) : 64;
-    const long groups = (dv + cw - 1) / cw;
-    const long items = B * (L ? (L + CONV_BT - 1) / CONV_BT : 1);
-    const long want = (items + 256 / cw - 1) / (256 / cw);
-    const long cap = (1024 + groups - 1) / groups;
-    return (int)(want < cap ? want : cap);
 }
 
 extern "C" void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
