@@ -83,6 +83,43 @@ struct Weights {
     }
 };
 
+// The same for the backward, whose registers hold the column gradients: in LDS
+// where a thread has one chunk. Each thread reads back only what it put there.
+template <int VPT, bool VEC, bool RES>
+struct WeightsBack {
+    static constexpr bool KEEP = VPT == 1;
+    f32x4* mine;  // [3][2][blockDim]
+
+    __device__ __forceinline__ WeightsBack(const BlockNormParams& p, int c, float* lds) {
+        mine = (f32x4*)lds + threadIdx.x;
+        if (!KEEP) return;
+        keep(p.post, c, p.D, 0);
+        if (RES) keep(p.scale, c, p.D, 1);
+        if (RES) keep(p.pre, c, p.D, 2);
+    }
+    __device__ __forceinline__ void keep(const float* from, int c, int D, int which) {
+        float v[SEQ_CH];
+        param8<VEC>(from, c, D - c, v);
+        mine[(which * 2) * blockDim.x] = f32x4{v[0], v[1], v[2], v[3]};
+        mine[(which * 2 + 1) * blockDim.x] = f32x4{v[4], v[5], v[6], v[7]};
+    }
+    template <int WHICH>
+    __device__ __forceinline__ void get(const float* from, int c, int D, float (&v)[SEQ_CH]) const {
+        if (KEEP) {
+            unsigned at = WHICH * 2 * blockDim.x;
+            asm volatile("" : "+v"(at));  // read here, not kept over the rows
+            const f32x4 a = mine[at], b = mine[at + blockDim.x];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = a[j];
+                v[4 + j] = b[j];
+            }
+        } else {
+            param8<VEC>(from, c, D - c, v);
+        }
+    }
+};
+
 // A thread keeps its columns and takes one row after another; with one chunk a
 // thread a row's loads are in flight while the row before is worked on.
 template <typename T, typename TR, int VPT, bool VEC, bool RES>
@@ -182,9 +219,10 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 //   dp0 = inv1 (q - n1 mean(q n1));  dx, dgate by the product and silu'
 // Column gradients stay in registers over a thread's rows, are joined in LDS
 // over the block's row groups and written once per block.
-template <typename T, typename TR, int VPT, bool VEC, bool RES>
+template <typename T, typename TR, int VPT, bool VEC, bool RES, bool GATE>
 __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
-    extern __shared__ float dyn[];  // [rpb][VPT * tpr * SEQ_CH] when rpb > 1
+    // the weights, then [rpb][VPT * tpr * SEQ_CH] to join the column gradients
+    extern __shared__ __attribute__((aligned(16))) float dyn[];
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr, rg = threadIdx.x / tpr;
@@ -192,7 +230,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
     const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
     long r = (long)blockIdx.x * rpb + rg;
 
-    const Weights<VPT, VEC, RES> wt(p, lane * SEQ_CH);
+    const WeightsBack<VPT, VEC, RES> wt(p, lane * SEQ_CH, dyn);
     constexpr bool AHEAD = VPT == 1;
     float dpost[VPT][SEQ_CH] = {}, dscale[VPT][SEQ_CH] = {}, dpre[VPT][SEQ_CH] = {};
     Raw8<T> xr[VPT], gr[VPT], yr[VPT];
@@ -206,7 +244,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             const int c = (i * tpr + lane) * SEQ_CH;
             const int n = there ? p.D - c : 0;
             raw8<T, VEC>(p.x, row * p.x_r + c, n, xr[i]);
-            if (p.gate) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
+            if (GATE) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
             if (!RES || p.pre) raw8<T, VEC>(p.dy, row * p.D + c, p.dy ? n : 0, yr[i]);
             if (RES && p.pre) raw8<TR, VEC>(p.res, row * p.r_r + c, n, rr[i]);
             if (RES) raw8<TR, VEC>(p.dh, row * p.D + c, p.dh ? n : 0, hr[i]);
@@ -228,8 +266,8 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             gk[i] = gr[i];
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                const float g = p.gate ? gr[i].get(j) : 0.f;
-                const float sg = p.gate ? g * fast_sigmoid(g) : 1.f;
+                const float g = GATE ? gr[i].get(j) : 0.f;
+                const float sg = GATE ? g * fast_sigmoid(g) : 1.f;
                 v[i][j] = xr[i].get(j) * sg * inv1;
                 d[i][j] = RES ? hr[i].get(j) : yr[i].get(j);
                 if (RES && p.pre) {
@@ -291,7 +329,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             for (int j = 0; j < SEQ_CH; ++j) {
                 const float dp = inv1 * fmaf(-m1, v[i][j], d[i][j]);
                 o[j] = dp;
-                if (p.gate) {
+                if (GATE) {
                     const float g = gk[i].get(j), sg = fast_sigmoid(g), si = g * sg;
                     o[j] = dp * si;
                     og[j] = dp * xk[i].get(j) * (sg + si * (1.f - sg));
@@ -299,7 +337,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
             }
             if (live && c < p.D) {
                 store8<T, VEC>((T*)p.dx + r * p.D + c, p.D - c, o);
-                if (p.gate) store8<T, VEC>((T*)p.dgate + r * p.D + c, p.D - c, og);
+                if (GATE) store8<T, VEC>((T*)p.dgate + r * p.D + c, p.D - c, og);
             }
         }
     }
@@ -348,10 +386,11 @@ inline void row_shape(long D, int* tpr, int* vpt) {
 // Whole rows in a block of about 256 threads.
 inline int block_threads(int tpr) { return tpr >= 256 ? tpr : 256 / tpr * tpr; }
 
-// Blocks that take the rows in turn: as many waves as stay on the card.
-inline long row_blocks(long R, int tpr, long waves) {
-    const int block = block_threads(tpr);
-    const long want = (R + block / tpr - 1) / (block / tpr), cap = (waves * 64 + block - 1) / block;
+// Blocks that take the rows in turn: as many as 256 CUs hold at once, given the
+// waves a CU has registers for. More would leave a second, emptier round.
+inline long row_blocks(long R, int tpr, int waves) {
+    const int block = block_threads(tpr), per_cu = waves / (block / 64);
+    const long want = (R + block / tpr - 1) / (block / tpr), cap = 256L * (per_cu ? per_cu : 1);
     return want < cap ? want : cap;
 }
 
@@ -360,7 +399,7 @@ struct NormFwd {
     hipStream_t s;
     template <typename T, typename TR, int VPT, bool V, bool RES>
     void operator()(int tpr) const {
-        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, V, RES>), dim3((unsigned)row_blocks(p.R, tpr, 5120)),
+        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, V, RES>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
                            dim3(block_threads(tpr)), 0, s, p, tpr);
     }
 };
@@ -371,8 +410,11 @@ struct NormBwd {
     template <typename T, typename TR, int VPT, bool V, bool RES>
     void operator()(int tpr) const {
         const int block = block_threads(tpr);
-        const size_t smem = block > tpr ? (size_t)block * VPT * SEQ_CH * sizeof(float) : 0;
-        hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+        const size_t smem = (size_t)block * SEQ_CH * sizeof(float) * (VPT > 1 ? VPT : RES ? 3 : 1);
+        if (p.gate)
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES, true>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+        if (!p.gate)
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES, false>), dim3(p.slots), dim3(block), smem, s, p, tpr);
     }
 };
 
@@ -406,12 +448,11 @@ void by_type(const BlockNormParams& p, int is_f32, int res_f32, F f) {
 
 }  // namespace
 
-// Blocks of the backward, each with its own row of column gradients: about
-// twelve waves a CU, what its registers allow.
-extern "C" int block_norm_slots(long R, long D) {
+// Blocks of the backward, each with its own row of column gradients.
+extern "C" int block_norm_slots(long R, long D, int res, int gate) {
     int tpr, vpt;
     row_shape(D, &tpr, &vpt);
-    return (int)row_blocks(R, tpr, 3072);
+    return (int)row_blocks(R, tpr, vpt > 1 ? 8 : !res ? 16 : gate ? 8 : 12);
 }
 
 extern "C" void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s) {

@@ -410,7 +410,7 @@ std::vector<Tensor> block_norm_bwd(Opt dy, Opt dh, Tensor x, Opt gate, Opt post,
     const long nw = has(post) + has(scale) + has(pre);
     Tensor sums;
     if (R && D) {
-        p.slots = block_norm_slots(R, D);
+        p.slots = block_norm_slots(R, D, has(res), has(gate));
         auto ws = empty_f32(x, {p.slots, nw * D});
         sums = empty_f32(x, {nw, D});
         p.inv1 = (float*)fptr(inv1);

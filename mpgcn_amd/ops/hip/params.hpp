@@ -287,7 +287,7 @@ void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStre
 void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32, hipStream_t s);
 void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s);
-int block_norm_slots(long R, long D);
+int block_norm_slots(long R, long D, int res, int gate);
 void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);
 void block_norm_bwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);
 }
