@@ -305,12 +305,14 @@ Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor C
     const long B = u.size(0), D = u.size(1);
     TORCH_CHECK(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be (D, N), N in 1..64");
     const long N = A.size(1);
-    TORCH_CHECK(Bm.dim() == 3 && Bm.size(1) >= 1 && D % Bm.size(1) == 0, "B must be (B, G, N), G a divisor of D");
-    const long G = Bm.size(1);
+    TORCH_CHECK(Bm.dim() == 2 || Bm.dim() == 3, "B must be (B, N) or (B, G, N)");
+    const bool grouped = Bm.dim() == 3;
+    const long G = grouped ? Bm.size(1) : 1;
+    TORCH_CHECK(G >= 1 && D % G == 0, "the groups must divide the channels");
     check_data(u, u, u.sizes(), "u");
     check_data(delta, u, {B, D}, "delta");
-    check_data(Bm, u, {B, G, N}, "B");
-    check_data(Cm, u, {B, G, N}, "C");
+    check_data(Bm, u, grouped ? at::IntArrayRef({B, G, N}) : at::IntArrayRef({B, N}), "B");
+    check_data(Cm, u, grouped ? at::IntArrayRef({B, G, N}) : at::IntArrayRef({B, N}), "C");
     check_f32(A, u, {D, N}, "A");
     check_f32(skip, u, {D}, "skip");
     check_f32(dbias, u, {D}, "delta_bias");
@@ -323,7 +325,8 @@ Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor C
         p.A = A.data_ptr<float>(); p.skip = fptr(skip); p.dbias = fptr(dbias);
         p.h = state.data_ptr<float>(); p.h_out = state_out.data_ptr<float>(); p.y = y.data_ptr();
         p.u_b = u.stride(0); p.d_b = delta.stride(0);
-        p.B_b = Bm.stride(0); p.B_g = Bm.stride(1); p.C_b = Cm.stride(0); p.C_g = Cm.stride(1);
+        p.B_b = Bm.stride(0); p.B_g = grouped ? Bm.stride(1) : 0;
+        p.C_b = Cm.stride(0); p.C_g = grouped ? Cm.stride(1) : 0;
         p.B = (int)B; p.D = (int)D; p.N = (int)N; p.G = (int)G;
         p.softplus = softplus ? 1 : 0;
         p.bvec = N % 4 == 0 && aligned(Bm, 4) && aligned(Cm, 4) && aligned(A, 4) && aligned(state, 4) &&
@@ -434,6 +437,89 @@ std::vector<Tensor> block_norm_bwd(Opt dy, Opt dh, Tensor x, Opt gate, Opt post,
     return {dx, dg, dpost, dr, dscale, dpre};
 }
 
+// ---- calls that need no preparation -----------------------------------------
+//
+// The operators' common case at inference, without Python's share of the time:
+// every argument is in the kernels' form and no gradient is wanted. Any other
+// call gives None and goes through the checks and conversions of
+// mpgcn_amd/ops/sequence.py, which name what is wrong.
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t && t->defined() && t->requires_grad()) return true;
+    return false;
+}
+const Tensor* tp(const Opt& t) { return t.has_value() ? &*t : nullptr; }
+
+template <typename F>
+py::object direct(F f) {
+    try {
+        return f();
+    } catch (const c10::Error&) {
+        return py::none();
+    }
+}
+
+// Two states that a step may read and write: the same memory or none shared.
+bool apart(const Tensor& a, const Tensor& b) {
+    const char *pa = (const char*)a.data_ptr(), *pb = (const char*)b.data_ptr();
+    const long d = pa < pb ? pb - pa : pa - pb;
+    return d == 0 || d >= (long)(a.numel() * a.element_size());
+}
+
+py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state) {
+    if (!x.is_cuda() || wants_grad({&x, &w, tp(bias), tp(s0)})) return py::none();
+    return direct([&]() -> py::object {
+        auto r = short_conv_fwd(x, w, bias, s0, lens, silu, want_state);
+        return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
+    });
+}
+
+py::object short_conv_step_direct(Tensor x, Tensor state, Opt state_out, Tensor w, Opt bias, bool silu) {
+    const Tensor out = has(state_out) ? *state_out : state;
+    if (!x.is_cuda() || wants_grad({&x, &state, &out, &w, tp(bias)}) || !apart(state, out)) return py::none();
+    return direct([&] { return py::make_tuple(short_conv_step(x, state, out, w, bias, silu), out); });
+}
+
+py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias, Opt h0,
+                                 Opt lens, bool softplus, bool want_state) {
+    if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)})) return py::none();
+    return direct([&]() -> py::object {
+        auto grouped = [](const Tensor& t) { return t.dim() == 3 ? t.unsqueeze(2) : t; };
+        auto r = selective_scan_fwd(u, delta, A, grouped(Bm), grouped(Cm), skip, dbias, h0, lens, softplus, want_state,
+                                    false);
+        return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
+    });
+}
+
+py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state,
+                                      Opt state_out, Opt skip, Opt dbias, bool softplus) {
+    const Tensor out = has(state_out) ? *state_out : state;
+    if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, &state, &out, tp(skip), tp(dbias)}) || !apart(state, out))
+        return py::none();
+    return direct([&] {
+        return py::make_tuple(selective_scan_step(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus), out);
+    });
+}
+
+py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps) {
+    if (!x.is_cuda() || x.dim() < 1 || !(eps > 0) ||
+        wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)}))
+        return py::none();
+    return direct([&]() -> py::object {
+        const auto shape = x.sizes().vec();
+        const bool flat = x.dim() == 2;
+        TORCH_CHECK(shape.back() >= 1 && (!has(gate) || gate->sizes() == x.sizes()) && (!has(res) || res->sizes() == x.sizes()));
+        auto rows = [&](const Tensor& t) { return flat ? t : t.reshape({-1, shape.back()}); };
+        auto opt = [&](const Opt& t) { return has(t) ? Opt(rows(*t)) : Opt(); };
+        auto r = block_norm_fwd(rows(x), opt(gate), post, opt(res), scale, pre, eps, false);
+        auto back = [&](const Tensor& t) { return flat ? t : t.view(shape); };
+        if (r[0].defined() && r[1].defined()) return py::make_tuple(back(r[0]), back(r[1]));
+        return py::cast(back(r[0].defined() ? r[0] : r[1]));
+    });
+}
+
 }  // namespace
 
 // A leaf whose gradient an eager graph, still alive, accumulates on another
@@ -455,4 +541,9 @@ void bind_sequence(pybind11::module_& m) {
     m.def("selective_scan_step", &selective_scan_step, "selective state space scan of one new token");
     m.def("block_norm_fwd", &block_norm_fwd, "norms around a block with gate and residual scale");
     m.def("block_norm_bwd", &block_norm_bwd, "backward of block_norm_fwd");
+    m.def("short_conv_direct", &short_conv_direct, "short_conv where no preparation is needed, else None");
+    m.def("short_conv_step_direct", &short_conv_step_direct, "short_conv_step, likewise");
+    m.def("selective_scan_direct", &selective_scan_direct, "selective_scan, likewise");
+    m.def("selective_scan_step_direct", &selective_scan_step_direct, "selective_scan_step, likewise");
+    m.def("block_norm_direct", &block_norm_direct, "norm_gate_residual, likewise");
 }

@@ -40,6 +40,10 @@ _MAX_STATES = 64
 _MAX_NORM_D = 16384
 
 
+def _on_gpu(t) -> bool:
+    return isinstance(t, torch.Tensor) and t.is_cuda
+
+
 # ---- argument checks --------------------------------------------------------
 
 def _check_act(t: torch.Tensor, name: str, shape, like: torch.Tensor | None = None) -> None:
@@ -203,12 +207,16 @@ def short_conv(x, weight, bias=None, *, state=None, lengths=None, activation="si
     bias: (D,). state: (B, K-1, D) of x's type, the inputs before the first
     (zeros if None). Returns y, or (y, state after the last valid token).
     """
+    silu = _check_activation(activation)
+    if _on_gpu(x):
+        out = _ops.get_ext().short_conv_direct(x, weight, bias, state, lengths, silu, return_state)
+        if out is not None:
+            return out
     _check_act(x, "x", None)
     if x.dim() != 3:
         raise ValueError(f"x must be (batch, length, channels), got {tuple(x.shape)}")
     B, _, D = x.shape
     K = _check_taps(weight, D)
-    silu = _check_activation(activation)
     weight = _param(weight, "weight", (D, K), x)
     bias = _param(bias, "bias", (D,), x)
     if state is not None:
@@ -230,12 +238,16 @@ def short_conv_step(x, state, weight, bias=None, *, activation="silu", state_out
     """short_conv of one new token per sequence. x: (B, D); state: (B, K-1, D)
     contiguous. Returns (y (B, D), the new state): written over ``state``, or to
     ``state_out`` if given."""
+    silu = _check_activation(activation)
+    if _on_gpu(x):
+        res = _ops.get_ext().short_conv_step_direct(x, state, state_out, weight, bias, silu)
+        if res is not None:
+            return res
     _check_act(x, "x", None)
     if x.dim() != 2:
         raise ValueError(f"x must be (batch, channels), got {tuple(x.shape)}")
     B, D = x.shape
     K = _check_taps(weight, D)
-    silu = _check_activation(activation)
     _no_grad_only("short_conv_step", x, state, weight, bias, state_out)
     weight = _param(weight, "weight", (D, K), x)
     bias = _param(bias, "bias", (D,), x)
@@ -319,6 +331,12 @@ def selective_scan(u, delta, A, B, C, skip=None, *, delta_bias=None, delta_softp
     state: (B, D, N) f32, h before the first token (zeros if None). Returns y,
     or (y, f32 state after the last valid token).
     """
+    softplus = bool(delta_softplus)
+    if _on_gpu(u):
+        out = _ops.get_ext().selective_scan_direct(u, delta, A, B, C, skip, delta_bias, state, lengths, softplus,
+                                                   return_state)
+        if out is not None:
+            return out
     A, B, C = _check_scan(u, delta, A, B, C, ("batch", "length"))
     nb, _, D = u.shape
     N = A.shape[1]
@@ -327,7 +345,6 @@ def selective_scan(u, delta, A, B, C, skip=None, *, delta_bias=None, delta_softp
     if state is not None:
         _check_carried(state, "state", (nb, D, N), _state_dtype(u), u)
     lengths = _check_lengths(lengths, nb, u)
-    softplus = bool(delta_softplus)
     if not u.is_cuda:
         y, last = eager.selective_scan_eager(u, delta, A, B, C, skip, delta_bias, softplus, state, lengths)
         return (y, last) if return_state else y
@@ -346,6 +363,11 @@ def selective_scan_step(u, delta, A, B, C, state, skip=None, *, delta_bias=None,
     """selective_scan of one new token per sequence. u, delta: (B, D); B, C:
     (B, N) or (B, G, N); state: (B, D, N) f32 contiguous. Returns (y (B, D), the
     new state): written over ``state``, or to ``state_out`` if given."""
+    softplus = bool(delta_softplus)
+    if _on_gpu(u):
+        res = _ops.get_ext().selective_scan_step_direct(u, delta, A, B, C, state, state_out, skip, delta_bias, softplus)
+        if res is not None:
+            return res
     A, B, C = _check_scan(u, delta, A, B, C, ("batch",))
     nb, D = u.shape
     _no_grad_only("selective_scan_step", u, delta, A, B, C, state, skip, delta_bias, state_out)
@@ -354,11 +376,11 @@ def selective_scan_step(u, delta, A, B, C, state, skip=None, *, delta_bias=None,
     out = _state_pair(state, state_out, (nb, D, A.shape[1]), _state_dtype(u), u)
     if not u.is_cuda:
         y, last = eager.selective_scan_eager(u.unsqueeze(1), delta.unsqueeze(1), A, B.unsqueeze(1), C.unsqueeze(1),
-                                             skip, delta_bias, bool(delta_softplus), state, None)
+                                             skip, delta_bias, softplus, state, None)
         out.copy_(last)
         return y.squeeze(1), out
     return _ops.get_ext().selective_scan_step(_rows(u), _rows(delta), A, _rows(B), _rows(C), state, out, skip,
-                                              delta_bias, bool(delta_softplus)), out
+                                              delta_bias, softplus), out
 
 
 # ---- norms around a block ---------------------------------------------------
@@ -404,6 +426,10 @@ def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=N
     residual. h feeds the second norm unrounded. Returns p without a residual,
     h without pre_weight, else (y, h): p and y of x's type, h of the residual's.
     """
+    if _on_gpu(x):
+        out = _ops.get_ext().block_norm_direct(x, gate, post_weight, residual, scale, pre_weight, eps)
+        if out is not None:
+            return out
     _check_act(x, "x", None)
     if x.dim() < 1:
         raise ValueError("x must have a channel axis")
