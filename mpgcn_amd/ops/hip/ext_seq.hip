@@ -225,7 +225,7 @@ std::vector<Tensor> selective_scan_fwd(Tensor u, Tensor delta, Tensor A, Tensor 
     auto h1 = want_state ? empty_f32(u, {p.B, p.D, p.N}) : Tensor();
     Tensor ck, seg_h, seg_s;
     if (p.B && p.D && (p.L || want_state)) {
-        const ScanPlan l = scan_plan(p, f32(u));
+        const ScanPlan l = scan_plan(p, f32(u), 0);
         const long tasks = l.groups * p.G * l.cb;
         // one chunk starts from the state given: nothing to keep
         if (train && l.chunks > 1) ck = empty_f32(u, {tasks, l.chunks, l.state});
@@ -263,7 +263,7 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
                                    s.narrow(0, D * N + D, D), dh0};
     };
     if (!B || !D) return split(torch::zeros({D * (N + 2)}, A.options()));
-    const ScanPlan l = scan_plan(p, f32(u));
+    const ScanPlan l = scan_plan(p, f32(u), 1);
     const long tasks = l.groups * G * l.cb;
     if (l.chunks > 1) {
         TORCH_CHECK(has(ck), "the forward kept no chunk states");

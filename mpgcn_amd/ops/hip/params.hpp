@@ -282,7 +282,7 @@ void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
 void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out, const float* w,
                             const float* bias, void* y, long B, int D, int K, int silu, int is_f32,
                             int vec, hipStream_t s);
-ScanPlan scan_plan(const ScanParams& p, int is_f32);
+ScanPlan scan_plan(const ScanParams& p, int is_f32, int back);
 void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32, hipStream_t s);
