@@ -271,7 +271,9 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     }
     auto ws = empty_f32(u, {l.slots, D * (N + 2)});
     auto sums = empty_f32(u, {D * (N + 2)});
-    auto dbc = empty_f32(u, {l.cb, B, G, l.chunks, 8, 2, l.state / (4 * l.cw * l.rw) * 4});
+    // one channel block leaves nothing to add up
+    Tensor dbc;
+    if (l.cb > 1) dbc = empty_f32(u, {l.cb, B, G, l.chunks, 8, 2, l.state / (4 * l.cw * l.rw) * 4});
     Tensor seg_h, seg_s;
     if (l.nseg > 1) {
         seg_h = empty_f32(u, {tasks, l.nseg, l.state});
@@ -287,12 +289,14 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     p.du = du.data_ptr();
     p.ddelta = dd.data_ptr();
     p.ckpt = has(ck) ? ck->data_ptr<float>() : nullptr;
-    p.dbc = dbc.data_ptr<float>();
+    p.dbc = dbc.defined() ? dbc.data_ptr<float>() : nullptr;
+    p.dB = dB.data_ptr();
+    p.dC = dC.data_ptr();
     p.ws = ws.data_ptr<float>();
     p.dh0 = want_state ? dh0.data_ptr<float>() : nullptr;
     scan_bwd_launch(p, l, f32(u), stream());
     seq_colsum_launch(p.ws, sums.data_ptr<float>(), l.slots, D * (N + 2), stream());
-    if (L) scan_bc_reduce_launch(p, l, dB.data_ptr(), dC.data_ptr(), f32(u), stream());
+    if (L && p.dbc) scan_bc_reduce_launch(p, l, f32(u), stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return split(sums);
 }

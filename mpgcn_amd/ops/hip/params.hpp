@@ -217,7 +217,8 @@ struct ScanParams {
     const void* dy;      // (B, L, D) contiguous
     const float* dh1;    // (B, D, N) or null
     void *du, *ddelta;   // (B, L, D) contiguous
-    float* dbc;          // (cblocks, B, G, chunks, 8, 2, N padded) partial dB | dC
+    void *dB, *dC;       // (B, L, G, N) contiguous
+    float* dbc;          // (cblocks, B, G, chunks, 8, 2, N padded) partial dB | dC, or null: one block
     float* ws;           // (slots, D*N + 2*D) partial dA | dskip | dbias
     float* dh0;          // (B, D, N) or null
     long u_b, d_b, B_b, B_g, C_b, C_g;
@@ -285,7 +286,7 @@ void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_o
 ScanPlan scan_plan(const ScanParams& p, int is_f32, int back);
 void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
-void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32, hipStream_t s);
+void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s);
 int block_norm_slots(long R, long D, int res, int gate);
 void block_norm_fwd_launch(const BlockNormParams& p, int is_f32, int res_f32, hipStream_t s);

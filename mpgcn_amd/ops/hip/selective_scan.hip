@@ -447,7 +447,8 @@ struct Item {
 };
 
 // A chunk's inputs on their way: of u, delta, dy, B and C those asked for.
-template <typename T, int NQ, int KQ, bool V, bool U, bool DY, bool B, bool C>
+// LEAN: lane offsets are worked out anew for every chunk.
+template <typename T, int NQ, int KQ, bool V, bool LEAN, bool U, bool DY, bool B, bool C>
 struct Inputs {
     using RowsT = Rows<T, KQ, V>;
     using StatesT = States<T, NQ, KQ, V>;
@@ -457,7 +458,7 @@ struct Inputs {
     __device__ __forceinline__ void read(const Work& w, const Item& m, int ck) {
         const ScanArgs a = args();
         const ScanParams& p = a.p;
-        const int lane = fresh_lane();
+        const int lane = LEAN ? fresh_lane() : threadIdx.x & 63;
         const long t0 = (long)ck * SCAN_CH;
         const int last = (int)(p.L - 1 - t0);
         if (U)
@@ -474,7 +475,7 @@ struct Inputs {
     // dyt: where dy goes
     template <typename Tl>
     __device__ __forceinline__ void stage(const Item& m, int ck, int cw, Tl& tile, T (*dyt)[RowsT::CH]) {
-        const int lane = fresh_lane(), t0 = ck * SCAN_CH;
+        const int lane = LEAN ? fresh_lane() : threadIdx.x & 63, t0 = ck * SCAN_CH;
         lds_order();
         if (U) RowsT::stage(cw, lane, u, m.len0 - t0, m.len1 - t0, tile.u);
         RowsT::stage(cw, lane, de, m.len0 - t0, m.len1 - t0, tile.de);
@@ -514,7 +515,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
         skip = a0.p.skip ? ((gmem<const float>)a0.p.skip)[q.d] : 0.f;
         dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
     }
-    Inputs<T, NQ, KQ, V, true, false, true, MAIN> in;
+    Inputs<T, NQ, KQ, V, false, true, false, true, MAIN> in;
     Item m(a0, w, w.slot, nseg, 0);
     if (m.c0 < m.c1) in.read(w, m, m.c0);
     for (int it = w.slot; it < items; it += step) {
@@ -567,7 +568,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
             if (MAIN) {
                 const ScanArgs a = args();
                 lds_order();
-                Rows<T, KQ, V>::write(a.p, a.l, fresh_lane(), w.g, w.cblk, (T*)a.p.y + (m.b0 * L + t0) * a.p.D, L - t0,
+                Rows<T, KQ, V>::write(a.p, a.l, lane, w.g, w.cblk, (T*)a.p.y + (m.b0 * L + t0) * a.p.D, L - t0,
                                       m.two, tile.u);
             }
         }
@@ -656,7 +657,7 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
     load_decay(a0.p, q, A2);
     const float dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
 
-    Inputs<T, NQ, KQ, V, false, true, false, true> in;
+    Inputs<T, NQ, KQ, V, false, false, true, false, true> in;
     Item m(a0, w, w.slot, nseg, 1);
     in.read(w, m, m.c1 - 1);
     for (int it = w.slot; it < items; it += step) {
@@ -697,6 +698,30 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
     }
 }
 
+// A chunk's dB and dC where one channel block has all of their terms.
+template <typename T, int NQ, int KQ, bool V>
+__device__ __forceinline__ void write_bc(const ScanParams& p, int lane, int g, long b0, int t0, bool two,
+                                         const TileBack<T, NQ, KQ>& tile) {
+    using TileT = typename TileBack<T, NQ, KQ>::B;
+    constexpr int NP = TileT::NP, PR = NP / 4, P = TileT::RW * SCAN_CH * 2 * PR;  // four states a piece
+#pragma unroll
+    for (int k = 0; k < (P + 63) / 64; ++k) {
+        const int i = k * 64 + lane;
+        const int n0 = i % PR * 4, which = i / PR % 2, j = i / (PR * 2) % SCAN_CH, rs = i / (PR * 2 * SCAN_CH);
+        if ((P % 64 && i >= P) || t0 + j >= p.L || (rs && !two)) continue;
+        const f32x4 v = ((const f32x4*)tile.dbc)[i];
+        const auto o = (gmem<T>)(which ? p.dC : p.dB) + (((b0 + rs) * p.L + t0 + j) * p.G + g) * p.N + n0;
+        if constexpr (V) {
+            typedef __attribute__((ext_vector_type(4))) T four;
+            *(gmem<four>)o = four{from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n0 + e < p.N) o[e] = from_f32<T>(v[e]);
+        }
+    }
+}
+
 template <typename T, int NQ, int KQ, bool V>
 __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
     using RowsT = Rows<T, KQ, V>;
@@ -729,7 +754,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
     const int obc = q.rs * (SCAN_CH * 2 * NP) + (idx >= NQ ? NP : 0) + q.n0 + (idx & (NQ - 1));
 
     // what the next chunk starts from: its inputs and the state before it
-    Inputs<T, NQ, KQ, V, true, true, true, true> in;
+    Inputs<T, NQ, KQ, V, true, true, true, true, true> in;
     f32x4 next_h[NQ];
     auto read_h = [&](const Item& m, int ck) {
         const ScanArgs a = args();
@@ -836,6 +861,10 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
             const int ln = fresh_lane();
             RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.du + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.u);
             RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.ddelta + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.de);
+            if (!a.p.dbc) {
+                write_bc<T, NQ, KQ, V>(a.p, ln, w.g, m.b0, t0, m.two, tile);
+                continue;
+            }
             const long row = (((long)w.cblk * a.p.B + m.b0) * a.p.G + w.g) * a.l.chunks + ck;
             constexpr int PC = SCAN_CH * 2 * NP / 4;  // 16-byte pieces of a chunk
 #pragma unroll
@@ -1082,16 +1111,16 @@ extern "C" void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f
     by_states(p.N, Typed<ScanBwd>{ScanBwd{p, l, s}, is_f32});
 }
 
-extern "C" void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, void* dB, void* dC, int is_f32,
+extern "C" void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, int is_f32,
                                       hipStream_t s) {
     const int NP = l.state / (4 * l.cw * l.rw) * 4;
     const long rows = (long)p.B * p.L * p.G;
     const dim3 grid((unsigned)((rows * (2 * NP / 4) + 255) / 256));
     if (is_f32) {
-        hipLaunchKernelGGL((scan_bc_reduce_kernel<float>), grid, dim3(256), 0, s, p.dbc, (float*)dB, (float*)dC, l.cb, rows,
+        hipLaunchKernelGGL((scan_bc_reduce_kernel<float>), grid, dim3(256), 0, s, p.dbc, (float*)p.dB, (float*)p.dC, l.cb, rows,
                            p.B, p.L, p.G, p.N, NP);
     } else {
-        hipLaunchKernelGGL((scan_bc_reduce_kernel<__bf16>), grid, dim3(256), 0, s, p.dbc, (__bf16*)dB, (__bf16*)dC, l.cb,
+        hipLaunchKernelGGL((scan_bc_reduce_kernel<__bf16>), grid, dim3(256), 0, s, p.dbc, (__bf16*)p.dB, (__bf16*)p.dC, l.cb,
                            rows, p.B, p.L, p.G, p.N, NP);
     }
 }
