@@ -40,6 +40,10 @@ __launch_bounds__(256) __global__ void row_gemm_kernel(RowGemmParams p, int nf16
         const int n = idx / KP, k = idx % KP;
         if (n >= p.N || k >= p.K) ldsWT[n * KP + k] = (T)0.f;
     }
+    // and the slack that the k tail of the last row's fragments reads into:
+    // those terms meet zeros of A, but 0 * NaN is NaN
+    for (int idx = tid; idx < 64 / (int)sizeof(T); idx += 256)
+        ldsWT[nf16 * 16 * KP + idx] = (T)0.f;
     __syncthreads();
 
     const int w = tid / WAVE, lane = tid % WAVE;
