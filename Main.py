@@ -72,6 +72,10 @@ def build_parser() -> argparse.ArgumentParser:
                         choices=["mean", "attention"], default="mean",
                         help="branch fusion: arithmetic mean (reference) or "
                              "learned attention weights")
+    parser.add_argument("-temporal", "--temporal", type=str,
+                        choices=["lstm", "selective"], default="lstm",
+                        help="temporal encoder of each branch: LSTM (reference) "
+                             "or selective state space scan")
     parser.add_argument("-ref-quirks", "--ref_quirks", action="store_true",
                         help="reproduce the reference's dynamic D-graph "
                              "computation exactly (Data_Container_OD.py:53-56 "

@@ -24,6 +24,7 @@ import torch
 from torch import nn
 
 from mpgcn_amd.models.bdgcn import BDGCN
+from mpgcn_amd.models.selective import SelectiveEncoder
 from mpgcn_amd.ops import GraphOperator, fused_lstm_last, linear_act
 
 
@@ -65,8 +66,10 @@ class MPGCN(nn.Module):
                  lstm_num_layers: int, gcn_hidden_dim: int, gcn_num_layers: int,
                  num_nodes: int, user_bias: bool = True, activation: str = "relu",
                  compute_dtype: torch.dtype = torch.float32, fusion: str = "mean",
-                 fp8_forward: bool = False):
+                 fp8_forward: bool = False, temporal: str = "lstm"):
         super().__init__()
+        if temporal not in ("lstm", "selective"):
+            raise ValueError("temporal must be 'lstm' or 'selective'")
         if lstm_num_layers != 1:
             raise ValueError("MPGCN uses a 1-layer LSTM (Model_Trainer.py:50)")
         if fusion not in ("mean", "attention"):
@@ -86,6 +89,7 @@ class MPGCN(nn.Module):
                     "(ops/functional.py fp8_forward_compatible)")
         self.fp8_forward = fp8_forward
         self.M = M
+        self.temporal = temporal
         self.fusion = fusion
         self.K = K
         self.num_nodes = num_nodes
@@ -98,7 +102,9 @@ class MPGCN(nn.Module):
         self.branch_models = nn.ModuleList()
         for _ in range(M):
             branch = nn.ModuleDict()
-            branch["temporal"] = TemporalEncoder(input_dim, lstm_hidden_dim)
+            # 'lstm' keeps the reference's state_dict; 'selective' has its own
+            encoder = TemporalEncoder if temporal == "lstm" else SelectiveEncoder
+            branch["temporal"] = encoder(input_dim, lstm_hidden_dim)
             branch["spatial"] = nn.ModuleList()
             for n in range(gcn_num_layers):
                 cur_in = lstm_hidden_dim if n == 0 else gcn_hidden_dim

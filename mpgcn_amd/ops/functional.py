@@ -804,7 +804,9 @@ class _LinearActFn(torch.autograd.Function):
     def backward(ctx, dOut):
         X2d, weight, out = ctx.saved_tensors
         dY = (dOut * (out > 0).to(dOut.dtype) if ctx.relu else dOut).contiguous()
-        if weight.shape[0] == 1:
+        if not ctx.needs_input_grad[0]:
+            dX = None
+        elif weight.shape[0] == 1:
             # rank-1 head (the MPGCN FC): the outer product is a broadcast
             # multiply — rocBLAS spends ~250us + a workspace memset on it
             dX = dY * weight.to(dY.dtype).reshape(1, -1)

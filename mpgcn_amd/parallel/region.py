@@ -31,7 +31,6 @@ import torch.distributed as dist
 
 from mpgcn_amd.ops import (
     GraphOperator,
-    fused_lstm_last,
     linear_act,
     mode1_proj,
     mode2_bias_act,
@@ -281,14 +280,7 @@ def mpgcn_forward_sharded(model, x_seq_shard, G_list, group=None):
     outs = []
     for m in range(model.M):
         branch = model.branch_models[m]
-        h = fused_lstm_last(
-            lstm_in,
-            branch["temporal"].weight_ih_l0.to(cd),
-            branch["temporal"].weight_hh_l0.to(cd),
-            branch["temporal"].bias_ih_l0,
-            branch["temporal"].bias_hh_l0,
-            T=T,
-        )
+        h = branch["temporal"](lstm_in, T)
         X = h.reshape(B, N, Nl, model.lstm_hidden_dim)
         gop = gops[m]
         if fp8:

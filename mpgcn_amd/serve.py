@@ -48,6 +48,7 @@ class Forecaster:
             num_nodes=N, compute_dtype=compute_dtype,
             fusion=params.get("fusion", "mean"),
             fp8_forward=fp8,
+            temporal=params.get("temporal", "lstm"),
         ).to(self.device)
         ckpt = torch.load(params["checkpoint"], map_location=self.device,
                           weights_only=False)
@@ -203,6 +204,8 @@ def _params_from_cli():
     ap.add_argument("-K", "--cheby_order", type=int, default=2)
     ap.add_argument("-dtype", "--compute_dtype", default="bf16")
     ap.add_argument("-M", "--perspectives", type=int, default=2)
+    ap.add_argument("-temporal", "--temporal", choices=["lstm", "selective"],
+                    default="lstm")
     ap.add_argument("-split", "--split_ratio", type=float, nargs="+",
                     default=[6.4, 1.6, 2])
     ap.add_argument("-port", "--port", type=int, default=8321)

@@ -90,6 +90,7 @@ class ModelTrainer:
             compute_dtype=self.compute_dtype,
             fusion=self.params.get("fusion", "mean"),
             fp8_forward=self.fp8_forward,
+            temporal=self.params.get("temporal", "lstm"),
         )
 
     def get_loss(self):
