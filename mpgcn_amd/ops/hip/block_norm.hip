@@ -33,43 +33,24 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* lds, int& slot
 }
 
 // Eight weights of a row's chunk; ones where there is no such weight.
-template <bool VEC>
-__device__ __forceinline__ void param8(const float* w, int c, int n, float (&v)[SEQ_CH]) {
+__device__ __forceinline__ void param8(const float* w, int c, int D, float (&v)[SEQ_CH]) {
 #pragma unroll
     for (int j = 0; j < SEQ_CH; ++j) v[j] = 1.f;
-    if (w && n > 0) load8<float, VEC>(w + c, n, v);
-}
-
-// Eight elements as they are in memory; zeros where there are none.
-template <typename T>
-struct Raw8 {
-    static constexpr int E = Pack<T>::E;
-    Pack<T> w[SEQ_CH / E];
-    __device__ __forceinline__ float get(int j) const { return w[j / E].get(j % E); }
-};
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void raw8(const void* base, long at, int n, Raw8<T>& r) {
-    const T* p = (const T*)base + at;
-#pragma unroll
-    for (int i = 0; i < SEQ_CH / Raw8<T>::E; ++i) {
-        if (n > 0) r.w[i].template load<VEC>(p + i * Raw8<T>::E, n - i * Raw8<T>::E);
-        else r.w[i].w = i32x4{0, 0, 0, 0};
-    }
+    if (w && c < D) load8(w + c, D - c, D, v);
 }
 
 // The weights of a thread's columns: kept over its rows where it has one chunk,
 // else read where they are used, to leave the registers to the row.
-template <int VPT, bool VEC, bool RES>
+template <int VPT, bool RES>
 struct Weights {
     static constexpr bool KEEP = VPT == 1;
     float w[KEEP ? 3 : 1][SEQ_CH];
 
     __device__ __forceinline__ Weights(const BlockNormParams& p, int c) {
         if (!KEEP) return;
-        param8<VEC>(p.post, c, p.D - c, w[0]);
-        if (RES) param8<VEC>(p.scale, c, p.D - c, w[KEEP ? 1 : 0]);
-        if (RES) param8<VEC>(p.pre, c, p.D - c, w[KEEP ? 2 : 0]);
+        param8(p.post, c, p.D, w[0]);
+        if (RES) param8(p.scale, c, p.D, w[KEEP ? 1 : 0]);
+        if (RES) param8(p.pre, c, p.D, w[KEEP ? 2 : 0]);
     }
     // which: 0 post, 1 scale, 2 pre
     template <int WHICH>
@@ -78,14 +59,14 @@ struct Weights {
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) v[j] = w[KEEP ? WHICH : 0][j];
         } else {
-            param8<VEC>(from, c, D - c, v);
+            param8(from, c, D, v);
         }
     }
 };
 
 // The same for the backward, whose registers hold the column gradients: in LDS
 // where a thread has one chunk. Each thread reads back only what it put there.
-template <int VPT, bool VEC, bool RES>
+template <int VPT, bool RES>
 struct WeightsBack {
     static constexpr bool KEEP = VPT == 1;
     f32x4* mine;  // [3][2][blockDim]
@@ -99,7 +80,7 @@ struct WeightsBack {
     }
     __device__ __forceinline__ void keep(const float* from, int c, int D, int which) {
         float v[SEQ_CH];
-        param8<VEC>(from, c, D - c, v);
+        param8(from, c, D, v);
         mine[(which * 2) * blockDim.x] = f32x4{v[0], v[1], v[2], v[3]};
         mine[(which * 2 + 1) * blockDim.x] = f32x4{v[4], v[5], v[6], v[7]};
     }
@@ -115,14 +96,14 @@ struct WeightsBack {
                 v[4 + j] = b[j];
             }
         } else {
-            param8<VEC>(from, c, D - c, v);
+            param8(from, c, D, v);
         }
     }
 };
 
 // A thread keeps its columns and takes one row after another; with one chunk a
 // thread a row's loads are in flight while the row before is worked on.
-template <typename T, typename TR, int VPT, bool VEC, bool RES>
+template <typename T, typename TR, int VPT, bool RES>
 __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, int tpr) {
     __shared__ float lds[32];
     int slot = 0;
@@ -131,7 +112,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
     const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
     long r = (long)blockIdx.x * rpb + threadIdx.x / tpr;
 
-    const Weights<VPT, VEC, RES> wt(p, lane * SEQ_CH);
+    const Weights<VPT, RES> wt(p, lane * SEQ_CH);
     constexpr bool AHEAD = VPT == 1;
     Raw8<T> xr[VPT], gr[VPT];
     Raw8<TR> rr[VPT];
@@ -140,9 +121,9 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
             const int n = row < p.R ? p.D - c : 0;
-            raw8<T, VEC>(p.x, row * p.x_r + c, n, xr[i]);
-            if (p.gate) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
-            if (RES) raw8<TR, VEC>(p.res, row * p.r_r + c, n, rr[i]);
+            xr[i].load((const T*)p.x + row * p.x_r + c, n, p.D);
+            if (p.gate) gr[i].load((const T*)p.gate + row * p.g_r + c, n, p.D);
+            if (RES) rr[i].load((const TR*)p.res + row * p.r_r + c, n, p.D);
         }
     };
     if (AHEAD) read(r);
@@ -179,7 +160,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * tpr + lane) * SEQ_CH;
-                if (live && c < p.D) store8<T, VEC>((T*)p.y + r * p.D + c, p.D - c, v[i]);
+                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, p.D, v[i]);
             }
             continue;
         }
@@ -194,7 +175,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
                 hv[i][j] = fmaf(ws[j], v[i][j], hv[i][j]);  // zeros past the row's end
                 ss = fmaf(hv[i][j], hv[i][j], ss);
             }
-            if (live && c < p.D) store8<TR, VEC>((TR*)p.h + r * p.D + c, p.D - c, hv[i]);
+            if (live && c < p.D) store8<TR>((TR*)p.h + r * p.D + c, p.D - c, p.D, hv[i]);
         }
         if (p.pre) {
             const float inv = 1.f / sqrtf(row_sum(ss, tpr, lds, slot) * rd + p.eps);
@@ -206,7 +187,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
                 wt.template get<2>(p.pre, c, p.D, w2);
 #pragma unroll
                 for (int j = 0; j < SEQ_CH; ++j) hv[i][j] *= inv * w2[j];
-                if (live && c < p.D) store8<T, VEC>((T*)p.y + r * p.D + c, p.D - c, hv[i]);
+                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, p.D, hv[i]);
             }
         }
     }
@@ -219,7 +200,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 //   dp0 = inv1 (q - n1 mean(q n1));  dx, dgate by the product and silu'
 // Column gradients stay in registers over a thread's rows, are joined in LDS
 // over the block's row groups and written once per block.
-template <typename T, typename TR, int VPT, bool VEC, bool RES, bool GATE>
+template <typename T, typename TR, int VPT, bool RES, bool GATE>
 __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
     // the weights, then [rpb][VPT * tpr * SEQ_CH] to join the column gradients
     extern __shared__ __attribute__((aligned(16))) float dyn[];
@@ -230,7 +211,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
     const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
     long r = (long)blockIdx.x * rpb + rg;
 
-    const WeightsBack<VPT, VEC, RES> wt(p, lane * SEQ_CH, dyn);
+    const WeightsBack<VPT, RES> wt(p, lane * SEQ_CH, dyn);
     constexpr bool AHEAD = VPT == 1;
     float dpost[VPT][SEQ_CH] = {}, dscale[VPT][SEQ_CH] = {}, dpre[VPT][SEQ_CH] = {};
     Raw8<T> xr[VPT], gr[VPT], yr[VPT];
@@ -243,11 +224,11 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
             const int n = there ? p.D - c : 0;
-            raw8<T, VEC>(p.x, row * p.x_r + c, n, xr[i]);
-            if (GATE) raw8<T, VEC>(p.gate, row * p.g_r + c, n, gr[i]);
-            if (!RES || p.pre) raw8<T, VEC>(p.dy, row * p.D + c, p.dy ? n : 0, yr[i]);
-            if (RES && p.pre) raw8<TR, VEC>(p.res, row * p.r_r + c, n, rr[i]);
-            if (RES) raw8<TR, VEC>(p.dh, row * p.D + c, p.dh ? n : 0, hr[i]);
+            xr[i].load((const T*)p.x + row * p.x_r + c, n, p.D);
+            if (GATE) gr[i].load((const T*)p.gate + row * p.g_r + c, n, p.D);
+            if (!RES || p.pre) yr[i].load((const T*)p.dy + row * p.D + c, p.dy ? n : 0, p.D);
+            if (RES && p.pre) rr[i].load((const TR*)p.res + row * p.r_r + c, n, p.D);
+            if (RES) hr[i].load((const TR*)p.dh + row * p.D + c, p.dh ? n : 0, p.D);
         }
         if (p.post && there) i1 = p.inv1[row];
         if (RES && p.pre && there) i2 = p.inv2[row];
@@ -305,7 +286,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (RES && live && c < p.D) store8<TR, VEC>((TR*)p.dres + r * p.D + c, p.D - c, d[i]);
+            if (RES && live && c < p.D) store8<TR>((TR*)p.dres + r * p.D + c, p.D - c, p.D, d[i]);
             float w1[SEQ_CH], ws[SEQ_CH];
             wt.template get<0>(p.post, c, p.D, w1);
             if (RES) wt.template get<1>(p.scale, c, p.D, ws);
@@ -336,8 +317,8 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
                 }
             }
             if (live && c < p.D) {
-                store8<T, VEC>((T*)p.dx + r * p.D + c, p.D - c, o);
-                if (GATE) store8<T, VEC>((T*)p.dgate + r * p.D + c, p.D - c, og);
+                store8<T>((T*)p.dx + r * p.D + c, p.D - c, p.D, o);
+                if (GATE) store8<T>((T*)p.dgate + r * p.D + c, p.D - c, p.D, og);
             }
         }
     }
@@ -397,9 +378,9 @@ inline long row_blocks(long R, int tpr, int waves) {
 struct NormFwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool V, bool RES>
+    template <typename T, typename TR, int VPT, bool RES>
     void operator()(int tpr) const {
-        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, V, RES>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
+        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
                            dim3(block_threads(tpr)), 0, s, p, tpr);
     }
 };
@@ -407,14 +388,14 @@ struct NormFwd {
 struct NormBwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool V, bool RES>
+    template <typename T, typename TR, int VPT, bool RES>
     void operator()(int tpr) const {
         const int block = block_threads(tpr);
         const size_t smem = (size_t)block * SEQ_CH * sizeof(float) * (VPT > 1 ? VPT : RES ? 3 : 1);
         if (p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES, true>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, true>), dim3(p.slots), dim3(block), smem, s, p, tpr);
         if (!p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, V, RES, false>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, false>), dim3(p.slots), dim3(block), smem, s, p, tpr);
     }
 };
 
@@ -422,14 +403,9 @@ template <typename T, typename TR, bool RES, typename F>
 void by_shape(const BlockNormParams& p, F f) {
     int tpr, vpt;
     row_shape(p.D, &tpr, &vpt);
-    auto with = [&](auto v) {
-        constexpr bool V = decltype(v)::value;
-        if (vpt == 1) f.template operator()<T, TR, 1, V, RES>(tpr);
-        else if (vpt == 2) f.template operator()<T, TR, 2, V, RES>(tpr);
-        else f.template operator()<T, TR, 4, V, RES>(tpr);
-    };
-    if (p.vec) with(std::true_type{});
-    else with(std::false_type{});
+    if (vpt == 1) f.template operator()<T, TR, 1, RES>(tpr);
+    else if (vpt == 2) f.template operator()<T, TR, 2, RES>(tpr);
+    else f.template operator()<T, TR, 4, RES>(tpr);
 }
 
 template <typename F>

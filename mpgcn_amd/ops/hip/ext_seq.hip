@@ -58,16 +58,6 @@ void check_main(const Tensor& t, const char* name) {
     for (long s : t.sizes()) TORCH_CHECK(s <= INT_MAX / 2, name, ": extent too large");
 }
 
-// Rows of `t` can be read `elems` channels at a time, in pieces of 16 bytes at most.
-bool aligned(const Tensor& t, long elems) {
-    const long es = t.element_size(), step = elems * es < 16 ? elems * es : 16;
-    if ((uintptr_t)t.data_ptr() % step) return false;
-    for (long i = 0; i + 1 < t.dim(); ++i)
-        if (t.size(i) > 1 && t.stride(i) * es % step) return false;
-    return true;
-}
-bool aligned(const Opt& t, long elems) { return !has(t) || aligned(*t, elems); }
-
 Tensor empty_f32(const Tensor& like, at::IntArrayRef shape) {
     return torch::empty(shape, like.options().dtype(torch::kFloat));
 }
@@ -111,8 +101,7 @@ std::vector<Tensor> short_conv_fwd(Tensor x, Tensor w, Opt bias, Opt s0, Opt len
         p.y = y.data_ptr();
         p.s1 = want_state ? s1.data_ptr() : nullptr;
         short_conv_plan(&p, f32(x), 0);
-        const int vec = p.D % 8 == 0 && aligned(x, 8) && aligned(s0, 8);
-        short_conv_fwd_launch(p, (int)K, f32(x), vec, stream());
+        short_conv_fwd_launch(p, (int)K, f32(x), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return {y, s1};
@@ -140,8 +129,7 @@ std::vector<Tensor> short_conv_bwd(Tensor dy, Opt ds1, Tensor x, Tensor w, Opt b
     p.dx = dx.data_ptr();
     p.ds0 = want_state ? ds0.data_ptr() : nullptr;
     p.ws = ws.data_ptr<float>();
-    const int vec = D % 8 == 0 && aligned(x, 8) && aligned(s0, 8) && aligned(dy, 8) && aligned(ds1, 8);
-    short_conv_bwd_launch(p, (int)K, f32(x), vec, stream());
+    short_conv_bwd_launch(p, (int)K, f32(x), stream());
     seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, D * (K + 1), stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return {dx, sums.narrow(0, 0, D * K).view({D, K}), sums.narrow(0, D * K, D), ds0};
@@ -161,10 +149,9 @@ Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt b
     check_like(state_out, x, {B, K - 1, D}, "state_out");
     auto y = torch::empty({B, D}, x.options());
     if (B && D) {
-        const int vec = D % 8 == 0 && aligned(x, 8) && aligned(state, 8) && aligned(state_out, 8);
         short_conv_step_launch(x.data_ptr(), x.stride(0), state.data_ptr(), state_out.data_ptr(),
                                w.data_ptr<float>(), fptr(bias), y.data_ptr(), B, (int)D, (int)K, silu,
-                               f32(x), vec, stream());
+                               f32(x), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return y;
@@ -211,8 +198,6 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     p.C_b = Cm.stride(0); p.C_t = step(Cm); p.C_g = Cm.stride(2);
     p.B = (int)B; p.L = (int)L; p.D = (int)D; p.N = (int)N; p.G = (int)G;
     p.softplus = softplus ? 1 : 0;
-    p.rvec = D / G % 8 == 0 && aligned(u, 8) && aligned(delta, 8) && aligned(Bm, 8) && aligned(Cm, 8);
-    p.svec = aligned(h0, 4);
     return p;
 }
 
@@ -284,8 +269,6 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     const Tensor dyt = has(dy) ? *dy : torch::zeros({B, L, D}, u.options());
     p.dy = dyt.data_ptr();
     p.dh1 = fptr(dh1);
-    p.svec = p.svec && aligned(dh1, 4);
-    p.rvec = p.rvec && aligned(dyt, 8);
     p.du = du.data_ptr();
     p.ddelta = dd.data_ptr();
     p.ckpt = has(ck) ? ck->data_ptr<float>() : nullptr;
@@ -333,8 +316,6 @@ Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor C
         p.C_b = Cm.stride(0); p.C_g = grouped ? Cm.stride(1) : 0;
         p.B = (int)B; p.D = (int)D; p.N = (int)N; p.G = (int)G;
         p.softplus = softplus ? 1 : 0;
-        p.bvec = N % 4 == 0 && aligned(Bm, 4) && aligned(Cm, 4) && aligned(A, 4) && aligned(state, 4) &&
-                 aligned(state_out, 4);
         scan_step_launch(p, f32(u), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
@@ -374,8 +355,6 @@ BlockNormParams norm_params(const Tensor& x, const Opt& gate, const Opt& post, c
     p.R = R;
     p.D = (int)D;
     p.eps = (float)eps;
-    p.vec = D % 8 == 0 && aligned(x, 8) && aligned(gate, 8) && aligned(res, 8) && aligned(post, 8) &&
-            aligned(scale, 8) && aligned(pre, 8);
     return p;
 }
 
@@ -428,7 +407,6 @@ std::vector<Tensor> block_norm_bwd(Opt dy, Opt dh, Tensor x, Opt gate, Opt post,
         p.dgate = ptr(dg);
         p.dres = ptr(dr);
         p.ws = ws.data_ptr<float>();
-        p.vec = p.vec && aligned(dy, 8) && aligned(dh, 8);
         block_norm_bwd_launch(p, f32(x), has(res) ? f32(*res) : f32(x), stream());
         seq_colsum_launch(p.ws, sums.data_ptr<float>(), p.slots, nw * D, stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -225,8 +225,6 @@ struct ScanParams {
     int u_t, d_t, B_t, C_t;  // under 2^26 (checked: 8 of them are a lane's offset)
     int B, L, D, N, G;
     int softplus, lens64;
-    int rvec;            // 16-byte pieces of u, delta, Bm, Cm are whole and aligned
-    int svec;            // and of h0, dh1
 };
 
 // How a scan is laid over the card. A task is one wave's channels and
@@ -249,7 +247,6 @@ struct ScanStepParams {
     long u_b, d_b, B_b, B_g, C_b, C_g;
     int B, D, N, G;
     int softplus;
-    int bvec;            // N a multiple of 4 and every row of Bm/Cm, A, h aligned for it
 };
 
 struct BlockNormParams {
@@ -271,18 +268,16 @@ struct BlockNormParams {
     long R;
     int D;
     float eps;
-    int vec;             // every row of every tensor can be read 16 bytes at a time
     int slots;
 };
 
 extern "C" {
 void seq_colsum_launch(const float* ws, float* out, long nb, long E, hipStream_t s);
-void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
+void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, hipStream_t s);
 void short_conv_plan(ShortConvParams* p, int is_f32, int back);
-void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec, hipStream_t s);
+void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, hipStream_t s);
 void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out, const float* w,
-                            const float* bias, void* y, long B, int D, int K, int silu, int is_f32,
-                            int vec, hipStream_t s);
+                            const float* bias, void* y, long B, int D, int K, int silu, int is_f32, hipStream_t s);
 ScanPlan scan_plan(const ScanParams& p, int is_f32, int back);
 void scan_fwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);
 void scan_bwd_launch(const ScanParams& p, const ScanPlan& l, int is_f32, hipStream_t s);

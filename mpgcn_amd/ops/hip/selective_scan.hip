@@ -177,28 +177,37 @@ __device__ __forceinline__ void load_decay(const ScanParams& p, const Place<NQ, 
 }
 
 // The lane's states in a (B, D, N) tensor, or zeros, for a wave whose first
-// sequence is b0. VS: a channel's four are one aligned piece.
-template <bool VS, int NQ, int KQ>
+// sequence is b0.
+template <int NQ, int KQ>
 __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ, KQ>& q, const float* s, long b0,
                                             f32x4 (&h)[NQ]) {
-    const long b = b0 + q.rs;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) h[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (!s) return;
+    const long b = b0 + q.rs;
     // addresses and masks are formed here, not kept over the loop around
     int d4 = q.d4, nd = q.nd, n0 = q.n0;
     asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
     nd = b < p.B ? nd : 0;
-    if (VS && NQ == 4 && p.svec) {
-        // Unmasked, so that nothing waits for the loads here. VS has all four
-        // channels or none, and one there is not reads the first sequence's of
+    if (NQ == 4 && p.N == Place<NQ, KQ>::NP && p.D / p.G % 4 == 0) {
+        // Unmasked, so that nothing waits for the loads here. All four channels
+        // are there or none, and those that are not read the first sequence's of
         // the wave: states that meet only zeros and are not stored.
         s += ((b < p.B ? b : b0) * p.D + d4) * p.N + n0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const f32x4 v = *(gmem<const f32x4>)(s + (long)c * p.N);
+            const i32x4 v = *(gmem<const any16>)(s + (long)c * p.N);
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) h[i][c] = v[i & 3];
+            for (int i = 0; i < NQ; ++i) h[i][c] = __int_as_float(v[i & 3]);
+        }
+    } else if (NQ == 4) {
+        s += b < p.B ? (b * p.D + d4) * p.N + (n0 < p.N ? n0 : 0) : 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            Pack<float> v;
+            v.load(s + (long)c * p.N, c < nd ? p.N - n0 : 0, p.N % 4);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) h[i][c] = v.get(i & 3);
         }
     } else {
 #pragma unroll
@@ -207,27 +216,28 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
             for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, c < nd && n0 + i < p.N, (b * p.D + d4 + c) * p.N + n0 + i);
     }
 }
-template <bool VS, int NQ, int KQ>
-__device__ __forceinline__ void store_states(const ScanParams& p, const Place<NQ, KQ>& q, float* s, long b,
+template <int NQ, int KQ>
+__device__ __forceinline__ void store_states(const ScanParams& p, const Place<NQ, KQ>& q, float* s, long b0,
                                              const f32x4 (&h)[NQ]) {
+    const long b = b0 + q.rs;
     int d4 = q.d4, nd = q.nd, n0 = q.n0;
     asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
     if (b >= p.B) return;
     s += (b * p.D + d4) * p.N + n0;
-    if (VS && NQ == 4) {
+    if (NQ == 4) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            f32x4 v;
+            Pack<float> v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = h[i & (NQ - 1)][c];
-            if (c < nd) *(gmem<f32x4>)(s + c * p.N) = v;
+            for (int i = 0; i < 4; ++i) v.w[i] = __float_as_int(h[i & (NQ - 1)][c]);
+            v.store(s + (long)c * p.N, c < nd ? p.N - n0 : 0, p.N % 4);
         }
     } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
-                if (c < nd && n0 + i < p.N) ((gmem<float>)s)[c * p.N + i] = h[i][c];
+                if (c < nd && n0 + i < p.N) ((gmem<float>)s)[(long)c * p.N + i] = h[i][c];
     }
 }
 // the same in the order of a wave's lanes: 16 bytes a lane, NQ rows of them
@@ -301,36 +311,23 @@ __device__ __forceinline__ void lds_order() {
     asm volatile("" ::: "memory");
 }
 
-// A piece of a row, 16 bytes or a whole shorter row, n elements of it there. V: at once.
-template <typename T, int E, bool V>
-__device__ __forceinline__ void read_piece(const T* base, unsigned off, int n, T (&v)[E]) {
-    const auto s = (gmem<const T>)((gmem<const char>)base + off);
-    if constexpr (V && E * sizeof(T) == 16) {
-        *(i32x4*)v = *(gmem<const i32x4>)s;
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = e < n ? s[e] : (T)0.f;
-    }
-}
-
 // One (8 steps) x (the wave's channels) tensor.
-template <typename T, int KQ, bool V>
+template <typename T, int KQ>
 struct Rows {
-    static constexpr int CH = 64 / KQ, E = 16 / sizeof(T), PR = CH / E, P = SCAN_CH * PR;
+    static constexpr int CH = 64 / KQ, E = Pack<T>::E, PR = CH / E, P = SCAN_CH * PR;
     static constexpr int K = (P + 63) / 64;  // pieces a lane
-    struct Raw { alignas(16) T v[K][E]; };
+    struct Raw { Pack<T> v[K]; };
 
     // piece k of the lane: its step, sequence, first channel of the tensor, elements there
-    static __device__ __forceinline__ bool piece(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk, int k,
+    static __device__ __forceinline__ void piece(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk, int k,
                                                  int& row, int& rs, int& d, int& n) {
         const int i = k * 64 + lane;
         row = i / PR;
         const int col = i % PR * E;
         rs = col >= l.cw ? 1 : 0;
         const int per = p.D / p.G, c = cblk * l.cw + col - rs * l.cw;
-        n = per - c > E ? E : per - c;
-        d = g * per + (n > 0 ? c : 0);
-        return (P % 64 == 0 || i < P) && n > 0;
+        n = (P % 64 == 0 || i < P) && c < per ? per - c : 0;
+        d = g * per + (n ? c : 0);
     }
     // base: the wave's first sequence at the chunk's first step; last: the last step there is from it
     static __device__ __forceinline__ void read(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk,
@@ -338,11 +335,11 @@ struct Rows {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             int row, rs, d, n;
-            const bool ok = piece(p, l, lane, g, cblk, k, row, rs, d, n);
+            piece(p, l, lane, g, cblk, k, row, rs, d, n);
             row = row < last ? row : last;
             const unsigned off =
                 ((rs && two ? (unsigned)b_stride : 0u) + (unsigned)row * (unsigned)t_stride + (unsigned)d) * (unsigned)sizeof(T);
-            read_piece<T, E, V>(base, ok ? off : 0, ok ? n : 0, r.v[k]);
+            r.v[k].load((const T*)((const char*)base + off), n, p.D / p.G % E);
         }
     }
     static __device__ __forceinline__ void stage(int cw, int lane, const Raw& r, int live0, int live1, T (*tile)[CH]) {
@@ -350,10 +347,10 @@ struct Rows {
         for (int k = 0; k < K; ++k) {
             const int i = k * 64 + lane, row = i / PR;
             const bool on = row < (i % PR * E >= cw ? live1 : live0);
-            Chunk16 c = *(const Chunk16*)r.v[k];
+            i32x4 c;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c.v[j] = on ? c.v[j] : 0;
-            if (P % 64 == 0 || i < P) *(Chunk16*)((T*)tile + i * E) = c;
+            for (int j = 0; j < 4; ++j) c[j] = on ? r.v[k].w[j] : 0;
+            if (P % 64 == 0 || i < P) *(i32x4*)((T*)tile + i * E) = c;
         }
     }
     // back out: rows below `rows`, of a contiguous (B, L, D) tensor
@@ -362,27 +359,22 @@ struct Rows {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             int row, rs, d, n;
-            if (!piece(p, l, lane, g, cblk, k, row, rs, d, n) || row >= rows || (rs && !two)) continue;
-            const auto o = (gmem<T>)base + ((rs ? (long)p.L : 0) + row) * p.D + d;
-            const T* s = (const T*)tile + (k * 64 + lane) * E;
-            if constexpr (V) {
-                *(gmem<i32x4>)o = *(const i32x4*)s;
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e < n) o[e] = s[e];
-            }
+            piece(p, l, lane, g, cblk, k, row, rs, d, n);
+            if (n == 0 || row >= rows || (rs && !two)) continue;
+            const i32x4 c = *(const i32x4*)((const T*)tile + (k * 64 + lane) * E);
+            const Pack<T> v{c};
+            v.store(base + ((rs ? (long)p.L : 0) + row) * p.D + d, n, p.D / p.G % E);
         }
     }
 };
 
 // The chunk's rows of B or of C, to f32.
-template <typename T, int NQ, int KQ, bool V>
+template <typename T, int NQ, int KQ>
 struct States {
     static constexpr int NP = 4 * NQ * KQ, RW = KQ == 1 ? 2 : 1;
     static constexpr int E = NP * sizeof(T) < 16 ? NP : 16 / sizeof(T), PR = NP / E, P = SCAN_CH * RW * PR;
     static constexpr int K = (P + 63) / 64;
-    struct Raw { alignas(16) T v[K][E]; };
+    struct Raw { Pack<T, E> v[K]; };
 
     static __device__ __forceinline__ void read(const ScanParams& p, int lane, const T* base, long b_stride, int t_stride,
                                                 int last, bool two, Raw& r) {
@@ -392,10 +384,10 @@ struct States {
             const int rs = RW == 2 && two ? i / PR % RW : 0;
             int row = i / (PR * RW);
             row = row < last ? row : last;
-            const int n = p.N - e0;
+            const int n = p.N > e0 ? p.N - e0 : 0;
             const unsigned off = ((rs ? (unsigned)b_stride : 0u) + (unsigned)row * (unsigned)t_stride +
-                                  (unsigned)(n > 0 ? e0 : 0)) * (unsigned)sizeof(T);
-            read_piece<T, E, V>(base, off, n, r.v[k]);
+                                  (unsigned)(n ? e0 : 0)) * (unsigned)sizeof(T);
+            r.v[k].load((const T*)((const char*)base + off), n, p.N % E);
         }
     }
     static __device__ __forceinline__ void stage(int lane, const Raw& r, int which, int live0, int live1,
@@ -404,12 +396,14 @@ struct States {
         for (int k = 0; k < K; ++k) {
             const int i = k * 64 + lane, e0 = i % PR * E, rs = i / PR % RW, row = i / (PR * RW);
             const bool on = row < (rs ? live1 : live0);
-            float v[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = on ? to_f32(r.v[k][e]) : 0.f;
             if (P % 64 == 0 || i < P) {
 #pragma unroll
-                for (int e = 0; e < E; e += 4) *(f32x4*)&tile[row][rs][which][e0 + e] = *(const f32x4*)(v + e);
+                for (int e = 0; e < E; e += 4) {
+                    f32x4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = on ? r.v[k].get(e + j) : 0.f;
+                    *(f32x4*)&tile[row][rs][which][e0 + e] = v;
+                }
             }
         }
     }
@@ -448,10 +442,10 @@ struct Item {
 
 // A chunk's inputs on their way: of u, delta, dy, B and C those asked for.
 // LEAN: lane offsets are worked out anew for every chunk.
-template <typename T, int NQ, int KQ, bool V, bool LEAN, bool U, bool DY, bool B, bool C>
+template <typename T, int NQ, int KQ, bool LEAN, bool U, bool DY, bool B, bool C>
 struct Inputs {
-    using RowsT = Rows<T, KQ, V>;
-    using StatesT = States<T, NQ, KQ, V>;
+    using RowsT = Rows<T, KQ>;
+    using StatesT = States<T, NQ, KQ>;
     typename RowsT::Raw u, de, dy;
     typename StatesT::Raw Br, Cr;
 
@@ -490,7 +484,7 @@ struct Inputs {
 
 // MAIN: outputs, chunk states, final state. Otherwise the end state of a
 // segment from zero and its summed step size.
-template <typename T, int NQ, int KQ, bool V, bool MAIN>
+template <typename T, int NQ, int KQ, bool MAIN>
 __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
     __shared__ Tile<T, NQ, KQ> tiles[4];
     Tile<T, NQ, KQ>& tile = tiles[wave_id()];
@@ -515,7 +509,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
         skip = a0.p.skip ? ((gmem<const float>)a0.p.skip)[q.d] : 0.f;
         dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
     }
-    Inputs<T, NQ, KQ, V, false, true, false, true, MAIN> in;
+    Inputs<T, NQ, KQ, false, true, false, true, MAIN> in;
     Item m(a0, w, w.slot, nseg, 0);
     if (m.c0 < m.c1) in.read(w, m, m.c0);
     for (int it = w.slot; it < items; it += step) {
@@ -524,7 +518,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
         {
             const ScanArgs a = args();
             if (MAIN && nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, h);
-            else load_states<V>(a.p, q, MAIN ? a.p.h0 : nullptr, m.b0, h);
+            else load_states(a.p, q, MAIN ? a.p.h0 : nullptr, m.b0, h);
         }
         float total = 0.f;
         for (int ck = m.c0; ck < m.c1; ++ck) {
@@ -568,7 +562,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
             if (MAIN) {
                 const ScanArgs a = args();
                 lds_order();
-                Rows<T, KQ, V>::write(a.p, a.l, lane, w.g, w.cblk, (T*)a.p.y + (m.b0 * L + t0) * a.p.D, L - t0,
+                Rows<T, KQ>::write(a.p, a.l, lane, w.g, w.cblk, (T*)a.p.y + (m.b0 * L + t0) * a.p.D, L - t0,
                                       m.two, tile.u);
             }
         }
@@ -577,7 +571,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
             store_lanes<NQ>(a.p.seg_h, m.id * a.l.nseg + m.seg, lane, h);
             ((gmem<float>)a.p.seg_s)[(m.id * a.l.nseg + m.seg) * 64 + lane] = total;
         } else if (a.p.h1 && m.seg == a.l.nseg - 1) {
-            store_states<V>(a.p, q, a.p.h1, m.b0 + q.rs, h);
+            store_states(a.p, q, a.p.h1, m.b0, h);
         }
         if (it + step < items) m = Item(a, w, it + step, nseg, 0);
     }
@@ -642,7 +636,7 @@ __launch_bounds__(256) __global__ void scan_carry_kernel(ScanParams p, ScanPlan 
 // one the forward kept at its start and held in registers.
 
 // The adjoint that a segment hands to the one before it, from zero at its end.
-template <typename T, int NQ, int KQ, bool V>
+template <typename T, int NQ, int KQ>
 __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
     __shared__ Tile<T, NQ, KQ> tiles[4];
     Tile<T, NQ, KQ>& tile = tiles[wave_id()];
@@ -657,7 +651,7 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
     load_decay(a0.p, q, A2);
     const float dbias = a0.p.dbias ? ((gmem<const float>)a0.p.dbias)[q.d] : 0.f;
 
-    Inputs<T, NQ, KQ, V, false, false, true, false, true> in;
+    Inputs<T, NQ, KQ, false, false, true, false, true> in;
     Item m(a0, w, w.slot, nseg, 1);
     in.read(w, m, m.c1 - 1);
     for (int it = w.slot; it < items; it += step) {
@@ -699,7 +693,7 @@ __launch_bounds__(256) __global__ void scan_adjoint_kernel(ScanArgs) {
 }
 
 // A chunk's dB and dC where one channel block has all of their terms.
-template <typename T, int NQ, int KQ, bool V>
+template <typename T, int NQ, int KQ>
 __device__ __forceinline__ void write_bc(const ScanParams& p, int lane, int g, long b0, int t0, bool two,
                                          const TileBack<T, NQ, KQ>& tile) {
     using TileT = typename TileBack<T, NQ, KQ>::B;
@@ -710,21 +704,17 @@ __device__ __forceinline__ void write_bc(const ScanParams& p, int lane, int g, l
         const int n0 = i % PR * 4, which = i / PR % 2, j = i / (PR * 2) % SCAN_CH, rs = i / (PR * 2 * SCAN_CH);
         if ((P % 64 && i >= P) || t0 + j >= p.L || (rs && !two)) continue;
         const f32x4 v = ((const f32x4*)tile.dbc)[i];
-        const auto o = (gmem<T>)(which ? p.dC : p.dB) + (((b0 + rs) * p.L + t0 + j) * p.G + g) * p.N + n0;
-        if constexpr (V) {
-            typedef __attribute__((ext_vector_type(4))) T four;
-            *(gmem<four>)o = four{from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n0 + e < p.N) o[e] = from_f32<T>(v[e]);
-        }
+        const float f[4] = {v[0], v[1], v[2], v[3]};
+        Pack<T, 4> o;
+        o.set(f);
+        o.store((T*)(which ? p.dC : p.dB) + (((b0 + rs) * p.L + t0 + j) * p.G + g) * p.N + (n0 < p.N ? n0 : 0),
+                n0 < p.N ? p.N - n0 : 0, p.N % 4);
     }
 }
 
-template <typename T, int NQ, int KQ, bool V>
+template <typename T, int NQ, int KQ>
 __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
-    using RowsT = Rows<T, KQ, V>;
+    using RowsT = Rows<T, KQ>;
     using TileT = TileBack<T, NQ, KQ>;
     constexpr int NP = TileT::B::NP;
     __shared__ TileT tiles[4];
@@ -754,12 +744,12 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
     const int obc = q.rs * (SCAN_CH * 2 * NP) + (idx >= NQ ? NP : 0) + q.n0 + (idx & (NQ - 1));
 
     // what the next chunk starts from: its inputs and the state before it
-    Inputs<T, NQ, KQ, V, true, true, true, true, true> in;
+    Inputs<T, NQ, KQ, true, true, true, true, true> in;
     f32x4 next_h[NQ];
     auto read_h = [&](const Item& m, int ck) {
         const ScanArgs a = args();
         if (a.p.ckpt) load_lanes<NQ>(a.p.ckpt, m.id * a.l.chunks + ck, lane, next_h);
-        else load_states<V>(a.p, q, a.p.h0, m.b0, next_h);
+        else load_states(a.p, q, a.p.h0, m.b0, next_h);
     };
     Item m(a0, w, w.slot, nseg, 0);
     if (m.c0 < m.c1) {
@@ -772,7 +762,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
         {
             const ScanArgs a = args();
             if (nseg > 1) load_lanes<NQ>(a.p.seg_h, m.id * nseg + m.seg, lane, gs);
-            else load_states<V>(a.p, q, a.p.dh1, m.b0, gs);
+            else load_states(a.p, q, a.p.dh1, m.b0, gs);
         }
         for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
             const int t0 = ck * SCAN_CH;
@@ -862,7 +852,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
             RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.du + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.u);
             RowsT::write(a.p, a.l, ln, w.g, w.cblk, (T*)a.p.ddelta + (m.b0 * L + t0) * a.p.D, L - t0, m.two, tile.de);
             if (!a.p.dbc) {
-                write_bc<T, NQ, KQ, V>(a.p, ln, w.g, m.b0, t0, m.two, tile);
+                write_bc<T, NQ, KQ>(a.p, ln, w.g, m.b0, t0, m.two, tile);
                 continue;
             }
             const long row = (((long)w.cblk * a.p.B + m.b0) * a.p.G + w.g) * a.l.chunks + ck;
@@ -877,7 +867,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
             }
         }
         const ScanArgs a = args();
-        if (a.p.dh0 && m.seg == 0) store_states<V>(a.p, q, a.p.dh0, m.b0 + q.rs, gs);
+        if (a.p.dh0 && m.seg == 0) store_states(a.p, q, a.p.dh0, m.b0, gs);
         if (it + step < items) m = Item(a, w, it + step, nseg, 0);
     }
     const ScanArgs a1 = args();
@@ -933,7 +923,7 @@ __launch_bounds__(256) __global__ void scan_bc_reduce_kernel(const float* __rest
 // One new token. Bound by the state, read and written once: 4 states (16
 // bytes) a lane, `gp` lanes a channel, joined by lane exchanges for y. Every
 // lane reads its own states before it writes them: h_out may be h.
-template <typename T, bool VEC>
+template <typename T>
 __launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp, long items) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     const bool ok = i < items;
@@ -951,49 +941,23 @@ __launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp
     const T* Cm = (const T*)p.Cm + b * p.C_b + g * p.C_g;
     const float* h = p.h + r * N;
     const float* A = p.A + (long)d * N;
-    float hv[4], Av[4], Bv[4], Cv[4];
-    if (VEC && n0 < N) {
-        *(f32x4*)hv = *(const f32x4*)(h + n0);
-        *(f32x4*)Av = *(const f32x4*)(A + n0);
-        T tb[4], tc[4];
-        if constexpr (sizeof(T) == 2) {
-            *(long*)tb = *(const long*)(Bm + n0);
-            *(long*)tc = *(const long*)(Cm + n0);
-        } else {
-            *(f32x4*)tb = *(const f32x4*)(Bm + n0);
-            *(f32x4*)tc = *(const f32x4*)(Cm + n0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            Bv[j] = to_f32(tb[j]);
-            Cv[j] = to_f32(tc[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool on = n0 + j < N;
-            hv[j] = on ? h[n0 + j] : 0.f;
-            Av[j] = on ? A[n0 + j] : 0.f;
-            Bv[j] = on ? to_f32(Bm[n0 + j]) : 0.f;
-            Cv[j] = on ? to_f32(Cm[n0 + j]) : 0.f;
-        }
-    }
+    const int n = n0 < N ? N - n0 : 0, at = n ? n0 : 0;
+    Pack<float> hp, Ap;
+    Pack<T, 4> Bp, Cp;
+    hp.load(h + at, n, N % 4);
+    Ap.load(A + at, n, N % 4);
+    Bp.load(Bm + at, n, N % 4);
+    Cp.load(Cm + at, n, N % 4);
     float acc = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        hv[j] = fmaf(__builtin_amdgcn_exp2f(dt * (Av[j] * LOG2E)), hv[j], dt * uv * Bv[j]);
-        acc = fmaf(Cv[j], hv[j], acc);
+        const float v = fmaf(__builtin_amdgcn_exp2f(dt * (Ap.get(j) * LOG2E)), hp.get(j), dt * uv * Bp.get(j));
+        hp.w[j] = __float_as_int(v);
+        acc = fmaf(Cp.get(j), v, acc);
     }
     for (int m = 1; m < gp; m <<= 1) acc += __shfl_xor(acc, m);
     if (!ok) return;
-    float* ho = p.h_out + r * N;
-    if (VEC && n0 < N) {
-        *(f32x4*)(ho + n0) = *(const f32x4*)hv;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n0 + j < N) ho[n0 + j] = hv[j];
-    }
+    hp.store(p.h_out + r * N + at, n, N % 4);
     if (n0 == 0) ((T*)p.y)[b * p.D + d] = from_f32<T>(p.skip ? fmaf(p.skip[d], uv, acc) : acc);
 }
 
@@ -1012,14 +976,8 @@ struct Typed {
     int is_f32;
     template <int NQ, int KQ>
     void operator()() const {
-        const bool vb = f.p.rvec && f.p.N == 4 * NQ * KQ;
-        if (is_f32) {
-            if (vb) f.template run<float, NQ, KQ, true>();
-            else f.template run<float, NQ, KQ, false>();
-        } else {
-            if (vb) f.template run<__bf16, NQ, KQ, true>();
-            else f.template run<__bf16, NQ, KQ, false>();
-        }
+        if (is_f32) f.template run<float, NQ, KQ>();
+        else f.template run<__bf16, NQ, KQ>();
     }
 };
 
@@ -1029,16 +987,16 @@ struct ScanFwd {
     const ScanParams& p;
     const ScanPlan& l;
     hipStream_t s;
-    template <typename T, int NQ, int KQ, bool VB>
+    template <typename T, int NQ, int KQ>
     void run() const {
         const long tasks = l.groups * p.G * l.cb;
         if (l.nseg > 1) {
-            hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, VB, false>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256),
+            hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, false>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256),
                                0, s, ScanArgs{p, l});
             hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, false>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
                                tasks * NQ);
         }
-        hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, VB, true>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0,
+        hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, true>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0,
                            s, ScanArgs{p, l});
     }
 };
@@ -1047,16 +1005,16 @@ struct ScanBwd {
     const ScanParams& p;
     const ScanPlan& l;
     hipStream_t s;
-    template <typename T, int NQ, int KQ, bool VB>
+    template <typename T, int NQ, int KQ>
     void run() const {
         const long tasks = l.groups * p.G * l.cb;
         if (l.nseg > 1) {
-            hipLaunchKernelGGL((scan_adjoint_kernel<T, NQ, KQ, VB>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0, s,
+            hipLaunchKernelGGL((scan_adjoint_kernel<T, NQ, KQ>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0, s,
                                ScanArgs{p, l});
             hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, true>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
                                tasks * NQ);
         }
-        hipLaunchKernelGGL((scan_bwd_kernel<T, NQ, KQ, VB>), wave_blocks((long)l.slots * p.G * l.cb), dim3(256), 0, s,
+        hipLaunchKernelGGL((scan_bwd_kernel<T, NQ, KQ>), wave_blocks((long)l.slots * p.G * l.cb), dim3(256), 0, s,
                            ScanArgs{p, l});
     }
 };
@@ -1130,14 +1088,8 @@ extern "C" void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_
     const long items = (long)p.B * p.D * gp;
     const dim3 grid((unsigned)((items + 255) / 256));
     if (is_f32) {
-        if (p.bvec) hipLaunchKernelGGL((scan_step_kernel<float, true>), grid, dim3(256), 0, s,
-            p, gp, items);
-        else hipLaunchKernelGGL((scan_step_kernel<float, false>), grid, dim3(256), 0, s,
-            p, gp, items);
+        hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, s, p, gp, items);
     } else {
-        if (p.bvec) hipLaunchKernelGGL((scan_step_kernel<__bf16, true>), grid, dim3(256), 0, s,
-            p, gp, items);
-        else hipLaunchKernelGGL((scan_step_kernel<__bf16, false>), grid, dim3(256), 0, s,
-            p, gp, items);
+        hipLaunchKernelGGL((scan_step_kernel<__bf16>), grid, dim3(256), 0, s, p, gp, items);
     }
 }

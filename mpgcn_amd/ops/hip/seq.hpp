@@ -1,8 +1,8 @@
 // Device helpers of the sequence operators (gfx950).
 //
-// Tensors are read in chunks of 8 channels: 16 bytes of bf16 or 32 of f32. A
-// chunk that cannot be read whole (odd width, odd stride, odd base address)
-// is read one element at a time by the same code.
+// Tensors move in pieces of 16 bytes at any element's address: the hardware
+// takes wide accesses that are not aligned, so odd widths, strides and base
+// addresses run through the same code. Only a row's last piece may be partial.
 #pragma once
 
 #include "common.hpp"
@@ -15,41 +15,105 @@
 template <typename T>
 using gmem = __attribute__((address_space(1))) T*;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef i32x4 __attribute__((aligned(2))) any16;  // 16, 8, 4 bytes at any bf16's address
+typedef i32x2 __attribute__((aligned(2))) any8;
+typedef int __attribute__((aligned(2))) any4;
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)[SEQ_CH]) {
-    if constexpr (VEC) {
-        Chunk16 c[SEQ_CH * sizeof(T) / 16];
-#pragma unroll
-        for (int i = 0; i < (int)(SEQ_CH * sizeof(T) / 16); ++i) c[i] = ((const Chunk16*)p)[i];
-        const T* e = (const T*)c;
-#pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j) v[j] = to_f32(e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
+// A piece of E elements as it is in memory, two bf16 to a register: kept so
+// while it waits, or each of them would take a register of its own. `n` of the
+// elements are there; where that is neither all nor none it is `rem`, the same
+// for every thread: what a row's width leaves over.
+template <typename T, int E_ = 16 / sizeof(T)>
+struct Pack {
+    static constexpr int E = E_, W = E * sizeof(T) / 4;      // elements, registers
+    static constexpr int WORD = 4 / sizeof(T), HALF = E / 2;  // elements of 4 bytes, of half of 16
+    __attribute__((ext_vector_type(W))) int w;
+
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __int_as_float(w[j]);
+        else return __int_as_float(j & 1 ? w[j >> 1] & 0xffff0000 : w[j >> 1] << 16);
     }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v)[SEQ_CH]) {
-    if constexpr (VEC) {
-        Chunk16 c[SEQ_CH * sizeof(T) / 16];
-        T* e = (T*)c;
+    __device__ __forceinline__ void set(const float (&v)[E]) {
+        T t[E];
 #pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j) e[j] = from_f32<T>(v[j]);
-#pragma unroll
-        for (int i = 0; i < (int)(SEQ_CH * sizeof(T) / 16); ++i) ((Chunk16*)p)[i] = c[i];
-    } else {
-#pragma unroll
-        for (int j = 0; j < SEQ_CH; ++j)
-            if (j < n) p[j] = from_f32<T>(v[j]);
+        for (int j = 0; j < E; ++j) t[j] = from_f32<T>(v[j]);
+        __builtin_memcpy(&w, t, sizeof(w));
     }
-}
-
-__device__ __forceinline__ void zero8(float (&v)[SEQ_CH]) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < SEQ_CH; ++j) v[j] = 0.f;
+        for (int i = 0; i < W; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* from, int n, int rem) {
+        const auto p = (gmem<const T>)from;
+        if (n >= E) {
+            if constexpr (W == 4) w = *(gmem<const any16>)p;
+            else w = *(gmem<const any8>)p;
+            return;
+        }
+        clear();
+        if (rem == 0 || n <= 0) return;
+        // halves, words and single bf16 of what is left, each at its own place
+        const bool h = W == 4 && (rem & HALF), q = rem & WORD, o = WORD == 2 && (rem & 1);
+        i32x2 vh = {0, 0};
+        int vq = 0, vo = 0;
+        if (h) vh = *(gmem<const any8>)p;
+        if (q) vq = *(gmem<const any4>)(p + (h ? HALF : 0));
+        if (o) vo = *(gmem<const unsigned short>)(p + (h ? HALF : 0) + (q ? WORD : 0));
+        const int a = q ? vq : vo, b = q ? vo : 0;
+        w[0] = h ? vh[0] : a;
+        w[1] = h ? vh[1] : b;
+        if constexpr (W == 4) {
+            w[2] = h ? a : 0;
+            w[3] = h ? b : 0;
+        }
+    }
+    __device__ __forceinline__ void store(T* to, int n, int rem) const {
+        const auto p = (gmem<T>)to;
+        if (n >= E) {
+            if constexpr (W == 4) *(gmem<any16>)p = w;
+            else *(gmem<any8>)p = w;
+            return;
+        }
+        if (rem == 0 || n <= 0) return;
+        const bool h = W == 4 && (rem & HALF), q = rem & WORD, o = WORD == 2 && (rem & 1);
+        const int a = h ? w[W == 4 ? 2 : 0] : w[0], b = h ? w[W == 4 ? 3 : 1] : w[1];
+        if (h) *(gmem<any8>)p = i32x2{w[0], w[1]};
+        if (q) *(gmem<any4>)(p + (h ? HALF : 0)) = a;
+        if (o) *(gmem<unsigned short>)(p + (h ? HALF : 0) + (q ? WORD : 0)) = (unsigned short)(q ? b : a);
+    }
+};
+
+// Eight channels as f32; n of them are there, D the row's width.
+template <typename T>
+struct Raw8 {
+    static constexpr int E = Pack<T>::E;
+    Pack<T> w[SEQ_CH / E];
+    __device__ __forceinline__ float get(int j) const { return w[j / E].get(j % E); }
+    __device__ __forceinline__ void load(const T* p, int n, int D) {
+#pragma unroll
+        for (int i = 0; i < SEQ_CH / E; ++i) w[i].load(p + i * E, n - i * E, D % E);
+    }
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, int D, float (&v)[SEQ_CH]) {
+    Raw8<T> r;
+    r.load(p, n, D);
+#pragma unroll
+    for (int j = 0; j < SEQ_CH; ++j) v[j] = r.get(j);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, int D, const float (&v)[SEQ_CH]) {
+    constexpr int E = Pack<T>::E;
+#pragma unroll
+    for (int i = 0; i < SEQ_CH / E; ++i) {
+        float t[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) t[j] = v[i * E + j];
+        Pack<T> k;
+        k.set(t);
+        k.store(p + i * E, n - i * E, D % E);
+    }
 }
 
 // Valid length of sequence b, held inside [0, L].
@@ -58,36 +122,6 @@ __device__ __forceinline__ int seq_len(const void* lens, int is64, int b, int L)
     const long n = is64 ? ((gmem<const long>)lens)[b] : (long)((gmem<const int>)lens)[b];
     return n < 0 ? 0 : n > L ? L : (int)n;
 }
-
-// log(1 + e^x) without overflow; the tail keeps full relative accuracy.
-__device__ __forceinline__ float softplus_f(float x) {
-    return fmaxf(x, 0.f) + log1pf(__expf(-fabsf(x)));
-}
-
-// 16 bytes as they are in memory, two bf16 to a register: kept so while they
-// wait, or each of them would take a register of its own.
-template <typename T>
-struct Pack {
-    static constexpr int E = 16 / sizeof(T);
-    i32x4 w;
-
-    __device__ __forceinline__ float get(int j) const {
-        if constexpr (sizeof(T) == 4) return __int_as_float(w[j]);
-        else return __int_as_float(j & 1 ? w[j >> 1] & 0xffff0000 : w[j >> 1] << 16);
-    }
-    // n of the E elements are there; VEC: all, and aligned
-    template <bool VEC>
-    __device__ __forceinline__ void load(const T* p, int n) {
-        if constexpr (VEC) {
-            w = *(const i32x4*)p;
-        } else {
-            T v[E];
-#pragma unroll
-            for (int j = 0; j < E; ++j) v[j] = j < n ? p[j] : (T)0.f;
-            __builtin_memcpy(&w, v, 16);
-        }
-    }
-};
 
 static inline int pow2_ceil(long n) {
     int p = 1;

@@ -15,36 +15,32 @@ constexpr int conv_e() { return 16 / sizeof(T); }  // channels a thread
 
 __device__ __forceinline__ float silu_f(float s) { return s * fast_sigmoid(s); }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Pack<T> row_at(const T* p, int n) {
+// A thread's channels at one step; n of them are there, D all of them.
+template <typename T>
+__device__ __forceinline__ Pack<T> row_at(const T* p, int n, int D) {
     Pack<T> r;
-    r.template load<VEC>(p, n);
+    r.load(p, n, D % conv_e<T>());
     return r;
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void put_row(T* p, int n, const float (&v)[conv_e<T>()]) {
-    alignas(16) T r[conv_e<T>()];
-#pragma unroll
-    for (int j = 0; j < conv_e<T>(); ++j) r[j] = from_f32<T>(v[j]);
-    if constexpr (VEC) {
-        *(Chunk16*)p = *(const Chunk16*)r;
-    } else {
-#pragma unroll
-        for (int j = 0; j < conv_e<T>(); ++j)
-            if (j < n) p[j] = r[j];
-    }
+template <typename T>
+__device__ __forceinline__ void put_row(T* p, int n, int D, const float (&v)[conv_e<T>()]) {
+    Pack<T> r;
+    r.set(v);
+    r.store(p, n, D % conv_e<T>());
 }
 template <typename T>
 __device__ __forceinline__ Pack<T> no_row() {
-    return Pack<T>{i32x4{0, 0, 0, 0}};
+    Pack<T> r;
+    r.clear();
+    return r;
 }
 
 // Input t of a sequence: the carried state before the first, zero before that
 // and past the end.
-template <typename T, int K, bool VEC>
+template <typename T, int K>
 __device__ __forceinline__ Pack<T> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n) {
-    if (t >= 0 && t < len) return row_at<T, VEC>(x + t * p.x_t, n);
-    if (t < 0 && t >= -(K - 1) && s0) return row_at<T, VEC>(s0 + (long)(t + K - 1) * p.D, n);
+    if (t >= 0 && t < len) return row_at<T>(x + t * p.x_t, n, p.D);
+    if (t < 0 && t >= -(K - 1) && s0) return row_at<T>(s0 + (long)(t + K - 1) * p.D, n, p.D);
     return no_row<T>();
 }
 
@@ -59,7 +55,7 @@ __device__ __forceinline__ void taps(const float* w, const float* bias, int c0, 
     }
 }
 
-template <typename T, int K, bool VEC>
+template <typename T, int K>
 __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv, int tiles) {
     constexpr int E = conv_e<T>(), NB = 8;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -80,13 +76,13 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
         const T* s = x + t * p.x_t;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            raw[j] = t + j < len ? row_at<T, VEC>(s, n) : no_row<T>();
+            raw[j] = t + j < len ? row_at<T>(s, n, p.D) : no_row<T>();
             s += p.x_t;
         }
     };
     Pack<T> edge[K - 1];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K, VEC>(p, x, s0, t0 - (K - 1) + k, len, n);
+    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n);
     read(t0);
     taps<K, E>(p.w, p.bias, c0, n, w, bias);
 #pragma unroll
@@ -111,7 +107,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
                 for (int k = 0; k < K; ++k) s = fmaf(w[k][c], win[k][c], s);
                 o[c] = t + j < len ? (p.silu ? silu_f(s) : s) : 0.f;
             }
-            if (t + j < t1) put_row<T, VEC>(y, n, o);
+            if (t + j < t1) put_row<T>(y, n, p.D, o);
             y += p.D;
         }
     }
@@ -119,11 +115,11 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
         T* s1 = (T*)p.s1 + (long)b * (K - 1) * p.D + c0;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            const Pack<T> v = input_row<T, K, VEC>(p, x, s0, len - (K - 1) + j, len, n);
+            const Pack<T> v = input_row<T, K>(p, x, s0, len - (K - 1) + j, len, n);
             float o[E];
 #pragma unroll
             for (int c = 0; c < E; ++c) o[c] = v.get(c);
-            put_row<T, VEC>(s1 + (long)j * p.D, n, o);
+            put_row<T>(s1 + (long)j * p.D, n, p.D, o);
         }
     }
 }
@@ -134,7 +130,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
 // the last K values of ds; filter gradients stay in registers over all of its
 // tiles, are joined per block and written once, then summed in a fixed order
 // (no atomics).
-template <typename T, int K, bool VEC>
+template <typename T, int K>
 __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, int dv, int cw, int tiles) {
     constexpr int E = conv_e<T>(), NB = 4;
     constexpr int W = E * (K + 1);
@@ -163,12 +159,12 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const bool on = t + j < len;
-                    xr[j] = on ? row_at<T, VEC>(x + (t + j) * p.x_t, n) : no_row<T>();
-                    yr[j] = on ? row_at<T, VEC>(dy + (long)(t + j) * p.D, n) : no_row<T>();
+                    xr[j] = on ? row_at<T>(x + (t + j) * p.x_t, n, p.D) : no_row<T>();
+                    yr[j] = on ? row_at<T>(dy + (long)(t + j) * p.D, n, p.D) : no_row<T>();
                 }
             };
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K, VEC>(p, x, s0, t0 - (K - 1) + k, len, n);
+            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n);
             read(t0);
             float xw[K][E], gw[K][E];
 #pragma unroll
@@ -222,7 +218,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c) o[c] = 0.f;
                     const int tail = ti - (len - (K - 1));
                     if (ds1 && tail >= 0 && tail < K - 1) {
-                        const Pack<T> v = row_at<T, VEC>(ds1 + (long)tail * p.D, n);
+                        const Pack<T> v = row_at<T>(ds1 + (long)tail * p.D, n, p.D);
 #pragma unroll
                         for (int c = 0; c < E; ++c) o[c] = v.get(c);
                     }
@@ -230,8 +226,8 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c)
 #pragma unroll
                         for (int k = 0; k < K; ++k) o[c] = fmaf(w[K - 1 - k][c], gw[k][c], o[c]);
-                    if (ti >= 0) put_row<T, VEC>(dx + (long)ti * p.D, n, o);
-                    else put_row<T, VEC>(ds0 + (long)(ti + K - 1) * p.D, n, o);
+                    if (ti >= 0) put_row<T>(dx + (long)ti * p.D, n, p.D, o);
+                    else put_row<T>(ds0 + (long)(ti + K - 1) * p.D, n, p.D, o);
                 }
             }
         }
@@ -261,7 +257,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
 // One new token: the state shifts by one input. A thread owns its 8 channels
 // of the state alone and reads them all before it writes, so the new state may
 // overwrite the old.
-template <typename T, int K, bool VEC>
+template <typename T, int K>
 __launch_bounds__(256) __global__ void short_conv_step_kernel(
     const T* __restrict__ x, long x_b, const T* s_in, T* s_out, const float* __restrict__ w,
     const float* __restrict__ bias, T* __restrict__ y, long items, int dv, int D, int silu) {
@@ -272,8 +268,8 @@ __launch_bounds__(256) __global__ void short_conv_step_kernel(
     const int n = D - c0 < SEQ_CH ? D - c0 : SEQ_CH;
     float in[K][SEQ_CH], o[SEQ_CH];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) load8<T, VEC>(s_in + (b * (K - 1) + k) * D + c0, n, in[k]);
-    load8<T, VEC>(x + b * x_b + c0, n, in[K - 1]);
+    for (int k = 0; k < K - 1; ++k) load8<T>(s_in + (b * (K - 1) + k) * D + c0, n, D, in[k]);
+    load8<T>(x + b * x_b + c0, n, D, in[K - 1]);
 #pragma unroll
     for (int c = 0; c < SEQ_CH; ++c) {
         float s = (bias && c < n) ? bias[c0 + c] : 0.f;
@@ -281,9 +277,9 @@ __launch_bounds__(256) __global__ void short_conv_step_kernel(
         for (int k = 0; k < K; ++k) s = fmaf(c < n ? w[(long)(c0 + c) * K + k] : 0.f, in[k][c], s);
         o[c] = silu ? silu_f(s) : s;
     }
-    store8<T, VEC>(y + b * D + c0, n, o);
+    store8<T>(y + b * D + c0, n, D, o);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) store8<T, VEC>(s_out + (b * (K - 1) + k) * D + c0, n, in[k + 1]);
+    for (int k = 0; k < K - 1; ++k) store8<T>(s_out + (b * (K - 1) + k) * D + c0, n, D, in[k + 1]);
 }
 
 // Threads of a block side by side in the channels.
@@ -299,31 +295,26 @@ inline int conv_tile(long B, long L, long dv, long threads) {
 }
 
 template <typename F>
-void by_type(int K, int is_f32, int vec, F f) {
-    auto with_k = [&](auto t, auto v) {
+void by_type(int K, int is_f32, F f) {
+    auto with = [&](auto t) {
         using T = decltype(t);
-        constexpr bool V = decltype(v)::value;
-        if (K == 2) f.template operator()<T, 2, V>();
-        else if (K == 3) f.template operator()<T, 3, V>();
-        else f.template operator()<T, 4, V>();
+        if (K == 2) f.template operator()<T, 2>();
+        else if (K == 3) f.template operator()<T, 3>();
+        else f.template operator()<T, 4>();
     };
-    auto with_t = [&](auto t) {
-        if (vec) with_k(t, std::true_type{});
-        else with_k(t, std::false_type{});
-    };
-    if (is_f32) with_t(float{});
-    else with_t(__bf16{});
+    if (is_f32) with(float{});
+    else with(__bf16{});
 }
 
 struct Fwd {
     const ShortConvParams& p;
     hipStream_t s;
-    template <typename T, int K, bool V>
+    template <typename T, int K>
     void operator()() const {
         const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const long items = (long)p.B * tiles * dv;
-        hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, V>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p,
+        hipLaunchKernelGGL((short_conv_fwd_kernel<T, K>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p,
                            items, dv, tiles);
     }
 };
@@ -331,13 +322,13 @@ struct Fwd {
 struct Bwd {
     const ShortConvParams& p;
     hipStream_t s;
-    template <typename T, int K, bool V>
+    template <typename T, int K>
     void operator()() const {
         const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
         const int cw = conv_cw(dv);
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const size_t smem = 256 * conv_e<T>() * (K + 1) * sizeof(float);
-        hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3(p.slots, (dv + cw - 1) / cw), dim3(256), smem, s, p, dv,
+        hipLaunchKernelGGL((short_conv_bwd_kernel<T, K>), dim3(p.slots, (dv + cw - 1) / cw), dim3(256), smem, s, p, dv,
                            cw, tiles);
     }
 };
@@ -345,11 +336,11 @@ struct Bwd {
 struct Step {
     const void* x; long x_b; const void* s_in; void* s_out; const float* w; const float* bias;
     void* y; long B; int D, silu; hipStream_t s;
-    template <typename T, int K, bool V>
+    template <typename T, int K>
     void operator()() const {
         const int dv = (D + SEQ_CH - 1) / SEQ_CH;
         const long items = B * dv;
-        hipLaunchKernelGGL((short_conv_step_kernel<T, K, V>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s,
+        hipLaunchKernelGGL((short_conv_step_kernel<T, K>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s,
             (const T*)x, x_b, (const T*)s_in, (T*)s_out, w, bias, (T*)y, items, dv, D, silu);
     }
 };
@@ -368,20 +359,18 @@ extern "C" void short_conv_plan(ShortConvParams* p, int is_f32, int back) {
     p->slots = (int)(want < cap ? want : cap);
 }
 
-extern "C" void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
-                                      hipStream_t s) {
-    by_type(K, is_f32, vec, Fwd{p, s});
+extern "C" void short_conv_fwd_launch(const ShortConvParams& p, int K, int is_f32, hipStream_t s) {
+    by_type(K, is_f32, Fwd{p, s});
 }
 
-extern "C" void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, int vec,
-                                      hipStream_t s) {
-    by_type(K, is_f32, vec, Bwd{p, s});
+extern "C" void short_conv_bwd_launch(const ShortConvParams& p, int K, int is_f32, hipStream_t s) {
+    by_type(K, is_f32, Bwd{p, s});
 }
 
 extern "C" void short_conv_step_launch(const void* x, long x_b, const void* s_in, void* s_out,
                                        const float* w, const float* bias, void* y, long B, int D,
-                                       int K, int silu, int is_f32, int vec, hipStream_t s) {
-    by_type(K, is_f32, vec, Step{x, x_b, s_in, s_out, w, bias, y, B, D, silu, s});
+                                       int K, int silu, int is_f32, hipStream_t s) {
+    by_type(K, is_f32, Step{x, x_b, s_in, s_out, w, bias, y, B, D, silu, s});
 }
 
 // Column sums of a (nb, E) float workspace in a fixed order: 16 row threads a
