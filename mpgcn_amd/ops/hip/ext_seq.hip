@@ -5,7 +5,9 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPException.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "params.hpp"
 
@@ -419,12 +421,127 @@ std::vector<Tensor> block_norm_bwd(Opt dy, Opt dh, Tensor x, Opt gate, Opt post,
     return {dx, dg, dpost, dr, dscale, dpre};
 }
 
+// ---- gradients --------------------------------------------------------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+Tensor val(const Opt& t) { return has(t) ? *t : Tensor(); }
+Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
+Opt rows_of(const Tensor& t) { return t.defined() ? Opt(t.contiguous()) : Opt(); }
+bool any(const variable_list& g) {
+    for (const auto& t : g)
+        if (t.defined()) return true;
+    return false;
+}
+
+// The gradients have no gradient of their own: a second derivative raises when
+// it is asked for.
+variable_list once(variable_list g, const char* name) {
+    if (!at::GradMode::is_enabled()) return g;
+    for (auto& t : g)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
+    auto fn = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative",
+                                                              (int64_t)g.size());
+    return (*fn)(std::move(g));
+}
+
+struct ShortConvFn : Function<ShortConvFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& bias, const Opt& s0,
+                                 const Opt& lens, bool silu, bool want_state) {
+        ctx->set_materialize_grads(false);
+        auto r = short_conv_fwd(x, w, bias, s0, lens, silu, want_state);
+        ctx->save_for_backward({x, w, val(bias), val(s0), val(lens)});
+        ctx->saved_data["silu"] = silu;
+        ctx->saved_data["state"] = has(s0) && s0->requires_grad();
+        if (!want_state) r.pop_back();
+        return r;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(7);
+        if (any(g)) {
+            at::NoGradGuard no_grad;
+            auto v = ctx->get_saved_variables();
+            const Tensor dy = g[0].defined() ? g[0].contiguous() : torch::zeros(v[0].sizes(), v[0].options());
+            auto r = short_conv_bwd(dy, g.size() > 1 ? rows_of(g[1]) : Opt(), v[0], v[1], opt(v[2]), opt(v[3]),
+                                    opt(v[4]), ctx->saved_data["silu"].toBool(), ctx->saved_data["state"].toBool());
+            out[0] = r[0];
+            out[1] = r[1];
+            if (v[2].defined()) out[2] = r[2];
+            out[3] = r[3];
+        }
+        return once(out, "short_conv");
+    }
+};
+
+struct SelectiveScanFn : Function<SelectiveScanFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& u, const Tensor& delta, const Tensor& A,
+                                 const Tensor& Bm, const Tensor& Cm, const Opt& skip, const Opt& dbias, const Opt& h0,
+                                 const Opt& lens, bool softplus, bool want_state) {
+        ctx->set_materialize_grads(false);
+        auto r = selective_scan_fwd(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus, want_state, true);
+        ctx->save_for_backward({u, delta, A, Bm, Cm, val(skip), val(dbias), val(h0), val(lens), r[2]});
+        ctx->saved_data["softplus"] = softplus;
+        ctx->saved_data["state"] = has(h0) && h0->requires_grad();
+        r.resize(want_state ? 2 : 1);
+        return r;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(11);
+        if (any(g)) {
+            at::NoGradGuard no_grad;
+            auto v = ctx->get_saved_variables();
+            auto r = selective_scan_bwd(rows_of(g[0]), g.size() > 1 ? rows_of(g[1]) : Opt(), v[0], v[1], v[2], v[3], v[4],
+                                        opt(v[5]), opt(v[6]), opt(v[7]), opt(v[8]), opt(v[9]),
+                                        ctx->saved_data["softplus"].toBool(), ctx->saved_data["state"].toBool());
+            for (int i = 0; i < 8; ++i) out[i] = r[i];
+            if (!v[5].defined()) out[5] = Tensor();
+            if (!v[6].defined()) out[6] = Tensor();
+        }
+        return once(out, "selective_scan");
+    }
+};
+
+struct BlockNormFn : Function<BlockNormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Opt& gate, const Opt& post, const Opt& res,
+                                 const Opt& scale, const Opt& pre, double eps) {
+        ctx->set_materialize_grads(false);
+        auto r = block_norm_fwd(x, gate, post, res, scale, pre, eps, true);
+        ctx->save_for_backward({x, val(gate), val(post), val(res), val(scale), val(pre), r[2], r[3]});
+        ctx->saved_data["eps"] = eps;
+        if (!r[1].defined()) return {r[0]};
+        if (!r[0].defined()) return {r[1]};
+        return {r[0], r[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        variable_list out(7);
+        if (any(g)) {
+            at::NoGradGuard no_grad;
+            auto v = ctx->get_saved_variables();
+            const bool y = !v[3].defined() || v[5].defined();
+            const Opt dy = y ? rows_of(g[0]) : Opt(), dh = v[3].defined() ? rows_of(g.back()) : Opt();
+            auto r = block_norm_bwd(dy, dh, v[0], opt(v[1]), opt(v[2]), opt(v[3]), opt(v[4]), opt(v[5]), opt(v[6]),
+                                    opt(v[7]), ctx->saved_data["eps"].toDouble());
+            for (int i = 0; i < 6; ++i) out[i] = r[i];
+        }
+        return once(out, "norm_gate_residual");
+    }
+};
+
+py::object one_or_pair(const variable_list& r) {
+    return r.size() > 1 ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
+}
+
+// A capture needs the look at live graphs that Python takes first.
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
 // ---- calls that need no preparation -----------------------------------------
 //
-// The operators' common case at inference, without Python's share of the time:
-// every argument is in the kernels' form and no gradient is wanted. Any other
-// call gives None and goes through the checks and conversions of
-// mpgcn_amd/ops/sequence.py, which name what is wrong.
+// The operators' common case without Python's share of the time: every argument
+// is in the kernels' form. Any other call gives None and goes through the
+// checks and conversions of mpgcn_amd/ops/sequence.py, which name what is wrong
+// and come back here with `prepared` set.
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (!at::GradMode::is_enabled()) return false;
@@ -435,10 +552,11 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 const Tensor* tp(const Opt& t) { return t.has_value() ? &*t : nullptr; }
 
 template <typename F>
-py::object direct(F f) {
+py::object direct(bool prepared, F f) {
     try {
         return f();
     } catch (const c10::Error&) {
+        if (prepared) throw;
         return py::none();
     }
 }
@@ -450,28 +568,37 @@ bool apart(const Tensor& a, const Tensor& b) {
     return d == 0 || d >= (long)(a.numel() * a.element_size());
 }
 
-py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state) {
-    if (!x.is_cuda() || wants_grad({&x, &w, tp(bias), tp(s0)})) return py::none();
-    return direct([&]() -> py::object {
+py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state,
+                             bool prepared) {
+    if (!x.is_cuda()) return py::none();
+    const bool train = wants_grad({&x, &w, tp(bias), tp(s0)});
+    if (train && !prepared && capturing()) return py::none();
+    return direct(prepared, [&]() -> py::object {
+        if (train) return one_or_pair(ShortConvFn::apply(x, w, bias, s0, lens, silu, want_state));
         auto r = short_conv_fwd(x, w, bias, s0, lens, silu, want_state);
-        return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
+        if (!want_state) r.pop_back();
+        return one_or_pair(r);
     });
 }
 
 py::object short_conv_step_direct(Tensor x, Tensor state, Opt state_out, Tensor w, Opt bias, bool silu) {
     const Tensor out = has(state_out) ? *state_out : state;
     if (!x.is_cuda() || wants_grad({&x, &state, &out, &w, tp(bias)}) || !apart(state, out)) return py::none();
-    return direct([&] { return py::make_tuple(short_conv_step(x, state, out, w, bias, silu), out); });
+    return direct(false, [&] { return py::make_tuple(short_conv_step(x, state, out, w, bias, silu), out); });
 }
 
 py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias, Opt h0,
-                                 Opt lens, bool softplus, bool want_state) {
-    if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)})) return py::none();
-    return direct([&]() -> py::object {
-        auto grouped = [](const Tensor& t) { return t.dim() == 3 ? t.unsqueeze(2) : t; };
-        auto r = selective_scan_fwd(u, delta, A, grouped(Bm), grouped(Cm), skip, dbias, h0, lens, softplus, want_state,
-                                    false);
-        return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
+                                 Opt lens, bool softplus, bool want_state, bool prepared) {
+    if (!u.is_cuda()) return py::none();
+    const bool train = wants_grad({&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)});
+    if (train && !prepared && capturing()) return py::none();
+    return direct(prepared, [&]() -> py::object {
+        const Tensor B4 = Bm.dim() == 3 ? Bm.unsqueeze(2) : Bm, C4 = Cm.dim() == 3 ? Cm.unsqueeze(2) : Cm;
+        if (train)
+            return one_or_pair(SelectiveScanFn::apply(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus, want_state));
+        auto r = selective_scan_fwd(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus, want_state, false);
+        r.resize(want_state ? 2 : 1);
+        return one_or_pair(r);
     });
 }
 
@@ -480,25 +607,32 @@ py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor B
     const Tensor out = has(state_out) ? *state_out : state;
     if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, &state, &out, tp(skip), tp(dbias)}) || !apart(state, out))
         return py::none();
-    return direct([&] {
+    return direct(false, [&] {
         return py::make_tuple(selective_scan_step(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus), out);
     });
 }
 
-py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps) {
-    if (!x.is_cuda() || x.dim() < 1 || !(eps > 0) ||
-        wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)}))
-        return py::none();
-    return direct([&]() -> py::object {
+py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps, bool prepared) {
+    if (!x.is_cuda() || x.dim() < 1 || !(eps > 0)) return py::none();
+    const bool train = wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)});
+    if (train && !prepared && capturing()) return py::none();
+    return direct(prepared, [&]() -> py::object {
         const auto shape = x.sizes().vec();
         const bool flat = x.dim() == 2;
-        TORCH_CHECK(shape.back() >= 1 && (!has(gate) || gate->sizes() == x.sizes()) && (!has(res) || res->sizes() == x.sizes()));
+        TORCH_CHECK(shape.back() >= 1 && (!has(gate) || gate->sizes() == x.sizes()) &&
+                    (!has(res) || res->sizes() == x.sizes()), "gate and residual must have x's shape");
         auto rows = [&](const Tensor& t) { return flat ? t : t.reshape({-1, shape.back()}); };
-        auto opt = [&](const Opt& t) { return has(t) ? Opt(rows(*t)) : Opt(); };
-        auto r = block_norm_fwd(rows(x), opt(gate), post, opt(res), scale, pre, eps, false);
-        auto back = [&](const Tensor& t) { return flat ? t : t.view(shape); };
-        if (r[0].defined() && r[1].defined()) return py::make_tuple(back(r[0]), back(r[1]));
-        return py::cast(back(r[0].defined() ? r[0] : r[1]));
+        auto opt_rows = [&](const Opt& t) { return has(t) ? Opt(rows(*t)) : Opt(); };
+        variable_list r;
+        if (train) {
+            r = BlockNormFn::apply(rows(x), opt_rows(gate), post, opt_rows(res), scale, pre, eps);
+        } else {
+            for (auto& t : block_norm_fwd(rows(x), opt_rows(gate), post, opt_rows(res), scale, pre, eps, false))
+                if (t.defined()) r.push_back(t);
+        }
+        if (!flat)
+            for (auto& t : r) t = t.view(shape);
+        return one_or_pair(r);
     });
 }
 
@@ -515,17 +649,17 @@ bool accumulates_elsewhere(Tensor leaf) {
 
 void bind_sequence(pybind11::module_& m) {
     m.def("accumulates_elsewhere", &accumulates_elsewhere, "leaf has a live accumulator on another stream");
-    m.def("short_conv_fwd", &short_conv_fwd, "short causal convolution");
-    m.def("short_conv_bwd", &short_conv_bwd, "backward of short_conv_fwd");
+    const auto prepared = py::arg("prepared") = false;
+    m.def("short_conv_direct", &short_conv_direct, "short_conv where no preparation is needed, else None", py::arg("x"),
+          py::arg("weight"), py::arg("bias"), py::arg("state"), py::arg("lengths"), py::arg("silu"),
+          py::arg("return_state"), prepared);
     m.def("short_conv_step", &short_conv_step, "short causal convolution of one new token");
-    m.def("selective_scan_fwd", &selective_scan_fwd, "selective state space scan");
-    m.def("selective_scan_bwd", &selective_scan_bwd, "backward of selective_scan_fwd");
     m.def("selective_scan_step", &selective_scan_step, "selective state space scan of one new token");
-    m.def("block_norm_fwd", &block_norm_fwd, "norms around a block with gate and residual scale");
-    m.def("block_norm_bwd", &block_norm_bwd, "backward of block_norm_fwd");
-    m.def("short_conv_direct", &short_conv_direct, "short_conv where no preparation is needed, else None");
     m.def("short_conv_step_direct", &short_conv_step_direct, "short_conv_step, likewise");
-    m.def("selective_scan_direct", &selective_scan_direct, "selective_scan, likewise");
+    m.def("selective_scan_direct", &selective_scan_direct, "selective_scan, likewise", py::arg("u"), py::arg("delta"),
+          py::arg("A"), py::arg("B"), py::arg("C"), py::arg("skip"), py::arg("delta_bias"), py::arg("state"),
+          py::arg("lengths"), py::arg("softplus"), py::arg("return_state"), prepared);
     m.def("selective_scan_step_direct", &selective_scan_step_direct, "selective_scan_step, likewise");
-    m.def("block_norm_direct", &block_norm_direct, "norm_gate_residual, likewise");
+    m.def("block_norm_direct", &block_norm_direct, "norm_gate_residual, likewise", py::arg("x"), py::arg("gate"),
+          py::arg("post_weight"), py::arg("residual"), py::arg("scale"), py::arg("pre_weight"), py::arg("eps"), prepared);
 }

@@ -31,8 +31,6 @@ captured backward would have to wait for that stream.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from mpgcn_amd import ops as _ops
 from mpgcn_amd.ops import eager
 
@@ -126,14 +124,10 @@ def _no_grad_only(name: str, *tensors) -> None:
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def _check_capture(*tensors) -> None:
     """Refuse a training call inside a capture whose backward could not be
     captured: a leaf that an eager graph still holds on another stream."""
-    if not torch.cuda.is_current_stream_capturing():
+    if not (torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()):
         return
     ext = _ops.get_ext()
     seen, todo = set(), []
@@ -160,27 +154,6 @@ _LIVE_GRAPH = ("a leaf of this call is held by an eager autograd graph on anothe
 
 
 # ---- short causal convolution -----------------------------------------------
-
-class _ShortConvFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
-        ctx.set_materialize_grads(False)
-        y, last = _ops.get_ext().short_conv_fwd(x, weight, bias, state, lengths, silu, want_state)
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        ctx.silu = silu
-        return (y, last) if want_state else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dlast=None):
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        if dy is None and dlast is None:
-            return (None,) * 7
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
-        dx, dw, db, ds = _ops.get_ext().short_conv_bwd(
-            dy, None if dlast is None else dlast.contiguous(), x, weight, bias, state, lengths, ctx.silu,
-            ctx.needs_input_grad[3])
-        return dx, dw, db if bias is not None else None, ds, None, None, None
 
 
 def _check_taps(weight, D: int) -> int:
@@ -227,11 +200,8 @@ def short_conv(x, weight, bias=None, *, state=None, lengths=None, activation="si
         return (y, last) if return_state else y
     x = _rows(x)
     state = None if state is None else state.contiguous()
-    if _wants_grad(x, weight, bias, state):
-        _check_capture(x, weight, bias, state)
-        return _ShortConvFn.apply(x, weight, bias, state, lengths, silu, return_state)
-    y, last = _ops.get_ext().short_conv_fwd(x, weight, bias, state, lengths, silu, return_state)
-    return (y, last) if return_state else y
+    _check_capture(x, weight, bias, state)
+    return _ops.get_ext().short_conv_direct(x, weight, bias, state, lengths, silu, return_state, prepared=True)
 
 
 def short_conv_step(x, state, weight, bias=None, *, activation="silu", state_out=None):
@@ -260,28 +230,6 @@ def short_conv_step(x, state, weight, bias=None, *, activation="silu", state_out
 
 
 # ---- selective state space scan ---------------------------------------------
-
-class _SelectiveScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, u, delta, A, B, C, skip, delta_bias, state, lengths, softplus, want_state):
-        ctx.set_materialize_grads(False)
-        y, last, kept = _ops.get_ext().selective_scan_fwd(u, delta, A, B, C, skip, delta_bias, state, lengths,
-                                                          softplus, want_state, True)
-        ctx.save_for_backward(u, delta, A, B, C, skip, delta_bias, state, lengths, kept)
-        ctx.softplus = softplus
-        return (y, last) if want_state else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dlast=None):
-        u, delta, A, B, C, skip, delta_bias, state, lengths, kept = ctx.saved_tensors
-        if dy is None and dlast is None:
-            return (None,) * 11
-        du, dd, dA, dB, dC, ds, db, dh = _ops.get_ext().selective_scan_bwd(
-            None if dy is None else dy.contiguous(), None if dlast is None else dlast.contiguous(),
-            u, delta, A, B, C, skip, delta_bias, state, lengths, kept, ctx.softplus, ctx.needs_input_grad[7])
-        return (du, dd, dA, dB, dC, ds if skip is not None else None, db if delta_bias is not None else None, dh,
-                None, None, None)
 
 
 def _check_scan(u, delta, A, B, C, lead):
@@ -350,12 +298,9 @@ def selective_scan(u, delta, A, B, C, skip=None, *, delta_bias=None, delta_softp
         return (y, last) if return_state else y
     u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
     state = None if state is None else state.contiguous()
-    if _wants_grad(u, delta, A, B, C, skip, delta_bias, state):
-        _check_capture(u, delta, A, B, C, skip, delta_bias, state)
-        return _SelectiveScanFn.apply(u, delta, A, B, C, skip, delta_bias, state, lengths, softplus, return_state)
-    y, last, _ = _ops.get_ext().selective_scan_fwd(u, delta, A, B, C, skip, delta_bias, state, lengths, softplus,
-                                                   return_state, False)
-    return (y, last) if return_state else y
+    _check_capture(u, delta, A, B, C, skip, delta_bias, state)
+    return _ops.get_ext().selective_scan_direct(u, delta, A, B, C, skip, delta_bias, state, lengths, softplus,
+                                                return_state, prepared=True)
 
 
 def selective_scan_step(u, delta, A, B, C, state, skip=None, *, delta_bias=None, delta_softplus=False,
@@ -384,31 +329,6 @@ def selective_scan_step(u, delta, A, B, C, state, skip=None, *, delta_bias=None,
 
 
 # ---- norms around a block ---------------------------------------------------
-
-class _NormGateResidualFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, post, res, scale, pre, eps):
-        ctx.set_materialize_grads(False)
-        y, h, i1, i2 = _ops.get_ext().block_norm_fwd(x, gate, post, res, scale, pre, eps, True)
-        ctx.save_for_backward(x, gate, post, res, scale, pre, i1, i2)
-        ctx.eps = eps
-        return (y, h) if y is not None and h is not None else h if y is None else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        x, gate, post, res, scale, pre, i1, i2 = ctx.saved_tensors
-        if all(g is None for g in grads):
-            return (None,) * 7
-        grads = [None if g is None else g.contiguous() for g in grads]
-        if res is None:
-            dy, dh = grads[0], None
-        elif pre is None:
-            dy, dh = None, grads[0]
-        else:
-            dy, dh = grads
-        out = _ops.get_ext().block_norm_bwd(dy, dh, x, gate, post, res, scale, pre, i1, i2, ctx.eps)
-        return (*out, None)
 
 
 def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=None, pre_weight=None, eps=1e-5):
@@ -457,13 +377,6 @@ def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=N
     if not x.is_cuda:
         y, h = eager.norm_gate_residual_eager(x, gate, post, residual, scale, pre, eps)
         return (y, h) if y is not None and h is not None else h if y is None else y
-    shape = x.shape
-    x2, g2, r2 = (None if t is None else _rows(t.reshape(-1, D)) for t in (x, gate, residual))
-    if _wants_grad(x2, g2, post, r2, scale, pre):
-        _check_capture(x2, g2, post, r2, scale, pre)
-        out = _NormGateResidualFn.apply(x2, g2, post, r2, scale, pre, eps)
-        return tuple(o.view(shape) for o in out) if isinstance(out, tuple) else out.view(shape)
-    y, h, _, _ = _ops.get_ext().block_norm_fwd(x2, g2, post, r2, scale, pre, eps, False)
-    if y is not None and h is not None:
-        return y.view(shape), h.view(shape)
-    return (h if y is None else y).view(shape)
+    x, gate, residual = _rows(x), _rows(gate), _rows(residual)
+    _check_capture(x, gate, post, residual, scale, pre)
+    return _ops.get_ext().block_norm_direct(x, gate, post, residual, scale, pre, eps, prepared=True)

@@ -496,3 +496,46 @@ def test_argument_devices_are_checked():
         ops.norm_gate_residual(x, post_weight=w[:, 0].cpu())
     with pytest.raises(TypeError):
         ops.norm_gate_residual(x.double(), post_weight=w[:, 0])
+
+
+def test_second_derivatives_are_refused():
+    """First gradients under create_graph are the usual ones; differentiating
+    them again raises instead of giving zeros."""
+    x, w = rn(gen(95), 2, 5, 8).requires_grad_(), rn(gen(96), 8, 3).requires_grad_()
+    t, _ = scan_case(97, F, 2, 5, 8, 4, 1, False, None)
+    u = t["u"].requires_grad_()
+    for leaf, fn in ((x, lambda: ops.short_conv(x, w)),
+                     (u, lambda: ops.selective_scan(**t)),
+                     (x, lambda: ops.norm_gate_residual(x, gate=x * 2, post_weight=w[:, 0]))):
+        plain = torch.autograd.grad(fn().square().sum(), leaf)[0]
+        kept = torch.autograd.grad(fn().square().sum(), leaf, create_graph=True)[0]
+        assert torch.equal(plain, kept)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            kept.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_gradients_reach_only_what_asks(dtype):
+    """Any one leaf alone, the others constants."""
+    t, n = scan_case(98, dtype, 3, 9, 16, 5, 1, True, torch.int32)
+    ref = oracle.scan(**t, lengths=n, dy=torch.ones(3, 9, 16))
+    for name in t:
+        one = {k: v.detach().clone().requires_grad_(k == name) for k, v in t.items()}
+        y = ops.selective_scan(**one, lengths=n, delta_softplus=True)
+        y.backward(torch.ones_like(y))
+        oracle.within(one[name].grad, *ref[name], oracle.scan_roundings(9, 5) + 54, name)
+        assert all(v.grad is None for k, v in one.items() if k != name)
+
+
+def test_converted_arguments():
+    """Weights of another type and channels that are not contiguous take the
+    long way round, gradients included."""
+    x, w = rn(gen(99), 2, 8, 6).transpose(1, 2).requires_grad_(), rn(gen(100), 8, 3, dtype=BF).requires_grad_()
+    y = ops.short_conv(x, w)
+    dy = rn(gen(101), 2, 6, 8)
+    ref = oracle.conv(x, w.float(), dy=dy)
+    oracle.within(y, *ref["y"], oracle.conv_roundings(3))
+    gx, gw = grads([y], [dy], [x, w])
+    oracle.within(gx, *ref["x"], oracle.conv_roundings(3))
+    assert gw.dtype == BF
+    oracle.within(gw, *ref["weight"], oracle.conv_roundings(3) + 24)
