@@ -15,7 +15,7 @@ constexpr int conv_e() { return 16 / sizeof(T); }  // channels a thread
 
 __device__ __forceinline__ float silu_f(float s) { return s * fast_sigmoid(s); }
 
-// A thread's channels at one step; n of them are there, D all of them.
+// A thread's channels at one step; n of them are there, D in a row.
 template <typename T>
 __device__ __forceinline__ Pack<T> row_at(const T* p, int n, int D) {
     Pack<T> r;
@@ -38,9 +38,10 @@ __device__ __forceinline__ Pack<T> no_row() {
 // Input t of a sequence: the carried state before the first, zero before that
 // and past the end.
 template <typename T, int K>
-__device__ __forceinline__ Pack<T> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n) {
-    if (t >= 0 && t < len) return row_at<T>(x + t * p.x_t, n, p.D);
-    if (t < 0 && t >= -(K - 1) && s0) return row_at<T>(s0 + (long)(t + K - 1) * p.D, n, p.D);
+__device__ __forceinline__ Pack<T> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n,
+                                             int width) {
+    if (t >= 0 && t < len) return row_at<T>(x + t * p.x_t, n, width);
+    if (t < 0 && t >= -(K - 1) && s0) return row_at<T>(s0 + (long)(t + K - 1) * p.D, n, width);
     return no_row<T>();
 }
 
@@ -55,7 +56,8 @@ __device__ __forceinline__ void taps(const float* w, const float* bias, int c0, 
     }
 }
 
-template <typename T, int K>
+// WHOLE: every thread has all of its channels, and no code for fewer.
+template <typename T, int K, bool WHOLE>
 __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv, int tiles) {
     constexpr int E = conv_e<T>(), NB = 8;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -63,7 +65,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
     const int c0 = (int)(i % dv) * E;
     const long r = i / dv;
     const int tile = (int)(r % tiles), b = (int)(r / tiles);
-    const int n = p.D - c0 < E ? p.D - c0 : E;
+    const int n = WHOLE || p.D - c0 >= E ? E : p.D - c0, width = WHOLE ? E : p.D;
     const int len = seq_len(p.lens, p.lens64, b, p.L);
     const T* x = (const T*)p.x + b * p.x_b + c0;
     const T* s0 = p.s0 ? (const T*)p.s0 + (long)b * (K - 1) * p.D + c0 : nullptr;
@@ -76,13 +78,13 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
         const T* s = x + t * p.x_t;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            raw[j] = t + j < len ? row_at<T>(s, n, p.D) : no_row<T>();
+            raw[j] = t + j < len ? row_at<T>(s, n, width) : no_row<T>();
             s += p.x_t;
         }
     };
     Pack<T> edge[K - 1];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n);
+    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
     read(t0);
     taps<K, E>(p.w, p.bias, c0, n, w, bias);
 #pragma unroll
@@ -107,7 +109,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
                 for (int k = 0; k < K; ++k) s = fmaf(w[k][c], win[k][c], s);
                 o[c] = t + j < len ? (p.silu ? silu_f(s) : s) : 0.f;
             }
-            if (t + j < t1) put_row<T>(y, n, p.D, o);
+            if (t + j < t1) put_row<T>(y, n, width, o);
             y += p.D;
         }
     }
@@ -115,11 +117,11 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
         T* s1 = (T*)p.s1 + (long)b * (K - 1) * p.D + c0;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            const Pack<T> v = input_row<T, K>(p, x, s0, len - (K - 1) + j, len, n);
+            const Pack<T> v = input_row<T, K>(p, x, s0, len - (K - 1) + j, len, n, width);
             float o[E];
 #pragma unroll
             for (int c = 0; c < E; ++c) o[c] = v.get(c);
-            put_row<T>(s1 + (long)j * p.D, n, p.D, o);
+            put_row<T>(s1 + (long)j * p.D, n, width, o);
         }
     }
 }
@@ -130,7 +132,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
 // the last K values of ds; filter gradients stay in registers over all of its
 // tiles, are joined per block and written once, then summed in a fixed order
 // (no atomics).
-template <typename T, int K>
+template <typename T, int K, bool WHOLE>
 __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, int dv, int cw, int tiles) {
     constexpr int E = conv_e<T>(), NB = 4;
     constexpr int W = E * (K + 1);
@@ -138,7 +140,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
     const int rt = threadIdx.x / cw, nrt = 256 / cw;
     const int cv = blockIdx.y * cw + threadIdx.x % cw;
     const int c0 = cv * E;
-    const int n = p.D - c0 < E ? p.D - c0 : E;
+    const int n = WHOLE || p.D - c0 >= E ? E : p.D - c0, width = WHOLE ? E : p.D;
     float dw[K][E] = {}, db[E] = {};
     if (cv < dv) {
         float w[K][E], bias[E];
@@ -159,12 +161,12 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const bool on = t + j < len;
-                    xr[j] = on ? row_at<T>(x + (t + j) * p.x_t, n, p.D) : no_row<T>();
-                    yr[j] = on ? row_at<T>(dy + (long)(t + j) * p.D, n, p.D) : no_row<T>();
+                    xr[j] = on ? row_at<T>(x + (t + j) * p.x_t, n, width) : no_row<T>();
+                    yr[j] = on ? row_at<T>(dy + (long)(t + j) * p.D, n, width) : no_row<T>();
                 }
             };
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n);
+            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
             read(t0);
             float xw[K][E], gw[K][E];
 #pragma unroll
@@ -218,7 +220,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c) o[c] = 0.f;
                     const int tail = ti - (len - (K - 1));
                     if (ds1 && tail >= 0 && tail < K - 1) {
-                        const Pack<T> v = row_at<T>(ds1 + (long)tail * p.D, n, p.D);
+                        const Pack<T> v = row_at<T>(ds1 + (long)tail * p.D, n, width);
 #pragma unroll
                         for (int c = 0; c < E; ++c) o[c] = v.get(c);
                     }
@@ -226,8 +228,8 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c)
 #pragma unroll
                         for (int k = 0; k < K; ++k) o[c] = fmaf(w[K - 1 - k][c], gw[k][c], o[c]);
-                    if (ti >= 0) put_row<T>(dx + (long)ti * p.D, n, p.D, o);
-                    else put_row<T>(ds0 + (long)(ti + K - 1) * p.D, n, p.D, o);
+                    if (ti >= 0) put_row<T>(dx + (long)ti * p.D, n, width, o);
+                    else put_row<T>(ds0 + (long)(ti + K - 1) * p.D, n, width, o);
                 }
             }
         }
@@ -314,8 +316,11 @@ struct Fwd {
         const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const long items = (long)p.B * tiles * dv;
-        hipLaunchKernelGGL((short_conv_fwd_kernel<T, K>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p,
-                           items, dv, tiles);
+        const dim3 grid((unsigned)((items + 255) / 256));
+        if (p.D % conv_e<T>() == 0)
+            hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, true>), grid, dim3(256), 0, s, p, items, dv, tiles);
+        if (p.D % conv_e<T>() != 0)
+            hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, false>), grid, dim3(256), 0, s, p, items, dv, tiles);
     }
 };
 
@@ -328,8 +333,11 @@ struct Bwd {
         const int cw = conv_cw(dv);
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const size_t smem = 256 * conv_e<T>() * (K + 1) * sizeof(float);
-        hipLaunchKernelGGL((short_conv_bwd_kernel<T, K>), dim3(p.slots, (dv + cw - 1) / cw), dim3(256), smem, s, p, dv,
-                           cw, tiles);
+        const dim3 grid(p.slots, (dv + cw - 1) / cw);
+        if (p.D % conv_e<T>() == 0)
+            hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, true>), grid, dim3(256), smem, s, p, dv, cw, tiles);
+        if (p.D % conv_e<T>() != 0)
+            hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, false>), grid, dim3(256), smem, s, p, dv, cw, tiles);
     }
 };
 
