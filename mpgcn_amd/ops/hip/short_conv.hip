@@ -11,38 +11,39 @@
 namespace {
 
 template <typename T>
-constexpr int conv_e() { return 16 / sizeof(T); }  // channels a thread
+constexpr int conv_e() { return 16 / sizeof(T); }  // channels a thread, forward
+#define CONV_BE 4  // backward: with 8 of bf16 its windows and sums would take all registers and some more
 
 __device__ __forceinline__ float silu_f(float s) { return s * fast_sigmoid(s); }
 
-// A thread's channels at one step; n of them are there, D in a row.
-template <typename T>
-__device__ __forceinline__ Pack<T> row_at(const T* p, int n, int D) {
-    Pack<T> r;
-    r.load(p, n, D % conv_e<T>());
+// A thread's E channels at one step; n of them are there, D in a row.
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> row_at(const T* p, int n, int D) {
+    Pack<T, E> r;
+    r.load(p, n, D % E);
     return r;
 }
-template <typename T>
-__device__ __forceinline__ void put_row(T* p, int n, int D, const float (&v)[conv_e<T>()]) {
-    Pack<T> r;
+template <typename T, int E>
+__device__ __forceinline__ void put_row(T* p, int n, int D, const float (&v)[E]) {
+    Pack<T, E> r;
     r.set(v);
-    r.store(p, n, D % conv_e<T>());
+    r.store(p, n, D % E);
 }
-template <typename T>
-__device__ __forceinline__ Pack<T> no_row() {
-    Pack<T> r;
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> no_row() {
+    Pack<T, E> r;
     r.clear();
     return r;
 }
 
 // Input t of a sequence: the carried state before the first, zero before that
 // and past the end.
-template <typename T, int K>
-__device__ __forceinline__ Pack<T> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n,
-                                             int width) {
-    if (t >= 0 && t < len) return row_at<T>(x + t * p.x_t, n, width);
-    if (t < 0 && t >= -(K - 1) && s0) return row_at<T>(s0 + (long)(t + K - 1) * p.D, n, width);
-    return no_row<T>();
+template <typename T, int E, int K>
+__device__ __forceinline__ Pack<T, E> input_row(const ShortConvParams& p, const T* x, const T* s0, int t, int len, int n,
+                                                int width) {
+    if (t >= 0 && t < len) return row_at<T, E>(x + t * p.x_t, n, width);
+    if (t < 0 && t >= -(K - 1) && s0) return row_at<T, E>(s0 + (long)(t + K - 1) * p.D, n, width);
+    return no_row<T, E>();
 }
 
 template <int K, int E>
@@ -59,7 +60,7 @@ __device__ __forceinline__ void taps(const float* w, const float* bias, int c0, 
 // WHOLE: every thread has all of its channels, and no code for fewer.
 template <typename T, int K, bool WHOLE>
 __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv, int tiles) {
-    constexpr int E = conv_e<T>(), NB = 8;
+    constexpr int E = conv_e<T>(), NB = 4;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
     const int c0 = (int)(i % dv) * E;
@@ -72,19 +73,19 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
     const int t0 = tile * p.tile, t1 = t0 + p.tile < p.L ? t0 + p.tile : p.L;
     T* y = (T*)p.y + ((long)b * p.L + t0) * p.D + c0;
 
-    Pack<T> raw[NB];
+    Pack<T, E> raw[NB];
     float w[K][E], bias[E], win[K][E];
     auto read = [&](int t) {
         const T* s = x + t * p.x_t;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            raw[j] = t + j < len ? row_at<T>(s, n, width) : no_row<T>();
+            raw[j] = t + j < len ? row_at<T, E>(s, n, width) : no_row<T, E>();
             s += p.x_t;
         }
     };
-    Pack<T> edge[K - 1];
+    Pack<T, E> edge[K - 1];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
+    for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, E, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
     read(t0);
     taps<K, E>(p.w, p.bias, c0, n, w, bias);
 #pragma unroll
@@ -92,7 +93,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
 #pragma unroll
         for (int c = 0; c < E; ++c) win[k + 1][c] = edge[k].get(c);
     for (int t = t0; t < t1; t += NB) {
-        Pack<T> cur[NB];
+        Pack<T, E> cur[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) cur[j] = raw[j];
         if (t + NB < t1) read(t + NB);
@@ -109,7 +110,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
                 for (int k = 0; k < K; ++k) s = fmaf(w[k][c], win[k][c], s);
                 o[c] = t + j < len ? (p.silu ? silu_f(s) : s) : 0.f;
             }
-            if (t + j < t1) put_row<T>(y, n, width, o);
+            if (t + j < t1) put_row<T, E>(y, n, width, o);
             y += p.D;
         }
     }
@@ -117,11 +118,11 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
         T* s1 = (T*)p.s1 + (long)b * (K - 1) * p.D + c0;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            const Pack<T> v = input_row<T, K>(p, x, s0, len - (K - 1) + j, len, n, width);
+            const Pack<T, E> v = input_row<T, E, K>(p, x, s0, len - (K - 1) + j, len, n, width);
             float o[E];
 #pragma unroll
             for (int c = 0; c < E; ++c) o[c] = v.get(c);
-            put_row<T>(s1 + (long)j * p.D, n, width, o);
+            put_row<T, E>(s1 + (long)j * p.D, n, width, o);
         }
     }
 }
@@ -134,7 +135,7 @@ __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, 
 // (no atomics).
 template <typename T, int K, bool WHOLE>
 __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, int dv, int cw, int tiles) {
-    constexpr int E = conv_e<T>(), NB = 4;
+    constexpr int E = CONV_BE, NB = 4;
     constexpr int W = E * (K + 1);
     extern __shared__ float lds[];  // [256][W]
     const int rt = threadIdx.x / cw, nrt = 256 / cw;
@@ -156,17 +157,17 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
             const T* dy = (const T*)p.dy + (long)b * p.L * p.D + c0;
             T* dx = (T*)p.dx + (long)b * p.L * p.D + c0;
             T* ds0 = p.ds0 ? (T*)p.ds0 + (long)b * (K - 1) * p.D + c0 : nullptr;
-            Pack<T> xr[NB], yr[NB], edge[K - 1];
+            Pack<T, E> xr[NB], yr[NB], edge[K - 1];
             auto read = [&](int t) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const bool on = t + j < len;
-                    xr[j] = on ? row_at<T>(x + (t + j) * p.x_t, n, width) : no_row<T>();
-                    yr[j] = on ? row_at<T>(dy + (long)(t + j) * p.D, n, width) : no_row<T>();
+                    xr[j] = on ? row_at<T, E>(x + (t + j) * p.x_t, n, width) : no_row<T, E>();
+                    yr[j] = on ? row_at<T, E>(dy + (long)(t + j) * p.D, n, width) : no_row<T, E>();
                 }
             };
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
+            for (int k = 0; k < K - 1; ++k) edge[k] = input_row<T, E, K>(p, x, s0, t0 - (K - 1) + k, len, n, width);
             read(t0);
             float xw[K][E], gw[K][E];
 #pragma unroll
@@ -179,7 +180,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
             // The first tile starts with the outputs whose window holds the
             // carried state, so it emits that state's gradient as it goes.
             for (int tb = t0; tb < t1 + K - 1; tb += NB) {
-                Pack<T> xc[NB], yc[NB];
+                Pack<T, E> xc[NB], yc[NB];
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     xc[j] = xr[j];
@@ -220,7 +221,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c) o[c] = 0.f;
                     const int tail = ti - (len - (K - 1));
                     if (ds1 && tail >= 0 && tail < K - 1) {
-                        const Pack<T> v = row_at<T>(ds1 + (long)tail * p.D, n, width);
+                        const Pack<T, E> v = row_at<T, E>(ds1 + (long)tail * p.D, n, width);
 #pragma unroll
                         for (int c = 0; c < E; ++c) o[c] = v.get(c);
                     }
@@ -228,8 +229,8 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
                     for (int c = 0; c < E; ++c)
 #pragma unroll
                         for (int k = 0; k < K; ++k) o[c] = fmaf(w[K - 1 - k][c], gw[k][c], o[c]);
-                    if (ti >= 0) put_row<T>(dx + (long)ti * p.D, n, width, o);
-                    else put_row<T>(ds0 + (long)(ti + K - 1) * p.D, n, width, o);
+                    if (ti >= 0) put_row<T, E>(dx + (long)ti * p.D, n, width, o);
+                    else put_row<T, E>(ds0 + (long)(ti + K - 1) * p.D, n, width, o);
                 }
             }
         }
@@ -329,14 +330,14 @@ struct Bwd {
     hipStream_t s;
     template <typename T, int K>
     void operator()() const {
-        const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
+        const int dv = (p.D + CONV_BE - 1) / CONV_BE;
         const int cw = conv_cw(dv);
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
-        const size_t smem = 256 * conv_e<T>() * (K + 1) * sizeof(float);
+        const size_t smem = 256 * CONV_BE * (K + 1) * sizeof(float);
         const dim3 grid(p.slots, (dv + cw - 1) / cw);
-        if (p.D % conv_e<T>() == 0)
+        if (p.D % CONV_BE == 0)
             hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, true>), grid, dim3(256), smem, s, p, dv, cw, tiles);
-        if (p.D % conv_e<T>() != 0)
+        if (p.D % CONV_BE != 0)
             hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, false>), grid, dim3(256), smem, s, p, dv, cw, tiles);
     }
 };
@@ -358,7 +359,7 @@ struct Step {
 // The tile of p and, for the backward, the blocks that share a channel group:
 // each writes a row of filter gradients.
 extern "C" void short_conv_plan(ShortConvParams* p, int is_f32, int back) {
-    const long e = is_f32 ? 4 : 8, dv = (p->D + e - 1) / e;
+    const long e = back ? CONV_BE : is_f32 ? 4 : 8, dv = (p->D + e - 1) / e;
     // 16 waves a CU forward, 8 backward: what the registers allow
     p->tile = conv_tile(p->B, p->L, dv, back ? 256L * 8 * 64 : 256L * 16 * 64);
     const long cw = conv_cw(dv), groups = (dv + cw - 1) / cw, rows = 256 / cw;
