@@ -578,50 +578,78 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
 }
 
 // Turns each segment's own end state into the state it starts from (forward),
-// or its own adjoint at the start into the one at its end (backward). One
-// thread per four states; all loads of 16 segments are in flight together.
+// or its own adjoint at the start into the one at its end (backward). A block
+// takes four states of a task's lanes; its waves share the segments: each runs
+// through its part from zero, the parts are joined in LDS, and each runs
+// through again from where the parts before it end. The loads of 16 segments
+// are in flight together.
 template <int NQ, int KQ, bool BACK>
-__launch_bounds__(256) __global__ void scan_carry_kernel(ScanParams p, ScanPlan l, long waves) {
-    const int lane = threadIdx.x & 63;
-    const long w = (long)blockIdx.x * 4 + wave_id();
-    if (w >= waves) return;
-    const int i = (int)(w % NQ);
-    const long id = w / NQ;
+__launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan l) {
+    __shared__ f32x4 end[16][64];
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = wave_id(), waves = blockDim.x / 64;
+    const int i = (int)(blockIdx.x % NQ);
+    const long id = blockIdx.x / NQ;
     const Place<NQ, KQ> q(p, l, lane, (int)(id / l.cb % p.G), (int)(id % l.cb));
     const long b = id / l.cb / p.G * l.rw + q.rs;
     const float* first = BACK ? p.dh1 : p.h0;
-    f32x4 A2, carry;
+    f32x4 A2, carry = {0.f, 0.f, 0.f, 0.f}, start;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const bool on = q.state(p, c, i);
         A2[c] = pick(p.A, on, (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
-        carry[c] = first ? pick(first, on && b < p.B, (b * p.D + q.d4 + c) * p.N + q.n0 + i) : 0.f;
+        start[c] = first ? pick(first, on && b < p.B, (b * p.D + q.d4 + c) * p.N + q.n0 + i) : 0.f;
     }
     f32x4* seg_h = (f32x4*)p.seg_h + (id * l.nseg * NQ + i) * 64 + lane;
     const float* seg_s = p.seg_s + id * l.nseg * 64 + lane;
+    const int part = (l.nseg + waves - 1) / waves, s_lo = wave * part;
+    const int s_hi = s_lo + part < l.nseg ? s_lo + part : l.nseg;
     constexpr int U = 16;
-    for (int s0 = 0; s0 < l.nseg; s0 += U) {
-        f32x4 own[U];
-        float sum[U];
+    auto run = [&](bool out, float& total) {
+        for (int s0 = s_lo; s0 < s_hi; s0 += U) {
+            f32x4 own[U];
+            float sum[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            // the last one in order has no successor: nothing was stored for it
-            const int s = s0 + j < l.nseg - 1 ? s0 + j : 0;
-            const long at = BACK ? l.nseg - 1 - s : s;
-            own[j] = seg_h[at * NQ * 64];
-            sum[j] = seg_s[at * 64];
+            for (int j = 0; j < U; ++j) {
+                // the last one in order has no successor: nothing was stored for it
+                const int s = s0 + j < l.nseg - 1 ? s0 + j : 0;
+                const long at = BACK ? l.nseg - 1 - s : s;
+                own[j] = seg_h[at * NQ * 64];
+                sum[j] = seg_s[at * 64];
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int s = s0 + j;
+                const bool on = s < s_hi;
+                const long at = BACK ? l.nseg - 1 - s : s;
+                if (out && on) seg_h[at * NQ * 64] = carry;
+                float ss[4];
+                const float sj = on ? sum[j] : 0.f;
+                quad_spread(sj, ss);
+                total += sj;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    carry[c] = fmaf(__builtin_amdgcn_exp2f(ss[c] * A2[c]), carry[c], on ? own[j][c] : 0.f);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int s = s0 + j;
-            const long at = BACK ? l.nseg - 1 - s : s;
-            if (s < l.nseg) seg_h[at * NQ * 64] = carry;
+    };
+    float total = 0.f;
+    if (waves > 1) {
+        run(false, total);
+        end[wave][lane] = carry;
+        sums[wave][lane] = total;
+        __syncthreads();
+        carry = start;
+        for (int v = 0; v < wave; ++v) {
             float ss[4];
-            quad_spread(sum[j], ss);
+            quad_spread(sums[v][lane], ss);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) carry[c] = fmaf(__builtin_amdgcn_exp2f(ss[c] * A2[c]), carry[c], own[j][c]);
+            for (int c = 0; c < 4; ++c) carry[c] = fmaf(__builtin_amdgcn_exp2f(ss[c] * A2[c]), carry[c], end[v][lane][c]);
         }
+    } else {
+        carry = start;
     }
+    run(true, total);
 }
 
 // ---- backward ---------------------------------------------------------------
@@ -983,6 +1011,12 @@ struct Typed {
 
 inline dim3 wave_blocks(long waves) { return dim3((unsigned)((waves + 3) / 4)); }
 
+// About 16 segments a wave of the carry.
+inline dim3 carry_threads(const ScanPlan& l) {
+    const int waves = (l.nseg + 15) / 16;
+    return dim3(64 * (waves < 16 ? waves : 16));
+}
+
 struct ScanFwd {
     const ScanParams& p;
     const ScanPlan& l;
@@ -993,8 +1027,7 @@ struct ScanFwd {
         if (l.nseg > 1) {
             hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, false>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256),
                                0, s, ScanArgs{p, l});
-            hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, false>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
-                               tasks * NQ);
+            hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, false>), dim3((unsigned)(tasks * NQ)), carry_threads(l), 0, s, p, l);
         }
         hipLaunchKernelGGL((scan_fwd_kernel<T, NQ, KQ, true>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0,
                            s, ScanArgs{p, l});
@@ -1011,8 +1044,7 @@ struct ScanBwd {
         if (l.nseg > 1) {
             hipLaunchKernelGGL((scan_adjoint_kernel<T, NQ, KQ>), wave_blocks((long)l.fslots * p.G * l.cb), dim3(256), 0, s,
                                ScanArgs{p, l});
-            hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, true>), wave_blocks(tasks * NQ), dim3(256), 0, s, p, l,
-                               tasks * NQ);
+            hipLaunchKernelGGL((scan_carry_kernel<NQ, KQ, true>), dim3((unsigned)(tasks * NQ)), carry_threads(l), 0, s, p, l);
         }
         hipLaunchKernelGGL((scan_bwd_kernel<T, NQ, KQ>), wave_blocks((long)l.slots * p.G * l.cb), dim3(256), 0, s,
                            ScanArgs{p, l});
@@ -1048,7 +1080,9 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32, int back) {
     // prompt of 16384 x 2048: 297 us against 317 with two.
     const long tasks = l.groups * p.G * l.cb, same = (long)p.G * l.cb;
     long nseg = tasks ? (back ? 2048 : 4096) / tasks : 1;
-    if (nseg > l.chunks / 4) nseg = l.chunks / 4;
+    // (two chunks where even so a quarter of the card would have no wave)
+    const long least = tasks * (l.chunks / 4) < 1024 ? 2 : 4;
+    if (nseg > l.chunks / least) nseg = l.chunks / least;
     if (nseg < 3) nseg = 1;
     l.seg_chunks = (int)(l.chunks ? (l.chunks + nseg - 1) / nseg : 1);
     l.nseg = l.chunks ? (l.chunks + l.seg_chunks - 1) / l.seg_chunks : 1;
