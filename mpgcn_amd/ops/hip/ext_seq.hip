@@ -2,6 +2,7 @@
 // scan, norms around a block. mpgcn_amd/ops/sequence.py checks the arguments
 // for its users; what the kernels rely on for their bounds is checked here too.
 #include <torch/extension.h>
+#include <cfloat>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPException.h>
@@ -170,6 +171,7 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     const long N = A.size(1);
     TORCH_CHECK(Bm.dim() == 4 && Bm.size(2) >= 1 && D % Bm.size(2) == 0, "B must be (B, L, G, N), G a divisor of D");
     const long G = Bm.size(2);
+    TORCH_CHECK(D < (1L << 26), "at most 2^26 channels");
     check_data(u, u, u.sizes(), "u");
     check_data(delta, u, {B, L, D}, "delta");
     check_data(Bm, u, {B, L, G, N}, "B");
@@ -613,7 +615,7 @@ py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor B
 }
 
 py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps, bool prepared) {
-    if (!x.is_cuda() || x.dim() < 1 || !(eps > 0)) return py::none();
+    if (!x.is_cuda() || x.dim() < 1 || !(eps >= FLT_MIN)) return py::none();
     const bool train = wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)});
     if (train && !prepared && capturing()) return py::none();
     return direct(prepared, [&]() -> py::object {

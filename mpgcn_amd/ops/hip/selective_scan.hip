@@ -142,9 +142,10 @@ struct Place {
 
 // log(1 + e^x) and its slope. e^-|x| with the argument's rounding put right,
 // the logarithm of 1 + e with that sum's: a few 2^-24 of the result over the
-// whole range.
+// whole range. Past the exponent's range the remainder is infinite or NaN and e
+// is 0: the bound keeps their product 0.
 __device__ __forceinline__ float softplus_s(float x, float& slope) {
-    const float a = -fabsf(x), hi = a * LOG2E, lo = fmaf(a, LOG2E, -hi);
+    const float a = -fabsf(x), hi = a * LOG2E, lo = fminf(fmaf(a, LOG2E, -hi), 1.f);
     float e = __builtin_amdgcn_exp2f(hi);
     e = fmaf(e * lo, LN2, e);
     const float s = 1.f + e, r = __builtin_amdgcn_rcpf(s);
@@ -932,61 +933,62 @@ __launch_bounds__(256) __global__ void scan_bc_reduce_kernel(const float* __rest
                                                              int G, int N, int NP) {
     // a thread: four padded states of one row, of dB and dC in turn
     const int pr = 2 * NP / 4;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const long row = i / pr;
-    if (row >= rows) return;
-    const int k = (int)(i % pr) * 4, which = k >= NP, n0 = which ? k - NP : k;
-    const int g = (int)(row % G);
-    const long bt = row / G, b = bt / L, t = bt % L;
     const long Lp = (L + SCAN_CH - 1) / SCAN_CH * SCAN_CH;
-    const f32x4* src = (const f32x4*)dbc + ((b * G + g) * Lp + t) * pr + k / 4;
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < cblocks; ++c) s += src[(long)c * B * G * Lp * pr];
-    T* o = (which ? dC : dB) + row * N + n0;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * pr; i += (long)gridDim.x * 256) {
+        const long row = i / pr;
+        const int k = (int)(i % pr) * 4, which = k >= NP, n0 = which ? k - NP : k;
+        const int g = (int)(row % G);
+        const long bt = row / G, b = bt / L, t = bt % L;
+        const f32x4* src = (const f32x4*)dbc + ((b * G + g) * Lp + t) * pr + k / 4;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < cblocks; ++c) s += src[(long)c * B * G * Lp * pr];
+        T* o = (which ? dC : dB) + row * N + n0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (n0 + j < N) o[j] = from_f32<T>(s[j]);
+        for (int j = 0; j < 4; ++j)
+            if (n0 + j < N) o[j] = from_f32<T>(s[j]);
+    }
 }
 
 // One new token. Bound by the state, read and written once: 4 states (16
-// bytes) a lane, `gp` lanes a channel, joined by lane exchanges for y. Every
-// lane reads its own states before it writes them: h_out may be h.
+// bytes) a lane, `gp` lanes a channel, joined by lane exchanges for y. A thread
+// keeps its channel and takes one sequence after another. Every lane reads its
+// own states before it writes them: h_out may be h.
 template <typename T>
-__launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp, long items) {
+__launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const bool ok = i < items;
-    const long r = ok ? i / gp : 0;
-    const int n0 = ok ? (int)(i % gp) * 4 : p.N;
-    const int d = (int)(r % p.D);
-    const long b = r / p.D;
-    const int g = d / (p.D / p.G);
-    const int N = p.N;
-    const float uv = to_f32(((const T*)p.u)[b * p.u_b + d]);
-    float dt = to_f32(((const T*)p.delta)[b * p.d_b + d]) + (p.dbias ? p.dbias[d] : 0.f);
-    float slope;
-    if (p.softplus) dt = softplus_s(dt, slope);
-    const T* Bm = (const T*)p.Bm + b * p.B_b + g * p.B_g;
-    const T* Cm = (const T*)p.Cm + b * p.C_b + g * p.C_g;
-    const float* h = p.h + r * N;
-    const float* A = p.A + (long)d * N;
+    const bool ok = i / gp < p.D;
+    const int d = ok ? (int)(i / gp) : 0, N = p.N;
+    const int n0 = ok ? (int)(i % gp) * 4 : N;
     const int n = n0 < N ? N - n0 : 0, at = n ? n0 : 0;
-    Pack<float> hp, Ap;
-    Pack<T, 4> Bp, Cp;
-    hp.load(h + at, n, N % 4);
-    Ap.load(A + at, n, N % 4);
-    Bp.load(Bm + at, n, N % 4);
-    Cp.load(Cm + at, n, N % 4);
-    float acc = 0.f;
+    const int g = d / (p.D / p.G);
+    Pack<float> Ap;
+    Ap.load(p.A + (long)d * N + at, n, N % 4);
+    float A2[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float v = fmaf(__builtin_amdgcn_exp2f(dt * (Ap.get(j) * LOG2E)), hp.get(j), dt * uv * Bp.get(j));
-        hp.w[j] = __float_as_int(v);
-        acc = fmaf(Cp.get(j), v, acc);
+    for (int j = 0; j < 4; ++j) A2[j] = Ap.get(j) * LOG2E;
+    const float dbias = p.dbias ? p.dbias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
+    for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+        const long r = (long)b * p.D + d;
+        Pack<float> hp;
+        Pack<T, 4> Bp, Cp;
+        hp.load(p.h + r * N + at, n, N % 4);
+        Bp.load((const T*)p.Bm + b * p.B_b + g * p.B_g + at, n, N % 4);
+        Cp.load((const T*)p.Cm + b * p.C_b + g * p.C_g + at, n, N % 4);
+        const float uv = to_f32(((const T*)p.u)[b * p.u_b + d]);
+        const float x = to_f32(((const T*)p.delta)[b * p.d_b + d]) + dbias;
+        float slope;
+        const float dt = p.softplus ? softplus_s(x, slope) : x, du = dt * uv;
+        float acc = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), hp.get(j), du * Bp.get(j));
+            hp.w[j] = __float_as_int(v);
+            acc = fmaf(Cp.get(j), v, acc);
+        }
+        for (int m = 1; m < gp; m <<= 1) acc += __shfl_xor(acc, m);
+        hp.store(p.h_out + r * N + at, n, N % 4);
+        if (ok && n0 == 0) ((T*)p.y)[r] = from_f32<T>(fmaf(skip, uv, acc));
     }
-    for (int m = 1; m < gp; m <<= 1) acc += __shfl_xor(acc, m);
-    if (!ok) return;
-    hp.store(p.h_out + r * N + at, n, N % 4);
-    if (n0 == 0) ((T*)p.y)[b * p.D + d] = from_f32<T>(p.skip ? fmaf(p.skip[d], uv, acc) : acc);
 }
 
 template <typename F>
@@ -1107,7 +1109,8 @@ extern "C" void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, in
                                       hipStream_t s) {
     const int NP = l.state / (4 * l.cw * l.rw) * 4;
     const long rows = (long)p.B * p.L * p.G;
-    const dim3 grid((unsigned)((rows * (2 * NP / 4) + 255) / 256));
+    const long blocks = (rows * (2 * NP / 4) + 255) / 256;
+    const dim3 grid((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20));
     if (is_f32) {
         hipLaunchKernelGGL((scan_bc_reduce_kernel<float>), grid, dim3(256), 0, s, p.dbc, (float*)p.dB, (float*)p.dC, l.cb, rows,
                            p.B, p.L, p.G, p.N, NP);
@@ -1119,11 +1122,13 @@ extern "C" void scan_bc_reduce_launch(const ScanParams& p, const ScanPlan& l, in
 
 extern "C" void scan_step_launch(const ScanStepParams& p, int is_f32, hipStream_t s) {
     const int gp = pow2_ceil((p.N + 3) / 4);
-    const long items = (long)p.B * p.D * gp;
-    const dim3 grid((unsigned)((items + 255) / 256));
+    const long across = ((long)p.D * gp + 255) / 256;
+    long down = 8192 / across;  // some rounds of full occupancy
+    down = down < 1 ? 1 : down > 65535 ? 65535 : down;
+    const dim3 grid((unsigned)across, (unsigned)(p.B < down ? p.B : down));
     if (is_f32) {
-        hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, s, p, gp, items);
+        hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, s, p, gp);
     } else {
-        hipLaunchKernelGGL((scan_step_kernel<__bf16>), grid, dim3(256), 0, s, p, gp, items);
+        hipLaunchKernelGGL((scan_step_kernel<__bf16>), grid, dim3(256), 0, s, p, gp);
     }
 }

@@ -36,6 +36,8 @@ from mpgcn_amd.ops import eager
 
 _MAX_STATES = 64
 _MAX_NORM_D = 16384
+_MIN_EPS = torch.finfo(torch.float32).tiny
+_MAX_STEP = 1 << 26  # elements between tokens that the scan's 32-bit lane offsets allow
 
 
 def _on_gpu(t) -> bool:
@@ -238,6 +240,8 @@ def _check_scan(u, delta, A, B, C, lead):
     if u.dim() != len(lead) + 1:
         raise ValueError(f"u must be ({', '.join(lead)}, channels), got {tuple(u.shape)}")
     D = u.shape[-1]
+    if D >= _MAX_STEP:
+        raise ValueError(f"u must have fewer than {_MAX_STEP} channels, got {D}")
     _check_act(delta, "delta", u.shape, u)
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != D:
         raise ValueError(f"A must have shape ({D}, N)")
@@ -296,7 +300,8 @@ def selective_scan(u, delta, A, B, C, skip=None, *, delta_bias=None, delta_softp
     if not u.is_cuda:
         y, last = eager.selective_scan_eager(u, delta, A, B, C, skip, delta_bias, softplus, state, lengths)
         return (y, last) if return_state else y
-    u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
+    u, delta, B, C = (t.contiguous() if t.shape[1] > 1 and t.stride(1) >= _MAX_STEP else _rows(t)
+                      for t in (u, delta, B, C))
     state = None if state is None else state.contiguous()
     _check_capture(u, delta, A, B, C, skip, delta_bias, state)
     return _ops.get_ext().selective_scan_direct(u, delta, A, B, C, skip, delta_bias, state, lengths, softplus,
@@ -360,8 +365,8 @@ def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=N
         raise ValueError("post_weight or pre_weight is needed")
     if residual is None and (scale is not None or pre_weight is not None):
         raise ValueError("scale and pre_weight need a residual")
-    if not eps > 0:
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not eps >= _MIN_EPS:
+        raise ValueError(f"eps must be at least {_MIN_EPS:.3g} (a normal float32), got {eps}")
     if gate is not None:
         _check_act(gate, "gate", x.shape, x)
     if residual is not None:

@@ -223,6 +223,8 @@ def test_extreme_decays_and_padding():
     n = torch.tensor([20, 4, 0], device=DEV)
     t["delta"][0, :5] = -200.0
     t["delta"][0, 5:9] = 1000.0
+    t["delta"][0, 9] = -3e38
+    t["delta"][0, 10] = float("-inf")
     t["A"][3] = -1e30
     clean = {k: v.clone() for k, v in t.items()}
     for k in ("u", "delta", "B", "C"):
@@ -539,3 +541,78 @@ def test_converted_arguments():
     oracle.within(gx, *ref["x"], oracle.conv_roundings(3))
     assert gw.dtype == BF
     oracle.within(gw, *ref["weight"], oracle.conv_roundings(3) + 24)
+
+
+def test_offsets_beyond_32_bits():
+    """Sequences 2^31 elements apart, and more than 2^31 elements in one tensor."""
+    pool = torch.empty(2 ** 31 + 4096, device=DEV, dtype=BF)
+    far = pool.as_strided((2, 6, 32), (2 ** 31 + 8, 64, 1))
+    near = rn(gen(110), 2, 6, 32, dtype=BF)
+    far.copy_(near)
+    # bit for bit; the raw steps (no softplus) grow some states past the range, where the formula gives NaN
+    same = lambda a, b: torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
+    w = rn(gen(111), 32, 4)
+    assert torch.equal(ops.short_conv(far, w), ops.short_conv(near, w))
+    t, _ = scan_case(112, BF, 2, 6, 32, 16, 1, False, None)
+    same(ops.selective_scan(**{**t, "u": far, "delta": far}), ops.selective_scan(**{**t, "u": near, "delta": near}))
+    step = pool.as_strided((3, 6, 8), (64, 2 ** 28, 1))  # tokens too far apart for lane offsets: a copy
+    step.copy_(near[:1, :, :8].expand(3, 6, 8))
+    t, _ = scan_case(113, BF, 3, 6, 8, 4, 1, False, None)
+    same(ops.selective_scan(**{**t, "u": step}), ops.selective_scan(**{**t, "u": step.contiguous()}))
+    rows = pool.as_strided((2, 40), (2 ** 31 + 8, 1))
+    rows.copy_(near[:, 0].repeat(1, 2)[:, :40])
+    pw = rn(gen(114), 40)
+    assert torch.equal(ops.norm_gate_residual(rows, post_weight=pw),
+                       ops.norm_gate_residual(rows.contiguous(), post_weight=pw))
+    del far, step, rows
+    # one tensor of 2^31 + elements: its end equals the end computed alone
+    L = 2 ** 31 // 32 + 64
+    x = pool[: L * 32].view(1, L, 32)
+    x.normal_()
+    y, last = ops.short_conv(x, w, return_state=True)
+    tail, last2 = ops.short_conv(x[:, -50:].contiguous(), w, return_state=True)
+    assert torch.equal(y[:, -40:], tail[:, -40:]) and torch.equal(last, last2)
+    del y
+    n = ops.norm_gate_residual(x[0], post_weight=w[:, 0])
+    assert torch.equal(n[-70:], ops.norm_gate_residual(x[0, -70:].contiguous(), post_weight=w[:, 0]))
+
+
+def test_long_sequence_equals_its_parts():
+    """65 k tokens in one call, in segments, against two calls that hand the
+    state over: the same recurrence from other segment starts."""
+    t, _ = scan_case(120, F, 1, 65536, 40, 16, 1, True, None)
+    kw = dict(delta_softplus=True, return_state=True)
+    y, h = ops.selective_scan(**t, **kw)
+    cut = 33333
+    part = lambda a, b: {k: v[:, a:b] if k in ("u", "delta", "B", "C") else v for k, v in t.items()}
+    y1, h1 = ops.selective_scan(**part(0, cut), **kw)
+    y2, h2 = ops.selective_scan(**{**part(cut, None), "state": h1}, **kw)
+    # states forget within some hundred steps: 4 roundings a step of them
+    mag = float(y.abs().max())
+    assert float((torch.cat([y1, y2], 1) - y).abs().max()) <= 4 * 1000 * 2.0 ** -24 * mag
+    assert float((h2 - h).abs().max()) <= 4 * 1000 * 2.0 ** -24 * float(h.abs().max())
+
+
+@pytest.mark.parametrize("dtype,B,L,D,N,lengths", [
+    (BF, 2, 700, 96, 16, torch.int32), (F, 1, 1500, 33, 13, None), (BF, 3, 530, 24, 8, torch.int64),
+    (F, 2, 600, 40, 40, torch.int32)])
+def test_selective_scan_in_segments(dtype, B, L, D, N, lengths):
+    """Few long sequences: the time axis is cut, ends fall inside segments."""
+    check_scan(*scan_case(B + L, dtype, B, L, D, N, 1, True, lengths), dtype)
+
+
+def test_only_the_last_state_has_a_gradient():
+    """Both without segments and in them; skip and C see none of it."""
+    for L in (9, 700):
+        t, n = scan_case(130 + L, F, 2, L, 24, 16, 1, True, torch.int32)
+        dl = rn(gen(131), 2, 24, 16)
+        leaves = {k: v.requires_grad_() for k, v in t.items()}
+        _, last = ops.selective_scan(**t, lengths=n, delta_softplus=True, return_state=True)
+        got = dict(zip(leaves, grads([last], [dl], list(leaves.values()))))
+        ref = oracle.scan(**t, softplus=True, lengths=n, dy=torch.zeros(2, L, 24, device=DEV), dlast=dl)
+        r = oracle.scan_roundings(L, 16)
+        for name in ("u", "delta", "A", "B", "delta_bias", "state"):
+            more = 24 if name == "B" else 4 * L if name in ("A", "delta_bias") else 0
+            oracle.within(got[name], *ref[name], r + more, name)
+        for name in ("C", "skip"):
+            assert got[name] is None or not got[name].any(), name

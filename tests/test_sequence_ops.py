@@ -250,6 +250,9 @@ def test_selective_scan_refusals():
     ]:
         with pytest.raises(err):
             ops.selective_scan(**{**i, **kw})
+    wide = torch.empty(1, 1, 2 ** 26, device="meta")
+    with pytest.raises(ValueError):
+        ops.selective_scan(wide, wide, wide.view(-1, 1), wide[..., :1], wide[..., :1])
     s = dict(u=i["u"][:, 0], delta=i["delta"][:, 0], A=i["A"], B=i["B"][:, 0], C=i["C"][:, 0])
     with pytest.raises(ValueError):
         ops.selective_scan_step(**s, state=randn(2, 6, 4))
@@ -269,6 +272,7 @@ def test_norm_refusals():
         (ValueError, dict(post_weight=randn(7))),
         (ValueError, dict(post_weight=w, eps=0.0)),
         (ValueError, dict(post_weight=w, eps=float("nan"))),
+        (ValueError, dict(post_weight=w, eps=1e-40)),
         (ValueError, dict(post_weight=w, gate=randn(2, 8))),
         (TypeError, dict(post_weight=w, gate=x.bfloat16())),
         (TypeError, dict(post_weight=w, residual=x.half())),
