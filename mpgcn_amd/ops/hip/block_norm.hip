@@ -103,11 +103,13 @@ struct WeightsBack {
 
 // A thread keeps its columns and takes one row after another; with one chunk a
 // thread a row's loads are in flight while the row before is worked on.
-template <typename T, typename TR, int VPT, bool RES>
+// WHOLE: every piece is whole or absent, and there is no code for a partial one.
+template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
 __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, int tpr) {
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr;
+    const int width = WHOLE ? SEQ_CH : p.D;
     const float rd = 1.f / (float)p.D;
     const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
     long r = (long)blockIdx.x * rpb + threadIdx.x / tpr;
@@ -121,9 +123,9 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
             const int n = row < p.R ? p.D - c : 0;
-            xr[i].load((const T*)p.x + row * p.x_r + c, n, p.D);
-            if (p.gate) gr[i].load((const T*)p.gate + row * p.g_r + c, n, p.D);
-            if (RES) rr[i].load((const TR*)p.res + row * p.r_r + c, n, p.D);
+            xr[i].load((const T*)p.x + row * p.x_r + c, n, width);
+            if (p.gate) gr[i].load((const T*)p.gate + row * p.g_r + c, n, width);
+            if (RES) rr[i].load((const TR*)p.res + row * p.r_r + c, n, width);
         }
     };
     if (AHEAD) read(r);
@@ -160,7 +162,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * tpr + lane) * SEQ_CH;
-                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, p.D, v[i]);
+                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, width, v[i]);
             }
             continue;
         }
@@ -175,7 +177,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
                 hv[i][j] = fmaf(ws[j], v[i][j], hv[i][j]);  // zeros past the row's end
                 ss = fmaf(hv[i][j], hv[i][j], ss);
             }
-            if (live && c < p.D) store8<TR>((TR*)p.h + r * p.D + c, p.D - c, p.D, hv[i]);
+            if (live && c < p.D) store8<TR>((TR*)p.h + r * p.D + c, p.D - c, width, hv[i]);
         }
         if (p.pre) {
             const float inv = 1.f / sqrtf(row_sum(ss, tpr, lds, slot) * rd + p.eps);
@@ -187,7 +189,7 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
                 wt.template get<2>(p.pre, c, p.D, w2);
 #pragma unroll
                 for (int j = 0; j < SEQ_CH; ++j) hv[i][j] *= inv * w2[j];
-                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, p.D, hv[i]);
+                if (live && c < p.D) store8<T>((T*)p.y + r * p.D + c, p.D - c, width, hv[i]);
             }
         }
     }
@@ -200,13 +202,14 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 //   dp0 = inv1 (q - n1 mean(q n1));  dx, dgate by the product and silu'
 // Column gradients stay in registers over a thread's rows, are joined in LDS
 // over the block's row groups and written once per block.
-template <typename T, typename TR, int VPT, bool RES, bool GATE>
+template <typename T, typename TR, int VPT, bool RES, bool GATE, bool WHOLE>
 __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
     // the weights, then [rpb][VPT * tpr * SEQ_CH] to join the column gradients
     extern __shared__ __attribute__((aligned(16))) float dyn[];
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr, rg = threadIdx.x / tpr;
+    const int width = WHOLE ? SEQ_CH : p.D;
     const float rd = 1.f / (float)p.D;
     const long stride = (long)gridDim.x * rpb, rounds = (p.R + stride - 1) / stride;
     long r = (long)blockIdx.x * rpb + rg;
@@ -224,11 +227,11 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
             const int n = there ? p.D - c : 0;
-            xr[i].load((const T*)p.x + row * p.x_r + c, n, p.D);
-            if (GATE) gr[i].load((const T*)p.gate + row * p.g_r + c, n, p.D);
-            if (!RES || p.pre) yr[i].load((const T*)p.dy + row * p.D + c, p.dy ? n : 0, p.D);
-            if (RES && p.pre) rr[i].load((const TR*)p.res + row * p.r_r + c, n, p.D);
-            if (RES) hr[i].load((const TR*)p.dh + row * p.D + c, p.dh ? n : 0, p.D);
+            xr[i].load((const T*)p.x + row * p.x_r + c, n, width);
+            if (GATE) gr[i].load((const T*)p.gate + row * p.g_r + c, n, width);
+            if (!RES || p.pre) yr[i].load((const T*)p.dy + row * p.D + c, p.dy ? n : 0, width);
+            if (RES && p.pre) rr[i].load((const TR*)p.res + row * p.r_r + c, n, width);
+            if (RES) hr[i].load((const TR*)p.dh + row * p.D + c, p.dh ? n : 0, width);
         }
         if (p.post && there) i1 = p.inv1[row];
         if (RES && p.pre && there) i2 = p.inv2[row];
@@ -286,7 +289,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (RES && live && c < p.D) store8<TR>((TR*)p.dres + r * p.D + c, p.D - c, p.D, d[i]);
+            if (RES && live && c < p.D) store8<TR>((TR*)p.dres + r * p.D + c, p.D - c, width, d[i]);
             float w1[SEQ_CH], ws[SEQ_CH];
             wt.template get<0>(p.post, c, p.D, w1);
             if (RES) wt.template get<1>(p.scale, c, p.D, ws);
@@ -317,8 +320,8 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
                 }
             }
             if (live && c < p.D) {
-                store8<T>((T*)p.dx + r * p.D + c, p.D - c, p.D, o);
-                if (GATE) store8<T>((T*)p.dgate + r * p.D + c, p.D - c, p.D, og);
+                store8<T>((T*)p.dx + r * p.D + c, p.D - c, width, o);
+                if (GATE) store8<T>((T*)p.dgate + r * p.D + c, p.D - c, width, og);
             }
         }
     }
@@ -378,9 +381,9 @@ inline long row_blocks(long R, int tpr, int waves) {
 struct NormFwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool RES>
+    template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
     void operator()(int tpr) const {
-        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
+        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES, WHOLE>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
                            dim3(block_threads(tpr)), 0, s, p, tpr);
     }
 };
@@ -388,14 +391,16 @@ struct NormFwd {
 struct NormBwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool RES>
+    template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
     void operator()(int tpr) const {
         const int block = block_threads(tpr);
         const size_t smem = (size_t)block * SEQ_CH * sizeof(float) * (VPT > 1 ? VPT : RES ? 3 : 1);
         if (p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, true>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, true, WHOLE>), dim3(p.slots), dim3(block), smem,
+                               s, p, tpr);
         if (!p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, false>), dim3(p.slots), dim3(block), smem, s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, false, WHOLE>), dim3(p.slots), dim3(block), smem,
+                               s, p, tpr);
     }
 };
 
@@ -403,9 +408,10 @@ template <typename T, typename TR, bool RES, typename F>
 void by_shape(const BlockNormParams& p, F f) {
     int tpr, vpt;
     row_shape(p.D, &tpr, &vpt);
-    if (vpt == 1) f.template operator()<T, TR, 1, RES>(tpr);
-    else if (vpt == 2) f.template operator()<T, TR, 2, RES>(tpr);
-    else f.template operator()<T, TR, 4, RES>(tpr);
+    if (vpt == 1 && p.D % SEQ_CH == 0) f.template operator()<T, TR, 1, RES, true>(tpr);
+    else if (vpt == 1) f.template operator()<T, TR, 1, RES, false>(tpr);
+    else if (vpt == 2) f.template operator()<T, TR, 2, RES, false>(tpr);
+    else f.template operator()<T, TR, 4, RES, false>(tpr);
 }
 
 template <typename F>
