@@ -62,39 +62,45 @@ __device__ __forceinline__ float fold(float a, float b, int lane) {
     }
 }
 
-// v[c] of the quad's lanes summed; the lane with index c in its quad gets v[c].
-__device__ __forceinline__ float quad_sum(const float (&v)[4], int lane) {
-    return fold<1>(fold<2>(v[0], v[2], lane), fold<2>(v[1], v[3], lane), lane);
+// Lane l of a quad holds its channels in the order l, l^1, l^2, l^3: then what a
+// lane has for another's channel stands at the same index as in that lane what
+// it has for this one's, and the exchanges need no selects.
+
+// Each lane's channel summed over the quad.
+__device__ __forceinline__ float quad_sum(const float (&v)[4]) {
+    return (v[0] + dpp<0xB1>(v[1])) + (dpp<0x4E>(v[2]) + dpp<0x1B>(v[3]));
 }
 
 template <int KQ>
-__device__ __forceinline__ float states_sum(const float (&v)[4], int lane) {
-    float s = quad_sum(v, lane);
+__device__ __forceinline__ float states_sum(const float (&v)[4]) {
+    float s = quad_sum(v);
     if constexpr (KQ >= 2) s += from_xor<4>(s);
     if constexpr (KQ >= 4) s += from_xor<8>(s);
     return s;
 }
 
+// The quad's values of v in a lane's order.
 __device__ __forceinline__ void quad_spread(float v, float (&o)[4]) {
-    o[0] = dpp<0x00>(v);
-    o[1] = dpp<0x55>(v);
-    o[2] = dpp<0xAA>(v);
-    o[3] = dpp<0xFF>(v);
+    o[0] = v;
+    o[1] = dpp<0xB1>(v);
+    o[2] = dpp<0x4E>(v);
+    o[3] = dpp<0x1B>(v);
 }
 
-// Sum V values over the quads of a sequence: lane bits from M up to below
-// `span`. While a lane carries more than one value each step halves them.
-template <int M, int LEFT, int V>
+// Sum V values over the quads of a sequence: lane bits from below `span` down to
+// M0. While a lane carries more than one value each step halves them; the high
+// bits go first, whose exchange needs no selects.
+template <int M, int M0, int LEFT, int V>
 __device__ __forceinline__ void reduce_quads(float (&v)[V], int span, int lane) {
-    if constexpr (M <= 32) {
-        if (M >= span) return;
-        if constexpr (LEFT > 1) {
+    if constexpr (M >= M0) {
+        constexpr int NEXT = LEFT > 1 ? LEFT / 2 : 1;
+        if (M < span) {
 #pragma unroll
-            for (int i = 0; i < LEFT / 2; ++i) v[i] = fold<M>(v[i], v[i + LEFT / 2], lane);
+            for (int i = 0; i < NEXT; ++i) v[i] = fold<M>(v[i], v[LEFT > 1 ? i + NEXT : i], lane);
+            reduce_quads<M / 2, M0, NEXT>(v, span, lane);
         } else {
-            v[0] = fold<M>(v[0], v[0], lane);
+            reduce_quads<M / 2, M0, LEFT>(v, span, lane);
         }
-        reduce_quads<M * 2, (LEFT > 1 ? LEFT / 2 : 1), V>(v, span, lane);
     }
 }
 
@@ -103,7 +109,7 @@ __device__ __forceinline__ void reduce_quads(float (&v)[V], int span, int lane) 
 template <int V, int M0>
 __device__ __forceinline__ void reduced_place(int span, int lane, int& idx, int& dup, int& left) {
     idx = 0; dup = 0; left = V;
-    for (int m = M0; m < span; m <<= 1) {
+    for (int m = span / 2; m >= M0; m >>= 1) {
         if (left > 1) {
             left >>= 1;
             idx += (lane & m) ? left : 0;
@@ -121,7 +127,7 @@ template <int NQ, int KQ>
 struct Place {
     static constexpr int CH = 64 / KQ;       // channels of a wave, over its sequences
     static constexpr int NP = 4 * NQ * KQ;   // states, padded
-    int rs, col, d, n0, d4, nd;
+    int rs, col, d, n0, d4, nd, sub;
     bool okc;
 
     __device__ __forceinline__ Place(const ScanParams& p, const ScanPlan& l, int lane, int g, int cblk) {
@@ -131,13 +137,16 @@ struct Place {
         rs = lane / (l.cw * KQ);
         const int c4 = cblk * l.cw + quad * 4, c = c4 + (lane & 3);
         col = rs * l.cw + quad * 4 + (lane & 3);
+        sub = lane & 3;
         nd = per - c4 < 0 ? 0 : per - c4 > 4 ? 4 : per - c4;
         okc = c < per;
         d = g * per + (okc ? c : 0);
         d4 = g * per + (nd ? c4 : 0);
         n0 = (kq * 4 + (lane & 3)) * NQ;
     }
-    __device__ __forceinline__ bool state(const ScanParams& p, int c, int i) const { return c < nd && n0 + i < p.N; }
+    // the channel at index c, and whether there are it and its state i
+    __device__ __forceinline__ int ch(int c) const { return d4 + (c ^ sub); }
+    __device__ __forceinline__ bool state(const ScanParams& p, int c, int i) const { return (c ^ sub) < nd && n0 + i < p.N; }
 };
 
 // log(1 + e^x) and its slope. e^-|x| with the argument's rounding put right,
@@ -174,7 +183,7 @@ __device__ __forceinline__ void load_decay(const ScanParams& p, const Place<NQ, 
     for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-            A2[i][c] = pick(p.A, q.state(p, c, i), (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
+            A2[i][c] = pick(p.A, q.state(p, c, i), (long)q.ch(c) * p.N + q.n0 + i) * LOG2E;
 }
 
 // The lane's states in a (B, D, N) tensor, or zeros, for a wave whose first
@@ -187,8 +196,8 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
     if (!s) return;
     const long b = b0 + q.rs;
     // addresses and masks are formed here, not kept over the loop around
-    int d4 = q.d4, nd = q.nd, n0 = q.n0;
-    asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
+    int d4 = q.d4, nd = q.nd, n0 = q.n0, sub = q.sub;
+    asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0), "+v"(sub));
     nd = b < p.B ? nd : 0;
     if (NQ == 4 && p.N == Place<NQ, KQ>::NP && p.D / p.G % 4 == 0) {
         // Unmasked, so that nothing waits for the loads here. All four channels
@@ -197,7 +206,7 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
         s += ((b < p.B ? b : b0) * p.D + d4) * p.N + n0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const i32x4 v = *(gmem<const any16>)(s + (long)c * p.N);
+            const i32x4 v = *(gmem<const any16>)(s + (long)(c ^ sub) * p.N);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) h[i][c] = __int_as_float(v[i & 3]);
         }
@@ -206,7 +215,7 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             Pack<float> v;
-            v.load(s + (long)c * p.N, c < nd ? p.N - n0 : 0, p.N % 4);
+            v.load(s + (long)(c ^ sub) * p.N, (c ^ sub) < nd ? p.N - n0 : 0, p.N % 4);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) h[i][c] = v.get(i & 3);
         }
@@ -214,15 +223,15 @@ __device__ __forceinline__ void load_states(const ScanParams& p, const Place<NQ,
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, c < nd && n0 + i < p.N, (b * p.D + d4 + c) * p.N + n0 + i);
+            for (int i = 0; i < NQ; ++i) h[i][c] = pick(s, (c ^ sub) < nd && n0 + i < p.N, (b * p.D + d4 + (c ^ sub)) * p.N + n0 + i);
     }
 }
 template <int NQ, int KQ>
 __device__ __forceinline__ void store_states(const ScanParams& p, const Place<NQ, KQ>& q, float* s, long b0,
                                              const f32x4 (&h)[NQ]) {
     const long b = b0 + q.rs;
-    int d4 = q.d4, nd = q.nd, n0 = q.n0;
-    asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0));
+    int d4 = q.d4, nd = q.nd, n0 = q.n0, sub = q.sub;
+    asm volatile("" : "+v"(d4), "+v"(nd), "+v"(n0), "+v"(sub));
     if (b >= p.B) return;
     s += (b * p.D + d4) * p.N + n0;
     if (NQ == 4) {
@@ -231,14 +240,14 @@ __device__ __forceinline__ void store_states(const ScanParams& p, const Place<NQ
             Pack<float> v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v.w[i] = __float_as_int(h[i & (NQ - 1)][c]);
-            v.store(s + (long)c * p.N, c < nd ? p.N - n0 : 0, p.N % 4);
+            v.store(s + (long)(c ^ sub) * p.N, (c ^ sub) < nd ? p.N - n0 : 0, p.N % 4);
         }
     } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
-                if (c < nd && n0 + i < p.N) ((gmem<float>)s)[(long)c * p.N + i] = h[i][c];
+                if ((c ^ sub) < nd && n0 + i < p.N) ((gmem<float>)s)[(long)(c ^ sub) * p.N + i] = h[i][c];
     }
 }
 // the same in the order of a wave's lanes: 16 bytes a lane, NQ rows of them
@@ -556,7 +565,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
                     }
                 }
                 if (MAIN) {
-                    const float s = states_sum<KQ>(acc, lane);
+                    const float s = states_sum<KQ>(acc);
                     tile.u[j][q.col] = from_f32<T>(on ? fmaf(skip, uv, s) : 0.f);
                 }
             }
@@ -598,8 +607,8 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const bool on = q.state(p, c, i);
-        A2[c] = pick(p.A, on, (long)(q.d4 + c) * p.N + q.n0 + i) * LOG2E;
-        start[c] = first ? pick(first, on && b < p.B, (b * p.D + q.d4 + c) * p.N + q.n0 + i) : 0.f;
+        A2[c] = pick(p.A, on, (long)q.ch(c) * p.N + q.n0 + i) * LOG2E;
+        start[c] = first ? pick(first, on && b < p.B, (b * p.D + q.ch(c)) * p.N + q.n0 + i) : 0.f;
     }
     f32x4* seg_h = (f32x4*)p.seg_h + (id * l.nseg * NQ + i) * 64 + lane;
     const float* seg_s = p.seg_s + id * l.nseg * 64 + lane;
@@ -795,7 +804,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
         }
         for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
             const int t0 = ck * SCAN_CH;
-            f32x4 hist[SCAN_CH][NQ];  // before every step; the state after it follows from its decay again
+            f32x4 hist[SCAN_CH][NQ];  // before every step; the one after the last follows from its decay again
 #pragma unroll
             for (int i = 0; i < NQ; ++i) hist[0][i] = next_h[i];
             in.stage(m, ck, cw, tile, tile.dy);
@@ -845,7 +854,8 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                         const float back = a * hist[j][i][c];
                         gs[i][c] = fmaf(Ci, dys[c], gs[i][c]);
                         bc[i] = fmaf(gs[i][c], dus[c], bc[i]);
-                        bc[NQ + i] = fmaf(dys[c], fmaf(dus[c], Bi, back), bc[NQ + i]);
+                        const float h = j + 1 < SCAN_CH ? hist[(j + 1) % SCAN_CH][i][c] : fmaf(dus[c], Bi, back);
+                        bc[NQ + i] = fmaf(dys[c], h, bc[NQ + i]);
                         into[c] = fmaf(gs[i][c], Bi, into[c]);
                         const float gb = gs[i][c] * back;
                         dec[c] = fmaf(gb, A2[c], dec[c]);
@@ -853,14 +863,14 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                         gs[i][c] *= a;
                     }
                 }
-                const float in_n = states_sum<KQ>(into, lane);
-                float dx = fmaf(uv, in_n, states_sum<KQ>(dec, lane) * LN2) * slope;
+                const float in_n = states_sum<KQ>(into);
+                float dx = fmaf(uv, in_n, states_sum<KQ>(dec) * LN2) * slope;
                 dx = on ? dx : 0.f;
                 ddb += dx;
                 dskip = fmaf(dyv, uv, dskip);
                 tile.u[j][q.col] = from_f32<T>(on ? fmaf(skip, dyv, dt * in_n) : 0.f);
                 tile.de[j][q.col] = from_f32<T>(dx);
-                reduce_quads<4 * KQ, 2 * NQ>(bc, cw * KQ, lane);
+                reduce_quads<32, 4 * KQ, 2 * NQ>(bc, cw * KQ, lane);
                 float* o = &tile.dbc[0][j][0][0] + obc;
                 o[0] = bc[0];
                 if (keeps > 1) o[1] = bc[1];
@@ -918,7 +928,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
-                if (q.state(p, c, i)) ws[(long)(q.d4 + c) * N + q.n0 + i] = dA[i][c];
+                if (q.state(p, c, i)) ws[(long)q.ch(c) * N + q.n0 + i] = dA[i][c];
         if (q.okc) {
             ws[(long)D * N + q.d] = dskip;
             ws[(long)D * N + D + q.d] = ddb;
