@@ -7,6 +7,9 @@
 // States, sums and step sizes are f32 throughout; only what is stored as bf16
 // is rounded. Bound by vector arithmetic: an exp (two issue slots) and four
 // more operations per state and step against 6 bytes per channel and step.
+// With 16 states, bf16: 16384 x 2048 in 263 us (a state pass and the main one),
+// forward and backward of 262144 x 7 x 32 in 1155 us: 95 % and 75 % of the
+// issue slots.
 //
 // Layout. Four lanes share four channels: each owns NQ of the states of all
 // four, so a row of B or C costs a lane NQ values for 4 NQ states, and loads
@@ -962,7 +965,8 @@ __launch_bounds__(256) __global__ void scan_bc_reduce_kernel(const float* __rest
 // One new token. Bound by the state, read and written once: 4 states (16
 // bytes) a lane, `gp` lanes a channel, joined by lane exchanges for y. A thread
 // keeps its channel and takes one sequence after another. Every lane reads its
-// own states before it writes them: h_out may be h.
+// own states before it writes them: h_out may be h. 256 x 4096 x 16: 28.6 us,
+// 4.9 TB/s.
 template <typename T>
 __launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
