@@ -9,8 +9,9 @@
 // the registers of TPR threads (8 channels a chunk, VPT chunks a thread), both
 // norms are taken from there in f32, and h feeds the second norm unrounded.
 // 8192 x 2560 with an f32 residual: 57 us forward, 92 us backward (4.4 and 4.1
-// TB/s); 1835008 x 32 with a gate: 193 us both, at a copy's rate. The backward
-// of more than 8192 channels (four chunks a thread) spills registers.
+// TB/s); 1835008 x 32 with a gate: 193 us both, at a copy's rate. Both passes of
+// wide rows, f32 residual: 4096 x 5120 135 us, 2048 x 8192 160 us, 1024 x 16384
+// 332 us (4.6, 3.1, 1.5 TB/s): the backward of four chunks a thread spills.
 #include "seq.hpp"
 
 namespace {
@@ -99,6 +100,7 @@ struct WeightsBack {
                 v[4 + j] = b[j];
             }
         } else {
+            if (VPT > 2) asm volatile("" : "+v"(c));  // not kept between the walks
             param8(from, c, D, v);
         }
     }
@@ -107,8 +109,9 @@ struct WeightsBack {
 // A thread keeps its columns and takes one row after another; with one chunk a
 // thread a row's loads are in flight while the row before is worked on.
 // WHOLE: every piece is whole or absent, and there is no code for a partial one.
-template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
-__launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, int tpr) {
+// MOST: threads of a block; more than 512 leave a thread fewer registers.
+template <typename T, typename TR, int VPT, bool RES, bool WHOLE, int MOST>
+__launch_bounds__(MOST) __global__ void block_norm_fwd_kernel(BlockNormParams p, int tpr) {
     __shared__ float lds[32];
     int slot = 0;
     const int rpb = blockDim.x / tpr, lane = threadIdx.x % tpr;
@@ -205,8 +208,8 @@ __launch_bounds__(512) __global__ void block_norm_fwd_kernel(BlockNormParams p, 
 //   dp0 = inv1 (q - n1 mean(q n1));  dx, dgate by the product and silu'
 // Column gradients stay in registers over a thread's rows, are joined in LDS
 // over the block's row groups and written once per block.
-template <typename T, typename TR, int VPT, bool RES, bool GATE, bool WHOLE>
-__launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
+template <typename T, typename TR, int VPT, bool RES, bool GATE, bool WHOLE, int MOST>
+__launch_bounds__(MOST) __global__ void block_norm_bwd_kernel(BlockNormParams p, int tpr) {
     // the weights, then [rpb][VPT * tpr * SEQ_CH] to join the column gradients
     extern __shared__ __attribute__((aligned(16))) float dyn[];
     __shared__ float lds[32];
@@ -242,79 +245,107 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
     if (AHEAD) read(r);
     for (long k = 0; k < rounds; ++k, r += stride) {
         const bool live = r < p.R;
-        // v: the normed row without its weight; d: the gradient on its way down
-        float v[VPT][SEQ_CH], d[VPT][SEQ_CH], hv[VPT][SEQ_CH], t[VPT][SEQ_CH];
-        Raw8<T> xk[VPT], gk[VPT];
         if (!AHEAD) read(r);
         const float inv1 = i1, inv2 = i2;
+        Raw8<T> xk[VPT], gk[VPT], yk[VPT];
+        Raw8<TR> rk[VPT], hk[VPT];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             xk[i] = xr[i];
             gk[i] = gr[i];
-#pragma unroll
-            for (int j = 0; j < SEQ_CH; ++j) {
-                const float g = GATE ? gr[i].get(j) : 0.f;
-                const float sg = GATE ? g * fast_sigmoid(g) : 1.f;
-                v[i][j] = xr[i].get(j) * sg * inv1;
-                d[i][j] = RES ? hr[i].get(j) : yr[i].get(j);
-                if (RES && p.pre) {
-                    hv[i][j] = rr[i].get(j);
-                    t[i][j] = yr[i].get(j);
-                }
-            }
+            yk[i] = yr[i];
+            rk[i] = rr[i];
+            hk[i] = hr[i];
         }
         if (AHEAD && k + 1 < rounds) read(r + stride);
+        // With four chunks the row waits as it came, and what follows from it is
+        // formed anew by each of the three walks over it: kept it would spill.
+        auto anew = [&](auto& raw) {
+            if (VPT > 2) raw.fresh();
+        };
+        auto apart = [&] {  // one chunk's weights at a time
+            if (VPT > 2) __builtin_amdgcn_sched_barrier(0);
+        };
+        // the normed row without its weight; the one after the residual, y / pre
+        auto normed = [&](int i, float (&v)[SEQ_CH]) {
+#pragma unroll
+            for (int j = 0; j < SEQ_CH; ++j) {
+                const float g = GATE ? gk[i].get(j) : 0.f;
+                v[j] = xk[i].get(j) * (GATE ? g * fast_sigmoid(g) : 1.f) * inv1;
+            }
+        };
+        auto stream = [&](int i, const float (&v)[SEQ_CH], const float (&w1)[SEQ_CH], const float (&ws)[SEQ_CH],
+                          float (&h)[SEQ_CH]) {
+#pragma unroll
+            for (int j = 0; j < SEQ_CH; ++j) h[j] = fmaf(ws[j] * w1[j], v[j], rk[i].get(j)) * inv2;
+        };
+        float m = 0.f;
         if (RES && p.pre) {
             float sum2 = 0.f;
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
                 const int c = (i * tpr + lane) * SEQ_CH;
-                float w1[SEQ_CH], ws[SEQ_CH], w2[SEQ_CH];
+                float w1[SEQ_CH], ws[SEQ_CH], w2[SEQ_CH], v[SEQ_CH], h[SEQ_CH];
                 wt.template get<0>(p.post, c, p.D, w1);
                 wt.template get<1>(p.scale, c, p.D, ws);
                 wt.template get<2>(p.pre, c, p.D, w2);
+                normed(i, v);
+                stream(i, v, w1, ws, h);
 #pragma unroll
                 for (int j = 0; j < SEQ_CH; ++j) {
-                    hv[i][j] = fmaf(ws[j] * w1[j], v[i][j], hv[i][j]) * inv2;  // y / pre
-                    dpre[i][j] = fmaf(t[i][j], hv[i][j], dpre[i][j]);
-                    t[i][j] *= w2[j];
-                    sum2 = fmaf(t[i][j], hv[i][j], sum2);
-                    d[i][j] = fmaf(inv2, t[i][j], d[i][j]);
+                    const float t = yk[i].get(j);
+                    dpre[i][j] = fmaf(t, h[j], dpre[i][j]);
+                    sum2 = fmaf(t * w2[j], h[j], sum2);
                 }
+                apart();
             }
-            const float m = row_sum(sum2, tpr, lds, slot) * rd * inv2;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int j = 0; j < SEQ_CH; ++j) d[i][j] = fmaf(-m, hv[i][j], d[i][j]);
+            m = row_sum(sum2, tpr, lds, slot) * rd * inv2;
         }
-        float sum1 = 0.f;
+        float sum1 = 0.f, d[VPT][SEQ_CH];  // d: the gradient on its way down
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            if (RES && live && c < p.D) store8<TR>((TR*)p.dres + r * p.D + c, p.D - c, width, d[i]);
-            float w1[SEQ_CH], ws[SEQ_CH];
+            float w1[SEQ_CH], ws[SEQ_CH], v[SEQ_CH];
+            anew(xk[i]);
+            if (GATE) anew(gk[i]);
             wt.template get<0>(p.post, c, p.D, w1);
             if (RES) wt.template get<1>(p.scale, c, p.D, ws);
+            normed(i, v);
+#pragma unroll
+            for (int j = 0; j < SEQ_CH; ++j) d[i][j] = RES ? hk[i].get(j) : yk[i].get(j);
+            if (RES && p.pre) {
+                float w2[SEQ_CH], h[SEQ_CH];
+                anew(rk[i]);
+                anew(yk[i]);
+                wt.template get<2>(p.pre, c, p.D, w2);
+                stream(i, v, w1, ws, h);
+#pragma unroll
+                for (int j = 0; j < SEQ_CH; ++j) d[i][j] = fmaf(-m, h[j], fmaf(inv2, yk[i].get(j) * w2[j], d[i][j]));
+            }
+            if (RES && live && c < p.D) store8<TR>((TR*)p.dres + r * p.D + c, p.D - c, width, d[i]);
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
                 if (RES) {
-                    dscale[i][j] = fmaf(d[i][j], v[i][j] * w1[j], dscale[i][j]);
+                    dscale[i][j] = fmaf(d[i][j], v[j] * w1[j], dscale[i][j]);
                     d[i][j] *= ws[j];
                 }
-                dpost[i][j] = fmaf(d[i][j], v[i][j], dpost[i][j]);
+                dpost[i][j] = fmaf(d[i][j], v[j], dpost[i][j]);
                 d[i][j] *= w1[j];
-                sum1 = fmaf(d[i][j], v[i][j], sum1);
+                sum1 = fmaf(d[i][j], v[j], sum1);
             }
+            apart();
         }
         const float m1 = p.post ? row_sum(sum1, tpr, lds, slot) * rd : 0.f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = (i * tpr + lane) * SEQ_CH;
-            float o[SEQ_CH], og[SEQ_CH];
+            float v[SEQ_CH], o[SEQ_CH], og[SEQ_CH];
+            anew(xk[i]);
+            if (GATE) anew(gk[i]);
+            normed(i, v);
 #pragma unroll
             for (int j = 0; j < SEQ_CH; ++j) {
-                const float dp = inv1 * fmaf(-m1, v[i][j], d[i][j]);
+                const float dp = inv1 * fmaf(-m1, v[j], d[i][j]);
                 o[j] = dp;
                 if (GATE) {
                     const float g = gk[i].get(j), sg = fast_sigmoid(g), si = g * sg;
@@ -326,6 +357,7 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
                 store8<T>((T*)p.dx + r * p.D + c, p.D - c, width, o);
                 if (GATE) store8<T>((T*)p.dgate + r * p.D + c, p.D - c, width, og);
             }
+            apart();
         }
     }
     // column gradients of the weights there are, in the order post | scale | pre
@@ -362,11 +394,12 @@ __launch_bounds__(512) __global__ void block_norm_bwd_kernel(BlockNormParams p, 
 }
 
 // Threads a row, chunks a thread: a part of a wave while that holds the row,
-// then whole waves with one chunk a thread (to D = 4096), two, four. One chunk
-// leaves no thread of a row idle and registers for the next row's loads.
+// then whole waves with one chunk a thread (to D = 6144), two, four. One chunk
+// leaves no thread of a row idle and registers for the next row's loads: 4096 x
+// 5120 takes 135 us with one on 640 threads, 231 us with two on 320.
 inline void row_shape(long D, int* tpr, int* vpt) {
     const long chunks = (D + SEQ_CH - 1) / SEQ_CH;
-    *vpt = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
+    *vpt = chunks <= 768 ? 1 : chunks <= 1024 ? 2 : 4;
     *tpr = chunks <= 64 ? pow2_ceil(chunks) : (int)((chunks + 64 * *vpt - 1) / (64 * *vpt)) * 64;
 }
 
@@ -384,26 +417,26 @@ inline long row_blocks(long R, int tpr, int waves) {
 struct NormFwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
+    template <typename T, typename TR, int VPT, bool RES, bool WHOLE, int MOST>
     void operator()(int tpr) const {
-        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES, WHOLE>), dim3((unsigned)row_blocks(p.R, tpr, 20)),
-                           dim3(block_threads(tpr)), 0, s, p, tpr);
+        hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES, WHOLE, MOST>),
+                           dim3((unsigned)row_blocks(p.R, tpr, 20)), dim3(block_threads(tpr)), 0, s, p, tpr);
     }
 };
 
 struct NormBwd {
     const BlockNormParams& p;
     hipStream_t s;
-    template <typename T, typename TR, int VPT, bool RES, bool WHOLE>
+    template <typename T, typename TR, int VPT, bool RES, bool WHOLE, int MOST>
     void operator()(int tpr) const {
         const int block = block_threads(tpr);
         const size_t smem = (size_t)block * SEQ_CH * sizeof(float) * (VPT > 1 ? VPT : RES ? 3 : 1);
         if (p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, true, WHOLE>), dim3(p.slots), dim3(block), smem,
-                               s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, true, WHOLE, MOST>), dim3(p.slots), dim3(block),
+                               smem, s, p, tpr);
         if (!p.gate)
-            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, false, WHOLE>), dim3(p.slots), dim3(block), smem,
-                               s, p, tpr);
+            hipLaunchKernelGGL((block_norm_bwd_kernel<T, TR, VPT, RES, false, WHOLE, MOST>), dim3(p.slots), dim3(block),
+                               smem, s, p, tpr);
     }
 };
 
@@ -411,10 +444,11 @@ template <typename T, typename TR, bool RES, typename F>
 void by_shape(const BlockNormParams& p, F f) {
     int tpr, vpt;
     row_shape(p.D, &tpr, &vpt);
-    if (vpt == 1 && p.D % SEQ_CH == 0) f.template operator()<T, TR, 1, RES, true>(tpr);
-    else if (vpt == 1) f.template operator()<T, TR, 1, RES, false>(tpr);
-    else if (vpt == 2) f.template operator()<T, TR, 2, RES, false>(tpr);
-    else f.template operator()<T, TR, 4, RES, false>(tpr);
+    if (tpr > 512) f.template operator()<T, TR, 1, RES, false, 768>(tpr);
+    else if (vpt == 1 && p.D % SEQ_CH == 0) f.template operator()<T, TR, 1, RES, true, 512>(tpr);
+    else if (vpt == 1) f.template operator()<T, TR, 1, RES, false, 512>(tpr);
+    else if (vpt == 2) f.template operator()<T, TR, 2, RES, false, 512>(tpr);
+    else f.template operator()<T, TR, 4, RES, false, 512>(tpr);
 }
 
 template <typename F>

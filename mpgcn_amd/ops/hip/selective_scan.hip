@@ -1092,8 +1092,8 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32, int back) {
     // Segments of at least 4 chunks where that brings the waves towards four per
     // SIMD, in the backward the two its registers allow: they cost a second pass
     // over the recurrence, so fewer than 3 do not pay. Measured, forward and
-    // backward of 8192 x 1536: 412 us against 443 with four in the backward too;
-    // prompt of 16384 x 2048: 297 us against 317 with two.
+    // backward of 8192 x 1536: 378 us against 397 with four in the backward too;
+    // prompt of 16384 x 2048: 262 us against 290 with two.
     const long tasks = l.groups * p.G * l.cb, same = (long)p.G * l.cb;
     long nseg = tasks ? (back ? 2048 : 4096) / tasks : 1;
     // (two chunks where even so a quarter of the card would have no wave)

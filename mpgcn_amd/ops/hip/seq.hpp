@@ -90,6 +90,11 @@ struct Raw8 {
     static constexpr int E = Pack<T>::E;
     Pack<T> w[SEQ_CH / E];
     __device__ __forceinline__ float get(int j) const { return w[j / E].get(j % E); }
+    // what was formed from it is forgotten
+    __device__ __forceinline__ void fresh() {
+#pragma unroll
+        for (int i = 0; i < SEQ_CH / E; ++i) asm volatile("" : "+v"(w[i].w));
+    }
     __device__ __forceinline__ void load(const T* p, int n, int D) {
 #pragma unroll
         for (int i = 0; i < SEQ_CH / E; ++i) w[i].load(p + i * E, n - i * E, D % E);

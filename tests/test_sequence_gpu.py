@@ -264,7 +264,7 @@ def test_lengths_are_held_to_the_range():
 @pytest.mark.parametrize("dtype,res", [(BF, None), (F, None), (BF, BF), (BF, F), (F, F), (F, BF)])
 @pytest.mark.parametrize("gate", [False, True])
 @pytest.mark.parametrize("R,D", [(1, 1), (3, 8), (70, 32), (5, 33), (9, 512), (4, 520), (3, 1025), (2, 2560),
-                                 (2, 8200)])
+                                 (2, 4096), (3, 4100), (300, 5128), (2, 8200), (2, 16384)])
 def test_norm(dtype, res, gate, R, D):
     g = gen(R * D)
     modes = [dict(post=True)] if res is None else [dict(post=True, scale=True, pre=True), dict(pre=True),
