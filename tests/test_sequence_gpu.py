@@ -616,3 +616,70 @@ def test_only_the_last_state_has_a_gradient():
             oracle.within(got[name], *ref[name], r + more, name)
         for name in ("C", "skip"):
             assert got[name] is None or not got[name].any(), name
+
+
+def test_broadcast_inputs_and_gradients():
+    """Inputs that repeat (strides of 0), one tensor in two places, an expanded
+    gradient: what autograd adds up is the sum over the repeats."""
+    g = gen(140)
+    t, _ = scan_case(141, F, 1, 1, 24, 16, 1, False, None)
+    u, delta = rn(g, 3, 12, 24).requires_grad_(), rn(g, 1, 12, 24).requires_grad_()
+    Bm, s = rn(g, 3, 1, 1, 16).requires_grad_(), rn(g, 1, 24, 16).requires_grad_()
+    full = lambda: dict(u=u, delta=delta.expand(3, 12, 24), A=t["A"], B=Bm.expand(3, 12, 1, 16),
+                        C=Bm.expand(3, 12, 1, 16), state=s.expand(3, 24, 16))
+    y = ops.selective_scan(**full(), delta_softplus=True)
+    got = torch.autograd.grad(y.sum(), [u, delta, Bm, s])
+    clean = {k: v.detach().clone().requires_grad_() for k, v in full().items()}
+    y2 = ops.selective_scan(**clean, delta_softplus=True)
+    d = dict(zip(clean, torch.autograd.grad(y2, list(clean.values()), torch.ones_like(y2))))
+    assert torch.equal(y, y2) and torch.equal(got[0], d["u"])
+    both = (d["B"].double() + d["C"].double()).sum(1, keepdim=True)
+    for a, b, n in ((got[1], d["delta"].double().sum(0, keepdim=True), 3),
+                    (got[2], both, 24), (got[3], d["state"].double().sum(0, keepdim=True), 3)):
+        # n - 1 roundings of sums no larger than the sum of magnitudes, taken as n times the largest term
+        assert float((a.double() - b).abs().max()) <= n * n * 2.0 ** -24 * max(float(v.abs().max()) for v in d.values())
+    row = rn(g, 24).requires_grad_()
+    w = rn(g, 24, 4)
+    x = row.expand(2, 9, 24)
+    assert torch.equal(ops.short_conv(x, w), ops.short_conv(x.contiguous(), w))
+    y = ops.norm_gate_residual(x, gate=x, post_weight=w[:, 0])
+    assert torch.equal(y, ops.norm_gate_residual(x.contiguous(), gate=x.contiguous(), post_weight=w[:, 0]))
+    assert torch.equal(torch.autograd.grad(y.sum(), row)[0] != 0, torch.ones(24, dtype=torch.bool, device=DEV))
+
+
+def test_inference_mode():
+    t, n = scan_case(142, BF, 2, 20, 32, 16, 1, True, torch.int32)
+    x, w = t["u"], rn(gen(143), 32, 4)
+    want = (ops.short_conv(x, w), ops.selective_scan(**t, lengths=n), ops.norm_gate_residual(x, post_weight=w[:, 0]))
+    with torch.inference_mode():
+        got = (ops.short_conv(x, w), ops.selective_scan(**t, lengths=n),
+               ops.norm_gate_residual(x, post_weight=w[:, 0]))
+        state = torch.zeros(2, 3, 32, device=DEV, dtype=BF)
+        y, same = ops.short_conv_step(x[:, 0], state, w)
+    assert same is state and torch.equal(y, want[0][:, 0])
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
+
+
+def test_two_streams_at_once():
+    """The same calls side by side on two streams give what they give alone."""
+    t, _ = scan_case(144, BF, 1, 4000, 96, 16, 1, False, None)
+    leaves = {k: v.requires_grad_() for k, v in t.items() if v is not None}
+    dy = rn(gen(145), 1, 4000, 96, dtype=BF)
+
+    def run():
+        y = ops.selective_scan(**t, delta_softplus=True)
+        return [y, *torch.autograd.grad(y, list(leaves.values()), dy)]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(run())
+    torch.cuda.synchronize()
+    for o in outs:
+        for a, b in zip(o, want):
+            assert torch.equal(a, b)
