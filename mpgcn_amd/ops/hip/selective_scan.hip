@@ -1096,8 +1096,9 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32, int back) {
     // prompt of 16384 x 2048: 262 us against 290 with two.
     const long tasks = l.groups * p.G * l.cb, same = (long)p.G * l.cb;
     long nseg = tasks ? (back ? 2048 : 4096) / tasks : 1;
-    // (two chunks where even so a quarter of the card would have no wave)
-    const long least = tasks * (l.chunks / 4) < 1024 ? 2 : 4;
+    // Two chunks where four would leave less than two waves a SIMD: 2 x 1024 x
+    // 1536 forward and backward 150 us against 154.
+    const long least = tasks * (l.chunks / 4) < 2048 ? 2 : 4;
     if (nseg > l.chunks / least) nseg = l.chunks / least;
     if (nseg < 3) nseg = 1;
     l.seg_chunks = (int)(l.chunks ? (l.chunks + nseg - 1) / nseg : 1);
