@@ -8,8 +8,8 @@
 // is rounded. Bound by vector arithmetic: an exp (two issue slots) and four
 // more operations per state and step against 6 bytes per channel and step.
 // With 16 states, bf16: 16384 x 2048 in 263 us (a state pass and the main one),
-// forward and backward of 262144 x 7 x 32 in 1155 us: 95 % and 75 % of the
-// issue slots.
+// forward and backward of 262144 x 7 x 32 in 1155 us: the vector pipes are busy
+// throughout the one and for 93 % of the other.
 //
 // Layout. Four lanes share four channels: each owns NQ of the states of all
 // four, so a row of B or C costs a lane NQ values for 4 NQ states, and loads
