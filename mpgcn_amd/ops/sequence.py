@@ -348,7 +348,8 @@ def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=N
     x, gate: (..., D) of one type, D up to 16384; residual: (..., D) bf16 or f32,
     which need not be x's type; post_weight, scale, pre_weight: (D,). Parts left
     out are skipped: one norm at least, and scale and pre_weight only with a
-    residual. h feeds the second norm unrounded. Returns p without a residual,
+    residual. h feeds the second norm unrounded; squares are summed in f32, so
+    values past 1e18 overflow them. Returns p without a residual,
     h without pre_weight, else (y, h): p and y of x's type, h of the residual's.
     """
     if _on_gpu(x):
