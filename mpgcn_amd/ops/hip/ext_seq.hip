@@ -94,10 +94,9 @@ ShortConvParams conv_params(const Tensor& x, const Tensor& w, const Opt& bias, c
     return p;
 }
 
-std::vector<Tensor> short_conv_fwd(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state) {
+// p: conv_params of these arguments
+std::vector<Tensor> short_conv_fwd(ShortConvParams p, const Tensor& x, long K, bool want_state) {
     at::DeviceGuard guard(x.device());
-    auto p = conv_params(x, w, bias, s0, lens, silu);
-    const long K = w.size(1);
     auto y = torch::empty({p.B, p.L, p.D}, x.options());
     auto s1 = want_state ? torch::empty({p.B, K - 1, p.D}, x.options()) : Tensor();
     if (p.B && p.D && (p.L || want_state)) {
@@ -138,8 +137,7 @@ std::vector<Tensor> short_conv_bwd(Tensor dy, Opt ds1, Tensor x, Tensor w, Opt b
     return {dx, sums.narrow(0, 0, D * K).view({D, K}), sums.narrow(0, D * K, D), ds0};
 }
 
-Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt bias, bool silu) {
-    at::DeviceGuard guard(x.device());
+void check_conv_step(const Tensor& x, const Tensor& state, const Tensor& state_out, const Tensor& w, const Opt& bias) {
     check_main(x, "x");
     TORCH_CHECK(x.dim() == 2, "x must be (B, D)");
     const long B = x.size(0), D = x.size(1);
@@ -150,6 +148,13 @@ Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt b
     check_f32(bias, x, {D}, "bias");
     check_like(state, x, {B, K - 1, D}, "state");
     check_like(state_out, x, {B, K - 1, D}, "state_out");
+}
+
+// after check_conv_step
+Tensor run_conv_step(const Tensor& x, const Tensor& state, const Tensor& state_out, const Tensor& w, const Opt& bias,
+                     bool silu) {
+    at::DeviceGuard guard(x.device());
+    const long B = x.size(0), D = x.size(1), K = w.size(1);
     auto y = torch::empty({B, D}, x.options());
     if (B && D) {
         short_conv_step_launch(x.data_ptr(), x.stride(0), state.data_ptr(), state_out.data_ptr(),
@@ -158,6 +163,11 @@ Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt b
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return y;
+}
+
+Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt bias, bool silu) {
+    check_conv_step(x, state, state_out, w, bias);
+    return run_conv_step(x, state, state_out, w, bias, silu);
 }
 
 // ---- selective scan ---------------------------------------------------------
@@ -205,11 +215,9 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     return p;
 }
 
-// {y, final state, states entering every chunk or undefined}
-std::vector<Tensor> selective_scan_fwd(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias,
-                                       Opt h0, Opt lens, bool softplus, bool want_state, bool train) {
+// {y, final state, states entering every chunk or undefined}; p: scan_params of these arguments
+std::vector<Tensor> selective_scan_fwd(ScanParams p, const Tensor& u, bool want_state, bool train) {
     at::DeviceGuard guard(u.device());
-    auto p = scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus);
     auto y = torch::empty({p.B, p.L, p.D}, u.options());
     auto h1 = want_state ? empty_f32(u, {p.B, p.D, p.N}) : Tensor();
     Tensor ck, seg_h, seg_s;
@@ -288,9 +296,9 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
     return split(sums);
 }
 
-Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state, Tensor state_out,
-                           Opt skip, Opt dbias, bool softplus) {
-    at::DeviceGuard guard(u.device());
+ScanStepParams scan_step_params(const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                                const Tensor& state, const Tensor& state_out, const Opt& skip, const Opt& dbias,
+                                bool softplus) {
     check_main(u, "u");
     TORCH_CHECK(u.dim() == 2, "u must be (B, D)");
     const long B = u.size(0), D = u.size(1);
@@ -309,21 +317,33 @@ Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor C
     check_f32(dbias, u, {D}, "delta_bias");
     check_f32(state, u, {B, D, N}, "state");
     check_f32(state_out, u, {B, D, N}, "state_out");
-    auto y = torch::empty({B, D}, u.options());
-    if (B && D) {
-        ScanStepParams p{};
-        p.u = u.data_ptr(); p.delta = delta.data_ptr(); p.Bm = Bm.data_ptr(); p.Cm = Cm.data_ptr();
-        p.A = A.data_ptr<float>(); p.skip = fptr(skip); p.dbias = fptr(dbias);
-        p.h = state.data_ptr<float>(); p.h_out = state_out.data_ptr<float>(); p.y = y.data_ptr();
-        p.u_b = u.stride(0); p.d_b = delta.stride(0);
-        p.B_b = Bm.stride(0); p.B_g = grouped ? Bm.stride(1) : 0;
-        p.C_b = Cm.stride(0); p.C_g = grouped ? Cm.stride(1) : 0;
-        p.B = (int)B; p.D = (int)D; p.N = (int)N; p.G = (int)G;
-        p.softplus = softplus ? 1 : 0;
+    ScanStepParams p{};
+    p.u = u.data_ptr(); p.delta = delta.data_ptr(); p.Bm = Bm.data_ptr(); p.Cm = Cm.data_ptr();
+    p.A = A.data_ptr<float>(); p.skip = fptr(skip); p.dbias = fptr(dbias);
+    p.h = state.data_ptr<float>(); p.h_out = state_out.data_ptr<float>();
+    p.u_b = u.stride(0); p.d_b = delta.stride(0);
+    p.B_b = Bm.stride(0); p.B_g = grouped ? Bm.stride(1) : 0;
+    p.C_b = Cm.stride(0); p.C_g = grouped ? Cm.stride(1) : 0;
+    p.B = (int)B; p.D = (int)D; p.N = (int)N; p.G = (int)G;
+    p.softplus = softplus ? 1 : 0;
+    return p;
+}
+
+// p: scan_step_params of u and the rest
+Tensor run_scan_step(ScanStepParams p, const Tensor& u) {
+    at::DeviceGuard guard(u.device());
+    auto y = torch::empty({p.B, p.D}, u.options());
+    if (p.B && p.D) {
+        p.y = y.data_ptr();
         scan_step_launch(p, f32(u), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return y;
+}
+
+Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state, Tensor state_out,
+                           Opt skip, Opt dbias, bool softplus) {
+    return run_scan_step(scan_step_params(u, delta, A, Bm, Cm, state, state_out, skip, dbias, softplus), u);
 }
 
 // ---- norms around a block ---------------------------------------------------
@@ -362,16 +382,14 @@ BlockNormParams norm_params(const Tensor& x, const Opt& gate, const Opt& post, c
     return p;
 }
 
-// {y, h, inv1, inv2}, those that there are
-std::vector<Tensor> block_norm_fwd(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps,
-                                   bool train) {
+// {y, h, inv1, inv2}, those that there are; p: norm_params of these arguments
+std::vector<Tensor> block_norm_fwd(BlockNormParams p, const Tensor& x, const Opt& res, bool train) {
     at::DeviceGuard guard(x.device());
-    auto p = norm_params(x, gate, post, res, scale, pre, eps);
     const long R = p.R, D = p.D;
-    auto y = has(pre) || !has(res) ? torch::empty({R, D}, x.options()) : Tensor();
+    auto y = p.pre || !has(res) ? torch::empty({R, D}, x.options()) : Tensor();
     auto h = has(res) ? torch::empty({R, D}, res->options()) : Tensor();
-    auto i1 = train && has(post) ? empty_f32(x, {R}) : Tensor();
-    auto i2 = train && has(pre) ? empty_f32(x, {R}) : Tensor();
+    auto i1 = train && p.post ? empty_f32(x, {R}) : Tensor();
+    auto i2 = train && p.pre ? empty_f32(x, {R}) : Tensor();
     if (R && D) {
         p.y = y.defined() ? y.data_ptr() : nullptr;
         p.h = h.defined() ? h.data_ptr() : nullptr;
@@ -453,7 +471,7 @@ struct ShortConvFn : Function<ShortConvFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& bias, const Opt& s0,
                                  const Opt& lens, bool silu, bool want_state) {
         ctx->set_materialize_grads(false);
-        auto r = short_conv_fwd(x, w, bias, s0, lens, silu, want_state);
+        auto r = short_conv_fwd(conv_params(x, w, bias, s0, lens, silu), x, w.size(1), want_state);
         ctx->save_for_backward({x, w, val(bias), val(s0), val(lens)});
         ctx->saved_data["silu"] = silu;
         ctx->saved_data["state"] = has(s0) && s0->requires_grad();
@@ -482,7 +500,7 @@ struct SelectiveScanFn : Function<SelectiveScanFn> {
                                  const Tensor& Bm, const Tensor& Cm, const Opt& skip, const Opt& dbias, const Opt& h0,
                                  const Opt& lens, bool softplus, bool want_state) {
         ctx->set_materialize_grads(false);
-        auto r = selective_scan_fwd(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus, want_state, true);
+        auto r = selective_scan_fwd(scan_params(u, delta, A, Bm, Cm, skip, dbias, h0, lens, softplus), u, want_state, true);
         ctx->save_for_backward({u, delta, A, Bm, Cm, val(skip), val(dbias), val(h0), val(lens), r[2]});
         ctx->saved_data["softplus"] = softplus;
         ctx->saved_data["state"] = has(h0) && h0->requires_grad();
@@ -509,7 +527,7 @@ struct BlockNormFn : Function<BlockNormFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Opt& gate, const Opt& post, const Opt& res,
                                  const Opt& scale, const Opt& pre, double eps) {
         ctx->set_materialize_grads(false);
-        auto r = block_norm_fwd(x, gate, post, res, scale, pre, eps, true);
+        auto r = block_norm_fwd(norm_params(x, gate, post, res, scale, pre, eps), x, res, true);
         ctx->save_for_backward({x, val(gate), val(post), val(res), val(scale), val(pre), r[2], r[3]});
         ctx->saved_data["eps"] = eps;
         if (!r[1].defined()) return {r[0]};
@@ -553,13 +571,20 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 }
 const Tensor* tp(const Opt& t) { return t.has_value() ? &*t : nullptr; }
 
+// Whether the checks pass. They alone say that a call needs preparation; an
+// error of the call itself (memory, a launch) is the caller's to see, since
+// running it again could advance a state twice.
 template <typename F>
-py::object direct(bool prepared, F f) {
+bool fits(bool prepared, F checks) {
+    if (prepared) {
+        checks();
+        return true;
+    }
     try {
-        return f();
+        checks();
+        return true;
     } catch (const c10::Error&) {
-        if (prepared) throw;
-        return py::none();
+        return false;
     }
 }
 
@@ -575,18 +600,20 @@ py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, boo
     if (!x.is_cuda()) return py::none();
     const bool train = wants_grad({&x, &w, tp(bias), tp(s0)});
     if (train && !prepared && capturing()) return py::none();
-    return direct(prepared, [&]() -> py::object {
-        if (train) return one_or_pair(ShortConvFn::apply(x, w, bias, s0, lens, silu, want_state));
-        auto r = short_conv_fwd(x, w, bias, s0, lens, silu, want_state);
-        if (!want_state) r.pop_back();
-        return one_or_pair(r);
-    });
+    ShortConvParams p;
+    if (!fits(prepared, [&] { p = conv_params(x, w, bias, s0, lens, silu); })) return py::none();
+    if (train) return one_or_pair(ShortConvFn::apply(x, w, bias, s0, lens, silu, want_state));
+    auto r = short_conv_fwd(p, x, w.size(1), want_state);
+    if (!want_state) r.pop_back();
+    return one_or_pair(r);
 }
 
 py::object short_conv_step_direct(Tensor x, Tensor state, Opt state_out, Tensor w, Opt bias, bool silu) {
     const Tensor out = has(state_out) ? *state_out : state;
-    if (!x.is_cuda() || wants_grad({&x, &state, &out, &w, tp(bias)}) || !apart(state, out)) return py::none();
-    return direct(false, [&] { return py::make_tuple(short_conv_step(x, state, out, w, bias, silu), out); });
+    if (!x.is_cuda() || wants_grad({&x, &state, &out, &w, tp(bias)}) || !apart(state, out) ||
+        !fits(false, [&] { check_conv_step(x, state, out, w, bias); }))
+        return py::none();
+    return py::make_tuple(run_conv_step(x, state, out, w, bias, silu), out);
 }
 
 py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias, Opt h0,
@@ -594,14 +621,15 @@ py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Te
     if (!u.is_cuda()) return py::none();
     const bool train = wants_grad({&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)});
     if (train && !prepared && capturing()) return py::none();
-    return direct(prepared, [&]() -> py::object {
-        const Tensor B4 = Bm.dim() == 3 ? Bm.unsqueeze(2) : Bm, C4 = Cm.dim() == 3 ? Cm.unsqueeze(2) : Cm;
-        if (train)
-            return one_or_pair(SelectiveScanFn::apply(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus, want_state));
-        auto r = selective_scan_fwd(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus, want_state, false);
-        r.resize(want_state ? 2 : 1);
-        return one_or_pair(r);
-    });
+    const Tensor B4 = Bm.dim() == 3 ? Bm.unsqueeze(2) : Bm, C4 = Cm.dim() == 3 ? Cm.unsqueeze(2) : Cm;
+    ScanParams p;
+    if (!fits(prepared, [&] { p = scan_params(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus); }))
+        return py::none();
+    if (train)
+        return one_or_pair(SelectiveScanFn::apply(u, delta, A, B4, C4, skip, dbias, h0, lens, softplus, want_state));
+    auto r = selective_scan_fwd(p, u, want_state, false);
+    r.resize(want_state ? 2 : 1);
+    return one_or_pair(r);
 }
 
 py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state,
@@ -609,33 +637,39 @@ py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor B
     const Tensor out = has(state_out) ? *state_out : state;
     if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, &state, &out, tp(skip), tp(dbias)}) || !apart(state, out))
         return py::none();
-    return direct(false, [&] {
-        return py::make_tuple(selective_scan_step(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus), out);
-    });
+    ScanStepParams p;
+    if (!fits(false, [&] { p = scan_step_params(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus); }))
+        return py::none();
+    return py::make_tuple(run_scan_step(p, u), out);
 }
 
 py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps, bool prepared) {
     if (!x.is_cuda() || x.dim() < 1 || !(eps >= FLT_MIN)) return py::none();
     const bool train = wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)});
     if (train && !prepared && capturing()) return py::none();
-    return direct(prepared, [&]() -> py::object {
-        const auto shape = x.sizes().vec();
-        const bool flat = x.dim() == 2;
-        TORCH_CHECK(shape.back() >= 1 && (!has(gate) || gate->sizes() == x.sizes()) &&
-                    (!has(res) || res->sizes() == x.sizes()), "gate and residual must have x's shape");
-        auto rows = [&](const Tensor& t) { return flat ? t : t.reshape({-1, shape.back()}); };
-        auto opt_rows = [&](const Opt& t) { return has(t) ? Opt(rows(*t)) : Opt(); };
-        variable_list r;
-        if (train) {
-            r = BlockNormFn::apply(rows(x), opt_rows(gate), post, opt_rows(res), scale, pre, eps);
-        } else {
-            for (auto& t : block_norm_fwd(rows(x), opt_rows(gate), post, opt_rows(res), scale, pre, eps, false))
-                if (t.defined()) r.push_back(t);
-        }
-        if (!flat)
-            for (auto& t : r) t = t.view(shape);
-        return one_or_pair(r);
-    });
+    const auto shape = x.sizes().vec();
+    const bool flat = x.dim() == 2;
+    if (!fits(prepared, [&] {
+            TORCH_CHECK(shape.back() >= 1 && (!has(gate) || gate->sizes() == x.sizes()) &&
+                        (!has(res) || res->sizes() == x.sizes()), "gate and residual must have x's shape");
+        }))
+        return py::none();
+    auto rows = [&](const Tensor& t) { return flat ? t : t.reshape({-1, shape.back()}); };  // may copy
+    auto opt_rows = [&](const Opt& t) { return has(t) ? Opt(rows(*t)) : Opt(); };
+    const Tensor x2 = rows(x);
+    const Opt gate2 = opt_rows(gate), res2 = opt_rows(res);
+    BlockNormParams p;
+    if (!fits(prepared, [&] { p = norm_params(x2, gate2, post, res2, scale, pre, eps); })) return py::none();
+    variable_list r;
+    if (train) {
+        r = BlockNormFn::apply(x2, gate2, post, res2, scale, pre, eps);
+    } else {
+        for (auto& t : block_norm_fwd(p, x2, res2, false))
+            if (t.defined()) r.push_back(t);
+    }
+    if (!flat)
+        for (auto& t : r) t = t.view(shape);
+    return one_or_pair(r);
 }
 
 }  // namespace
