@@ -61,6 +61,12 @@ void check_main(const Tensor& t, const char* name) {
     for (long s : t.sizes()) TORCH_CHECK(s <= INT_MAX / 2, name, ": extent too large");
 }
 
+// A kernel is about to write t: graphs that saved it must not use it any more.
+// Tensors made in inference mode have no version, and no graph may save them.
+void will_write(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor empty_f32(const Tensor& like, at::IntArrayRef shape) {
     return torch::empty(shape, like.options().dtype(torch::kFloat));
 }
@@ -157,6 +163,7 @@ Tensor run_conv_step(const Tensor& x, const Tensor& state, const Tensor& state_o
     const long B = x.size(0), D = x.size(1), K = w.size(1);
     auto y = torch::empty({B, D}, x.options());
     if (B && D) {
+        will_write(state_out);
         short_conv_step_launch(x.data_ptr(), x.stride(0), state.data_ptr(), state_out.data_ptr(),
                                w.data_ptr<float>(), fptr(bias), y.data_ptr(), B, (int)D, (int)K, silu,
                                f32(x), stream());
@@ -329,12 +336,13 @@ ScanStepParams scan_step_params(const Tensor& u, const Tensor& delta, const Tens
     return p;
 }
 
-// p: scan_step_params of u and the rest
-Tensor run_scan_step(ScanStepParams p, const Tensor& u) {
+// p: scan_step_params of u, state_out and the rest
+Tensor run_scan_step(ScanStepParams p, const Tensor& u, const Tensor& state_out) {
     at::DeviceGuard guard(u.device());
     auto y = torch::empty({p.B, p.D}, u.options());
     if (p.B && p.D) {
         p.y = y.data_ptr();
+        will_write(state_out);
         scan_step_launch(p, f32(u), stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
@@ -343,7 +351,7 @@ Tensor run_scan_step(ScanStepParams p, const Tensor& u) {
 
 Tensor selective_scan_step(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state, Tensor state_out,
                            Opt skip, Opt dbias, bool softplus) {
-    return run_scan_step(scan_step_params(u, delta, A, Bm, Cm, state, state_out, skip, dbias, softplus), u);
+    return run_scan_step(scan_step_params(u, delta, A, Bm, Cm, state, state_out, skip, dbias, softplus), u, state_out);
 }
 
 // ---- norms around a block ---------------------------------------------------
@@ -640,7 +648,7 @@ py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor B
     ScanStepParams p;
     if (!fits(false, [&] { p = scan_step_params(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus); }))
         return py::none();
-    return py::make_tuple(run_scan_step(p, u), out);
+    return py::make_tuple(run_scan_step(p, u, out), out);
 }
 
 py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps, bool prepared) {
