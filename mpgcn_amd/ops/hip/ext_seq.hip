@@ -3,6 +3,7 @@
 // for its users; what the kernels rely on for their bounds is checked here too.
 #include <torch/extension.h>
 #include <cfloat>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPException.h>
@@ -458,10 +459,20 @@ using torch::autograd::variable_list;
 Tensor val(const Opt& t) { return has(t) ? *t : Tensor(); }
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 Opt rows_of(const Tensor& t) { return t.defined() ? Opt(t.contiguous()) : Opt(); }
-bool any(const variable_list& g) {
-    for (const auto& t : g)
-        if (t.defined()) return true;
-    return false;
+// The kernels would drop the tangent of forward mode in silence.
+void refuse(const char* name, const Tensor& t) {
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t.defined() || !t._fw_grad(0).defined(), name,
+                " has no forward-mode derivative on a GPU");
+}
+
+// Whether any gradient has arrived.
+bool any(const variable_list& g, const char* name) {
+    bool there = false;
+    for (const auto& t : g) {
+        refuse(name, t);
+        there |= t.defined();
+    }
+    return there;
 }
 
 // The gradients have no gradient of their own: a second derivative raises when
@@ -488,7 +499,7 @@ struct ShortConvFn : Function<ShortConvFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         variable_list out(7);
-        if (any(g)) {
+        if (any(g, "short_conv")) {
             at::NoGradGuard no_grad;
             auto v = ctx->get_saved_variables();
             const Tensor dy = g[0].defined() ? g[0].contiguous() : torch::zeros(v[0].sizes(), v[0].options());
@@ -517,7 +528,7 @@ struct SelectiveScanFn : Function<SelectiveScanFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         variable_list out(11);
-        if (any(g)) {
+        if (any(g, "selective_scan")) {
             at::NoGradGuard no_grad;
             auto v = ctx->get_saved_variables();
             auto r = selective_scan_bwd(rows_of(g[0]), g.size() > 1 ? rows_of(g[1]) : Opt(), v[0], v[1], v[2], v[3], v[4],
@@ -544,7 +555,7 @@ struct BlockNormFn : Function<BlockNormFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         variable_list out(7);
-        if (any(g)) {
+        if (any(g, "norm_gate_residual")) {
             at::NoGradGuard no_grad;
             auto v = ctx->get_saved_variables();
             const bool y = !v[3].defined() || v[5].defined();
@@ -571,7 +582,14 @@ bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c1
 // checks and conversions of mpgcn_amd/ops/sequence.py, which name what is wrong
 // and come back here with `prepared` set.
 
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
+using Inputs = std::initializer_list<const Tensor*>;
+
+void refuse(const char* name, Inputs ts) {
+    for (const Tensor* t : ts)
+        if (t) refuse(name, *t);
+}
+
+bool wants_grad(Inputs ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : ts)
         if (t && t->defined() && t->requires_grad()) return true;
@@ -606,7 +624,9 @@ bool apart(const Tensor& a, const Tensor& b) {
 py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, bool silu, bool want_state,
                              bool prepared) {
     if (!x.is_cuda()) return py::none();
-    const bool train = wants_grad({&x, &w, tp(bias), tp(s0)});
+    const Inputs ts = {&x, &w, tp(bias), tp(s0)};
+    refuse("short_conv", ts);
+    const bool train = wants_grad(ts);
     if (train && !prepared && capturing()) return py::none();
     ShortConvParams p;
     if (!fits(prepared, [&] { p = conv_params(x, w, bias, s0, lens, silu); })) return py::none();
@@ -617,9 +637,11 @@ py::object short_conv_direct(Tensor x, Tensor w, Opt bias, Opt s0, Opt lens, boo
 }
 
 py::object short_conv_step_direct(Tensor x, Tensor state, Opt state_out, Tensor w, Opt bias, bool silu) {
+    if (!x.is_cuda()) return py::none();
     const Tensor out = has(state_out) ? *state_out : state;
-    if (!x.is_cuda() || wants_grad({&x, &state, &out, &w, tp(bias)}) || !apart(state, out) ||
-        !fits(false, [&] { check_conv_step(x, state, out, w, bias); }))
+    const Inputs ts = {&x, &state, &out, &w, tp(bias)};
+    refuse("short_conv_step", ts);
+    if (wants_grad(ts) || !apart(state, out) || !fits(false, [&] { check_conv_step(x, state, out, w, bias); }))
         return py::none();
     return py::make_tuple(run_conv_step(x, state, out, w, bias, silu), out);
 }
@@ -627,7 +649,9 @@ py::object short_conv_step_direct(Tensor x, Tensor state, Opt state_out, Tensor 
 py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Opt skip, Opt dbias, Opt h0,
                                  Opt lens, bool softplus, bool want_state, bool prepared) {
     if (!u.is_cuda()) return py::none();
-    const bool train = wants_grad({&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)});
+    const Inputs ts = {&u, &delta, &A, &Bm, &Cm, tp(skip), tp(dbias), tp(h0)};
+    refuse("selective_scan", ts);
+    const bool train = wants_grad(ts);
     if (train && !prepared && capturing()) return py::none();
     const Tensor B4 = Bm.dim() == 3 ? Bm.unsqueeze(2) : Bm, C4 = Cm.dim() == 3 ? Cm.unsqueeze(2) : Cm;
     ScanParams p;
@@ -642,9 +666,11 @@ py::object selective_scan_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Te
 
 py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor Bm, Tensor Cm, Tensor state,
                                       Opt state_out, Opt skip, Opt dbias, bool softplus) {
+    if (!u.is_cuda()) return py::none();
     const Tensor out = has(state_out) ? *state_out : state;
-    if (!u.is_cuda() || wants_grad({&u, &delta, &A, &Bm, &Cm, &state, &out, tp(skip), tp(dbias)}) || !apart(state, out))
-        return py::none();
+    const Inputs ts = {&u, &delta, &A, &Bm, &Cm, &state, &out, tp(skip), tp(dbias)};
+    refuse("selective_scan_step", ts);
+    if (wants_grad(ts) || !apart(state, out)) return py::none();
     ScanStepParams p;
     if (!fits(false, [&] { p = scan_step_params(u, delta, A, Bm, Cm, state, out, skip, dbias, softplus); }))
         return py::none();
@@ -653,7 +679,9 @@ py::object selective_scan_step_direct(Tensor u, Tensor delta, Tensor A, Tensor B
 
 py::object block_norm_direct(Tensor x, Opt gate, Opt post, Opt res, Opt scale, Opt pre, double eps, bool prepared) {
     if (!x.is_cuda() || x.dim() < 1 || !(eps >= FLT_MIN)) return py::none();
-    const bool train = wants_grad({&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)});
+    const Inputs ts = {&x, tp(gate), tp(post), tp(res), tp(scale), tp(pre)};
+    refuse("norm_gate_residual", ts);
+    const bool train = wants_grad(ts);
     if (train && !prepared && capturing()) return py::none();
     const auto shape = x.sizes().vec();
     const bool flat = x.dim() == 2;

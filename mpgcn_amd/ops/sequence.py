@@ -19,9 +19,11 @@ take one new token per sequence: they update ``state`` in place (or write
 Activations are bf16 or f32 (f64 on CPU, for reference runs). Parameters are
 the f32 masters; another floating type is converted. Sums, states and norms
 are f32, each output is rounded once. Gradients of parameters and of B and C
-are added in a fixed order: the same call gives the same bits. Work is queued
-on the current stream of the inputs' device. On a GPU the HIP kernels run; on
-CPU the definitions in mpgcn_amd/ops/eager.py.
+are added in a fixed order: the same call gives the same bits. On a GPU
+forward-mode derivatives are refused.
+
+Work is queued on the current stream of the inputs' device. On a GPU the HIP
+kernels run; on CPU the definitions in mpgcn_amd/ops/eager.py.
 
 A training call may be captured into a graph. It is refused during capture if
 an eager graph of the same leaves is still alive on another stream, since the

@@ -1,14 +1,16 @@
 """The sequence operators beside the rest of autograd on the GPU: states that
-change under a graph that saved them."""
+change under a graph that saved them, forward-mode derivatives."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from mpgcn_amd import ops
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda:0"
+NAMES = ["short_conv", "short_conv_step", "selective_scan", "selective_scan_step", "norm_gate_residual"]
 
 
 def _rn(seed, *shape):
@@ -59,3 +61,46 @@ def test_only_the_state_that_is_written_counts_as_changed():
         step(want, None)
         step(held, None)  # a state made in inference mode, outside of it
         assert torch.equal(held, want)
+
+
+def _forms():
+    """name -> (call of its tensors, the tensors)."""
+    t = _scan(5)
+    w, h = _rn(21, 8, 3), _rn(22, 2, 8, 4)
+    x, z = _rn(23, 2, 5, 8), _rn(24, 2, 5, 8)
+    return {
+        "short_conv": (lambda x, w, b, s: ops.short_conv(x, w, b, state=s), (x, w, w[:, 0], _rn(25, 2, 2, 8))),
+        "short_conv_step": (lambda x, s, w: ops.short_conv_step(x, s, w)[0], (x[:, 0], _rn(25, 2, 2, 8), w)),
+        "selective_scan": (lambda u, d, A, B, C, k, b, s: ops.selective_scan(
+            u, d, A, B, C, k, delta_bias=b, delta_softplus=True, state=s), (*t.values(), w[:, 0], w[:, 1], h)),
+        "selective_scan_step": (lambda u, d, A, B, C, s: ops.selective_scan_step(u, d, A, B, C, s)[0],
+                                (*_step_of(t).values(), h)),
+        "norm_gate_residual": (lambda x, z, p, r, s, q: ops.norm_gate_residual(
+            x, gate=z, post_weight=p, residual=r, scale=s, pre_weight=q)[0], (x, z, w[:, 0], x, w[:, 1], w[:, 2])),
+    }
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(name, grad):
+    """No tangent is dropped in silence, whichever input carries it."""
+    call, args = _forms()[name]
+    with torch.set_grad_enabled(grad):
+        for i, a in enumerate(args):
+            with fwad.dual_level():
+                dual = fwad.make_dual(a, torch.ones_like(a))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*args[:i], dual, *args[i + 1:])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(call, args, tuple(torch.ones_like(a) for a in args))
+
+
+@pytest.mark.parametrize("name", ["short_conv", "selective_scan", "norm_gate_residual"])
+def test_forward_mode_over_the_gradient_is_refused(name):
+    call, args = _forms()[name]
+    leaf = args[0].clone().requires_grad_()
+    y = call(leaf, *args[1:])
+    with fwad.dual_level():
+        dy = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, dy)
