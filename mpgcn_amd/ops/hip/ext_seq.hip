@@ -10,6 +10,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "params.hpp"
 
@@ -584,7 +585,9 @@ bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c1
 
 using Inputs = std::initializer_list<const Tensor*>;
 
+// Nor does a trace see these calls: it would hold their outputs as constants.
 void refuse(const char* name, Inputs ts) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced on a GPU");
     for (const Tensor* t : ts)
         if (t) refuse(name, *t);
 }

@@ -20,7 +20,7 @@ Activations are bf16 or f32 (f64 on CPU, for reference runs). Parameters are
 the f32 masters; another floating type is converted. Sums, states and norms
 are f32, each output is rounded once. Gradients of parameters and of B and C
 are added in a fixed order: the same call gives the same bits. On a GPU
-forward-mode derivatives are refused.
+forward-mode derivatives and calls inside torch.jit.trace are refused.
 
 Work is queued on the current stream of the inputs' device. On a GPU the HIP
 kernels run; on CPU the definitions in mpgcn_amd/ops/eager.py.

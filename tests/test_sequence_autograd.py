@@ -1,5 +1,5 @@
 """The sequence operators beside the rest of autograd on the GPU: states that
-change under a graph that saved them, forward-mode derivatives."""
+change under a graph that saved them, forward-mode derivatives, tracing."""
 
 import pytest
 import torch
@@ -104,3 +104,11 @@ def test_forward_mode_over_the_gradient_is_refused(name):
         dy = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, leaf, dy)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(name):
+    """A trace would hold the outputs as constants."""
+    call, args = _forms()[name]
+    with torch.no_grad(), pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, tuple(args), check_trace=False)
