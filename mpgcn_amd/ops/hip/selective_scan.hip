@@ -590,6 +590,15 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
     }
 }
 
+// A state behind steps of size dt in all, with what they add on their way. The
+// decay goes on in two halves: between them the value lies between the old and
+// the new, so only one out of range itself leaves it, and a state of zero stays
+// zero where steps grow past it.
+__device__ __forceinline__ float carried(float state, float dt, float A2, float added) {
+    const float half = __builtin_amdgcn_exp2f(0.5f * dt * A2);
+    return state == 0.f ? added : fmaf(state * half, half, added);
+}
+
 // Turns each segment's own end state into the state it starts from (forward),
 // or its own adjoint at the start into the one at its end (backward). A block
 // takes four states of a task's lanes; its waves share the segments: each runs
@@ -642,7 +651,7 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
                 total += sj;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    carry[c] = fmaf(__builtin_amdgcn_exp2f(ss[c] * A2[c]), carry[c], on ? own[j][c] : 0.f);
+                    carry[c] = carried(carry[c], ss[c], A2[c], on ? own[j][c] : 0.f);
             }
         }
     };
@@ -657,7 +666,7 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
             float ss[4];
             quad_spread(sums[v][lane], ss);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) carry[c] = fmaf(__builtin_amdgcn_exp2f(ss[c] * A2[c]), carry[c], end[v][lane][c]);
+            for (int c = 0; c < 4; ++c) carry[c] = carried(carry[c], ss[c], A2[c], end[v][lane][c]);
         }
     } else {
         carry = start;
