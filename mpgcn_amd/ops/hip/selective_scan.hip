@@ -24,6 +24,8 @@
 //
 // Addresses are a wave-uniform 64-bit base and a 32-bit lane offset; where the
 // sequences of a wave lie too far apart for that a wave takes one sequence.
+#include <cfloat>
+
 #include "seq.hpp"
 
 #define SCAN_CH 8  // steps of a chunk: staged together, their states held by the backward
@@ -180,13 +182,26 @@ __device__ __forceinline__ float pick(const float* __restrict__ s, bool ok, long
     return ok ? v : 0.f;
 }
 
+// The decay of a state that there is not. Its state is zero as long as its
+// inputs' product with zero is: this keeps exp(dt A) finite up to an infinite
+// step, where that of 0 would be NaN, and 1 for every finite one.
+constexpr float NO_DECAY = -FLT_MIN;
+
+// log2(e) times the decay of state n0 + i of the lane's channel at index c
+template <int NQ, int KQ>
+__device__ __forceinline__ float decay(const ScanParams& p, const Place<NQ, KQ>& q, int c, int i) {
+    const bool ok = q.state(p, c, i);
+    const float v = pick(p.A, ok, (long)q.ch(c) * p.N + q.n0 + i) * LOG2E;
+    return ok ? v : NO_DECAY;
+}
+
 template <int NQ, int KQ>
 __device__ __forceinline__ void load_decay(const ScanParams& p, const Place<NQ, KQ>& q, f32x4 (&A2)[NQ]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-            A2[i][c] = pick(p.A, q.state(p, c, i), (long)q.ch(c) * p.N + q.n0 + i) * LOG2E;
+            A2[i][c] = decay(p, q, c, i);
 }
 
 // The lane's states in a (B, D, N) tensor, or zeros, for a wave whose first
@@ -619,7 +634,7 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const bool on = q.state(p, c, i);
-        A2[c] = pick(p.A, on, (long)q.ch(c) * p.N + q.n0 + i) * LOG2E;
+        A2[c] = decay(p, q, c, i);
         start[c] = first ? pick(first, on && b < p.B, (b * p.D + q.ch(c)) * p.N + q.n0 + i) : 0.f;
     }
     f32x4* seg_h = (f32x4*)p.seg_h + (id * l.nseg * NQ + i) * 64 + lane;
@@ -1006,7 +1021,7 @@ __launch_bounds__(256) __global__ void scan_step_kernel(ScanStepParams p, int gp
         for (int j = 0; j < 4; ++j) {
             const float v = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), hp.get(j), du * Bp.get(j));
             hp.w[j] = __float_as_int(v);
-            acc = fmaf(Cp.get(j), v, acc);
+            acc = j < n ? fmaf(Cp.get(j), v, acc) : acc;  // v is NaN past the last state where du is infinite
         }
         for (int m = 1; m < gp; m <<= 1) acc += __shfl_xor(acc, m);
         hp.store(p.h_out + r * N + at, n, N % 4);

@@ -281,7 +281,8 @@ def selective_scan(u, delta, A, B, C, skip=None, *, delta_bias=None, delta_softp
         y_t[d] = sum_n C_t[g, n] h_t[d, n] + skip[d] u_t[d]
 
     u, delta: (B, L, D); A: (D, N), N up to 64; B, C: (B, L, N) or (B, L, G, N),
-    group g of D / G channels sharing one row; skip, delta_bias: (D,).
+    group g of D / G channels sharing one row; skip, delta_bias: (D,). From a
+    step of +inf on its channel's outputs are inf or NaN.
     state: (B, D, N) f32, h before the first token (zeros if None). Returns y,
     or (y, f32 state after the last valid token).
     """

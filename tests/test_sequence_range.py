@@ -1,4 +1,5 @@
-"""The scan where the decay of a segment leaves the range of float32."""
+"""The scan where decays, states and steps leave the range of float32, over
+sequences that are cut into segments and in whole ones."""
 
 import pytest
 import torch
@@ -69,3 +70,43 @@ def test_a_segments_decay_past_the_range():
     r = oracle.scan_roundings(48, 16) + 4 * 145
     oracle.within(y, *ref["y"], r, "y")
     oracle.within(last, *ref["last"], r, "last")
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("L,at", [(20, 10), (700, 350)])
+@pytest.mark.parametrize("N", [3, 13, 16, 21])
+def test_an_infinite_step_is_not_seen_before_it(N, L, at, softplus):
+    """Tokens before an infinite step have the outputs and, where no loss comes
+    from behind it, the gradients of the sequence that ends there, also where the
+    states do not fill their lanes. From that step on a channel is not finite."""
+    t = _inputs(5, L, 12, N)
+    if softplus:
+        t["delta"] = t["delta"] - 3
+    t["delta"][:, at] = float("inf")
+    dy = torch.randn(1, L, 12, generator=torch.Generator().manual_seed(6)).to(DEV)
+    dy[:, at:] = 0
+    cut = {k: v[:, :at] if k != "A" else v for k, v in t.items()}
+    ref = oracle.scan(**cut, softplus=softplus, dy=dy[:, :at])
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    y = ops.selective_scan(**t, delta_softplus=softplus)
+    r = oracle.scan_roundings(at, N)
+    oracle.within(y[:, :at], *ref["y"], r, "y")
+    assert not torch.isfinite(y[:, at:]).any()
+    got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    for name in ("u", "delta", "B", "C"):
+        oracle.within(got[name][:, :at], *ref[name], r + (12 if name in ("B", "C") else 0), name)
+
+
+@pytest.mark.parametrize("N", [3, 13, 16, 21])
+def test_a_token_with_an_infinite_step(N):
+    t = _inputs(7, 1, 12, N)
+    t = {k: v.abs() if k in ("u", "B", "C") else v for k, v in t.items()}
+    t["delta"][:, 0, 5] = float("inf")
+    t["state"] = torch.ones(1, 12, N, device=DEV)
+    ref = oracle.scan(**t, softplus=False)
+    one = {k: v if k in ("A", "state") else v[:, 0] for k, v in t.items()}
+    y, s = ops.selective_scan_step(**one)
+    assert y[0, 5] == float("inf") and (s[0, 5] == float("inf")).all()
+    rest = [i for i in range(12) if i != 5]
+    oracle.within(y[:, rest], ref["y"][0][:, 0, rest], ref["y"][1][:, 0, rest], oracle.scan_roundings(1, N), "y")
+    oracle.within(s[:, rest], ref["last"][0][:, rest], ref["last"][1][:, rest], oracle.scan_roundings(1, N), "state")
