@@ -181,6 +181,9 @@ Tensor short_conv_step(Tensor x, Tensor state, Tensor state_out, Tensor w, Opt b
 
 // ---- selective scan ---------------------------------------------------------
 
+// At most a wave each in one launch, four to a block of 256.
+void check_channels(long D) { TORCH_CHECK(D <= (1L << 26) - 4, "at most 2^26 - 4 channels"); }
+
 ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
                        const Opt& skip, const Opt& dbias, const Opt& h0, const Opt& lens, bool softplus) {
     check_main(u, "u");
@@ -190,7 +193,7 @@ ScanParams scan_params(const Tensor& u, const Tensor& delta, const Tensor& A, co
     const long N = A.size(1);
     TORCH_CHECK(Bm.dim() == 4 && Bm.size(2) >= 1 && D % Bm.size(2) == 0, "B must be (B, L, G, N), G a divisor of D");
     const long G = Bm.size(2);
-    TORCH_CHECK(D < (1L << 26), "at most 2^26 channels");
+    check_channels(D);
     check_data(u, u, u.sizes(), "u");
     check_data(delta, u, {B, L, D}, "delta");
     check_data(Bm, u, {B, L, G, N}, "B");
@@ -311,6 +314,7 @@ ScanStepParams scan_step_params(const Tensor& u, const Tensor& delta, const Tens
     check_main(u, "u");
     TORCH_CHECK(u.dim() == 2, "u must be (B, D)");
     const long B = u.size(0), D = u.size(1);
+    check_channels(D);
     TORCH_CHECK(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be (D, N), N in 1..64");
     const long N = A.size(1);
     TORCH_CHECK(Bm.dim() == 2 || Bm.dim() == 3, "B must be (B, N) or (B, G, N)");

@@ -128,6 +128,14 @@ __device__ __forceinline__ int seq_len(const void* lens, int is64, int b, int L)
     return n < 0 ? 0 : n > L ? L : (int)n;
 }
 
+// A grid of `blocks`, and a block's number in it. One dimension of a grid holds
+// fewer than 2^32 threads; a launch of more is cut short without an error.
+static inline dim3 grid_of(long blocks) {
+    const long x = blocks < 1L << 21 ? blocks : 1L << 21;
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ long block_id() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 static inline int pow2_ceil(long n) {
     int p = 1;
     while (p < n) p <<= 1;

@@ -62,7 +62,7 @@ __device__ __forceinline__ void taps(const float* w, const float* bias, int c0, 
 template <typename T, int K, bool WHOLE>
 __launch_bounds__(256) __global__ void short_conv_fwd_kernel(ShortConvParams p, long items, int dv, int tiles) {
     constexpr int E = conv_e<T>(), NB = 4;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long i = block_id() * 256 + threadIdx.x;
     if (i >= items) return;
     const int c0 = (int)(i % dv) * E;
     const long r = i / dv;
@@ -140,7 +140,9 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
     constexpr int W = E * (K + 1);
     extern __shared__ float lds[];  // [256][W]
     const int rt = threadIdx.x / cw, nrt = 256 / cw;
-    const int cv = blockIdx.y * cw + threadIdx.x % cw;
+    // blocks of one channel group after those of another
+    const int group = blockIdx.x / p.slots, slot = blockIdx.x - group * p.slots;
+    const int cv = group * cw + threadIdx.x % cw;
     const int c0 = cv * E;
     const int n = WHOLE || p.D - c0 >= E ? E : p.D - c0, width = WHOLE ? E : p.D;
     float dw[K][E] = {}, db[E] = {};
@@ -148,7 +150,7 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
         float w[K][E], bias[E];
         taps<K, E>(p.w, p.bias, c0, n, w, bias);
         const long items = (long)p.B * tiles;
-        for (long i = (long)blockIdx.x * nrt + rt; i < items; i += (long)p.slots * nrt) {
+        for (long i = (long)slot * nrt + rt; i < items; i += (long)p.slots * nrt) {
             const int tile = (int)(i % tiles), b = (int)(i / tiles);
             const int len = seq_len(p.lens, p.lens64, b, p.L);
             const int t0 = tile * p.tile, t1 = t0 + p.tile < p.L ? t0 + p.tile : p.L;
@@ -244,10 +246,10 @@ __launch_bounds__(256) __global__ void short_conv_bwd_kernel(ShortConvParams p, 
         mine[E * K + c] = db[c];
     }
     __syncthreads();
-    float* ws = p.ws + (long)blockIdx.x * p.D * (K + 1);
+    float* ws = p.ws + (long)slot * p.D * (K + 1);
     for (int i = threadIdx.x; i < cw * W; i += 256) {
         const int v = i / W, e = i % W;
-        const int c = (blockIdx.y * cw + v) * E;
+        const int c = (group * cw + v) * E;
         float s = 0.f;
         for (int r = 0; r < nrt; ++r) s += lds[(r * cw + v) * W + e];
         if (e < E * K) {
@@ -265,7 +267,7 @@ template <typename T, int K>
 __launch_bounds__(256) __global__ void short_conv_step_kernel(
     const T* __restrict__ x, long x_b, const T* s_in, T* s_out, const float* __restrict__ w,
     const float* __restrict__ bias, T* __restrict__ y, long items, int dv, int D, int silu) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long i = block_id() * 256 + threadIdx.x;
     if (i >= items) return;
     const int c0 = (int)(i % dv) * SEQ_CH;
     const long b = i / dv;
@@ -318,7 +320,7 @@ struct Fwd {
         const int dv = (p.D + conv_e<T>() - 1) / conv_e<T>();
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const long items = (long)p.B * tiles * dv;
-        const dim3 grid((unsigned)((items + 255) / 256));
+        const dim3 grid = grid_of((items + 255) / 256);
         if (p.D % conv_e<T>() == 0)
             hipLaunchKernelGGL((short_conv_fwd_kernel<T, K, true>), grid, dim3(256), 0, s, p, items, dv, tiles);
         if (p.D % conv_e<T>() != 0)
@@ -335,7 +337,7 @@ struct Bwd {
         const int cw = conv_cw(dv);
         const int tiles = p.L ? (p.L + p.tile - 1) / p.tile : 1;
         const size_t smem = 256 * CONV_BE * (K + 1) * sizeof(float);
-        const dim3 grid(p.slots, (dv + cw - 1) / cw);
+        const dim3 grid((unsigned)p.slots * ((dv + cw - 1) / cw));
         if (p.D % CONV_BE == 0)
             hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, true>), grid, dim3(256), smem, s, p, dv, cw, tiles);
         if (p.D % CONV_BE != 0)
@@ -350,7 +352,7 @@ struct Step {
     void operator()() const {
         const int dv = (D + SEQ_CH - 1) / SEQ_CH;
         const long items = B * dv;
-        hipLaunchKernelGGL((short_conv_step_kernel<T, K>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s,
+        hipLaunchKernelGGL((short_conv_step_kernel<T, K>), grid_of((items + 255) / 256), dim3(256), 0, s,
             (const T*)x, x_b, (const T*)s_in, (T*)s_out, w, bias, (T*)y, items, dv, D, silu);
     }
 };
@@ -389,7 +391,7 @@ __launch_bounds__(1024) __global__ void seq_colsum_kernel(const float* __restric
                                                           float* __restrict__ out, long nb, long E) {
     __shared__ float part[16][65];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const long e = (long)blockIdx.x * 64 + c;
+    const long e = block_id() * 64 + c;
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
     if (e < E) {
         long b = r;
@@ -412,6 +414,6 @@ __launch_bounds__(1024) __global__ void seq_colsum_kernel(const float* __restric
 }
 
 extern "C" void seq_colsum_launch(const float* ws, float* out, long nb, long E, hipStream_t s) {
-    hipLaunchKernelGGL(seq_colsum_kernel, dim3((unsigned)((E + 63) / 64)), dim3(1024), 0, s,
+    hipLaunchKernelGGL(seq_colsum_kernel, grid_of((E + 63) / 64), dim3(1024), 0, s,
             ws, out, nb, E);
 }

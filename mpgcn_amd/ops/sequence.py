@@ -39,6 +39,7 @@ from mpgcn_amd.ops import eager
 _MAX_STATES = 64
 _MAX_NORM_D = 16384
 _MIN_EPS = torch.finfo(torch.float32).tiny
+_MAX_SCAN_D = (1 << 26) - 4  # where every channel is a group: a wave each in one launch
 _MAX_STEP = 1 << 26  # elements between tokens that the scan's 32-bit lane offsets allow
 
 
@@ -242,8 +243,8 @@ def _check_scan(u, delta, A, B, C, lead):
     if u.dim() != len(lead) + 1:
         raise ValueError(f"u must be ({', '.join(lead)}, channels), got {tuple(u.shape)}")
     D = u.shape[-1]
-    if D >= _MAX_STEP:
-        raise ValueError(f"u must have fewer than {_MAX_STEP} channels, got {D}")
+    if D > _MAX_SCAN_D:
+        raise ValueError(f"u must have at most {_MAX_SCAN_D} channels, got {D}")
     _check_act(delta, "delta", u.shape, u)
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != D:
         raise ValueError(f"A must have shape ({D}, N)")
