@@ -185,7 +185,7 @@ __device__ __forceinline__ float pick(const float* __restrict__ s, bool ok, long
 // The decay of a state that there is not. Its state is zero as long as its
 // inputs' product with zero is: this keeps exp(dt A) finite up to an infinite
 // step, where that of 0 would be NaN, and 1 for every finite one.
-constexpr float NO_DECAY = -FLT_MIN;
+constexpr float NO_DECAY = -2 * FLT_MIN;  // half of it is a number, too
 
 // log2(e) times the decay of state n0 + i of the lane's channel at index c
 template <int NQ, int KQ>
@@ -605,13 +605,14 @@ __launch_bounds__(256) __global__ void scan_fwd_kernel(ScanArgs) {
     }
 }
 
-// A state behind steps of size dt in all, with what they add on their way. The
-// decay goes on in two halves: between them the value lies between the old and
-// the new, so only one out of range itself leaves it, and a state of zero stays
-// zero where steps grow past it.
-__device__ __forceinline__ float carried(float state, float dt, float A2, float added) {
-    const float half = __builtin_amdgcn_exp2f(0.5f * dt * A2);
-    return state == 0.f ? added : fmaf(state * half, half, added);
+// A state behind steps of size dt in all, with what they add on their way; A2h
+// is half of the decay. It goes on in two halves: between them the value lies
+// between the old and the new, so only one out of range itself leaves it. The
+// bound keeps a state of zero at zero where steps grow past the range. (Where a
+// step's decay is NaN, what it adds is.)
+__device__ __forceinline__ float carried(float state, float dt, float A2h, float added) {
+    const float half = fminf(__builtin_amdgcn_exp2f(dt * A2h), FLT_MAX);
+    return fmaf(state * half, half, added);
 }
 
 // Turns each segment's own end state into the state it starts from (forward),
@@ -630,11 +631,11 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
     const Place<NQ, KQ> q(p, l, lane, (int)(id / l.cb % p.G), (int)(id % l.cb));
     const long b = id / l.cb / p.G * l.rw + q.rs;
     const float* first = BACK ? p.dh1 : p.h0;
-    f32x4 A2, carry = {0.f, 0.f, 0.f, 0.f}, start;
+    f32x4 A2h, carry = {0.f, 0.f, 0.f, 0.f}, start;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const bool on = q.state(p, c, i);
-        A2[c] = decay(p, q, c, i);
+        A2h[c] = 0.5f * decay(p, q, c, i);
         start[c] = first ? pick(first, on && b < p.B, (b * p.D + q.ch(c)) * p.N + q.n0 + i) : 0.f;
     }
     f32x4* seg_h = (f32x4*)p.seg_h + (id * l.nseg * NQ + i) * 64 + lane;
@@ -666,7 +667,7 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
                 total += sj;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    carry[c] = carried(carry[c], ss[c], A2[c], on ? own[j][c] : 0.f);
+                    carry[c] = carried(carry[c], ss[c], A2h[c], on ? own[j][c] : 0.f);
             }
         }
     };
@@ -681,7 +682,7 @@ __launch_bounds__(1024) __global__ void scan_carry_kernel(ScanParams p, ScanPlan
             float ss[4];
             quad_spread(sums[v][lane], ss);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) carry[c] = carried(carry[c], ss[c], A2[c], end[v][lane][c]);
+            for (int c = 0; c < 4; ++c) carry[c] = carried(carry[c], ss[c], A2h[c], end[v][lane][c]);
         }
     } else {
         carry = start;
