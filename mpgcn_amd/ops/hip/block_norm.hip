@@ -11,7 +11,8 @@
 // 8192 x 2560 with an f32 residual: 57 us forward, 92 us backward (4.4 and 4.1
 // TB/s); 1835008 x 32 with a gate: 193 us both, at a copy's rate. Both passes of
 // wide rows, f32 residual: 4096 x 5120 135 us, 2048 x 8192 160 us, 1024 x 16384
-// 332 us (4.6, 3.1, 1.5 TB/s): the backward of four chunks a thread spills.
+// 332 us (4.6, 3.1, 1.5 TB/s): the backward of four chunks a thread with a
+// residual spills 259 to 559 registers.
 #include "seq.hpp"
 
 namespace {
@@ -395,8 +396,10 @@ __launch_bounds__(MOST) __global__ void block_norm_bwd_kernel(BlockNormParams p,
 
 // Threads a row, chunks a thread: a part of a wave while that holds the row,
 // then whole waves with one chunk a thread (to D = 6144), two, four. One chunk
-// leaves no thread of a row idle and registers for the next row's loads: 4096 x
-// 5120 takes 135 us with one on 640 threads, 231 us with two on 320.
+// leaves registers for the next row's loads: 4096 x 5120 takes 135 us with one on
+// 640 threads, 231 us with two on 320. Widths just past a power of two of chunks,
+// or past whole waves of them, leave threads idle: 264 channels use 33 lanes of
+// 64, 520 use 65 threads of 128.
 inline void row_shape(long D, int* tpr, int* vpt) {
     const long chunks = (D + SEQ_CH - 1) / SEQ_CH;
     *vpt = chunks <= 768 ? 1 : chunks <= 1024 ? 2 : 4;
@@ -407,7 +410,9 @@ inline void row_shape(long D, int* tpr, int* vpt) {
 inline int block_threads(int tpr) { return tpr >= 256 ? tpr : 256 / tpr * tpr; }
 
 // Blocks that take the rows in turn: as many as 256 CUs hold at once, given the
-// waves a CU has registers for. More would leave a second, emptier round.
+// waves that a CU is taken to have registers for. More would leave a second,
+// emptier round, fewer an idle place: the counts below are those of the common
+// kernels of each kind, not of every one.
 inline long row_blocks(long R, int tpr, int waves) {
     const int block = block_threads(tpr), per_cu = waves / (block / 64);
     const long want = (R + block / tpr - 1) / (block / tpr), cap = 256L * (per_cu ? per_cu : 1);
@@ -419,6 +424,8 @@ struct NormFwd {
     hipStream_t s;
     template <typename T, typename TR, int VPT, bool RES, bool WHOLE, int MOST>
     void operator()(int tpr) const {
+        // 20 waves: what one chunk with a residual allows, but for f32 with an f32
+        // residual (16); without a residual 32 would fit, several chunks allow fewer
         hipLaunchKernelGGL((block_norm_fwd_kernel<T, TR, VPT, RES, WHOLE, MOST>),
                            dim3((unsigned)row_blocks(p.R, tpr, 20)), dim3(block_threads(tpr)), 0, s, p, tpr);
     }
@@ -471,6 +478,7 @@ void by_type(const BlockNormParams& p, int is_f32, int res_f32, F f) {
 extern "C" int block_norm_slots(long R, long D, int res, int gate) {
     int tpr, vpt;
     row_shape(D, &tpr, &vpt);
+    // a gate beside a residual: 8, though bf16 throughout has registers for 12
     return (int)row_blocks(R, tpr, vpt > 1 ? 8 : !res ? 16 : gate ? 8 : 12);
 }
 

@@ -363,7 +363,9 @@ struct Step {
 // each writes a row of filter gradients.
 extern "C" void short_conv_plan(ShortConvParams* p, int is_f32, int back) {
     const long e = back ? CONV_BE : is_f32 ? 4 : 8, dv = (p->D + e - 1) / e;
-    // 16 waves a CU forward, 8 backward: what the registers allow
+    // Tiles for 16 waves a CU forward, 8 backward. The registers allow 8 to 20 by
+    // type and taps: 12 for whole rows of bf16 and 4 taps, so that of the 1024
+    // blocks of 16384 x 4096 768 run at once; 8 to 16 backward.
     p->tile = conv_tile(p->B, p->L, dv, back ? 256L * 8 * 64 : 256L * 16 * 64);
     const long cw = conv_cw(dv), groups = (dv + cw - 1) / cw, rows = 256 / cw;
     const long items = p->B * (p->L ? ((long)p->L + p->tile - 1) / p->tile : 1);

@@ -352,9 +352,10 @@ def norm_gate_residual(x, *, gate=None, post_weight=None, residual=None, scale=N
     x, gate: (..., D) of one type, D up to 16384; residual: (..., D) bf16 or f32,
     which need not be x's type; post_weight, scale, pre_weight: (D,). Parts left
     out are skipped: one norm at least, and scale and pre_weight only with a
-    residual. h feeds the second norm unrounded; squares are summed in f32, so
-    values past 1e18 overflow them. Returns p without a residual,
-    h without pre_weight, else (y, h): p and y of x's type, h of the residual's.
+    residual. h feeds the second norm unrounded. Squares are summed in f32: a row
+    whose root mean square passes 1.8e19 / sqrt(D) overflows the sum and is
+    normed to zeros. Returns p without a residual, h without pre_weight, else
+    (y, h): p and y of x's type, h of the residual's.
     """
     if _on_gpu(x):
         out = _ops.get_ext().block_norm_direct(x, gate, post_weight, residual, scale, pre_weight, eps)
