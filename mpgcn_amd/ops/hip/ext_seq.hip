@@ -271,7 +271,11 @@ std::vector<Tensor> selective_scan_bwd(Opt dy, Opt dh1, Tensor u, Tensor delta, 
         return std::vector<Tensor>{du, dd, s.narrow(0, 0, D * N).view({D, N}), dB, dC, s.narrow(0, D * N, D),
                                    s.narrow(0, D * N + D, D), dh0};
     };
-    if (!B || !D) return split(torch::zeros({D * (N + 2)}, A.options()));
+    if (!B || !D) {
+        dB.zero_();
+        dC.zero_();
+        return split(torch::zeros({D * (N + 2)}, A.options()));
+    }
     const ScanPlan l = scan_plan(p, f32(u), 1);
     const long tasks = l.groups * G * l.cb;
     if (l.chunks > 1) {
