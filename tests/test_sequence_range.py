@@ -110,3 +110,17 @@ def test_a_token_with_an_infinite_step(N):
     rest = [i for i in range(12) if i != 5]
     oracle.within(y[:, rest], ref["y"][0][:, 0, rest], ref["y"][1][:, 0, rest], oracle.scan_roundings(1, N), "y")
     oracle.within(s[:, rest], ref["last"][0][:, rest], ref["last"][1][:, rest], oracle.scan_roundings(1, N), "state")
+
+
+@pytest.mark.parametrize("D,size", [(64, 2e18), (2560, 3e17), (16384, 1.2e17)])
+def test_norms_of_large_values(D, size):
+    """Rows whose root mean square stays below 1.8e19 / sqrt(D)."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.where(torch.rand(3, D, generator=g) < 0.5, -size, size).to(DEV)
+    w, q = torch.randn(D, generator=g).to(DEV), torch.randn(D, generator=g).to(DEV)
+    r = oracle.norm_roundings(D)
+    oracle.within(ops.norm_gate_residual(x, post_weight=w), *oracle.norm(x, None, w)["y"], r, "y")
+    y, h = ops.norm_gate_residual(x * 0, post_weight=w, residual=x, pre_weight=q)
+    ref = oracle.norm(x * 0, None, w, x, None, q)
+    oracle.within(h, *ref["h"], r, "h")
+    oracle.within(y, *ref["y"], r, "y")
