@@ -468,6 +468,7 @@ using torch::autograd::variable_list;
 Tensor val(const Opt& t) { return has(t) ? *t : Tensor(); }
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 Opt rows_of(const Tensor& t) { return t.defined() ? Opt(t.contiguous()) : Opt(); }
+
 // The kernels would drop the tangent of forward mode in silence.
 void refuse(const char* name, const Tensor& t) {
     TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t.defined() || !t._fw_grad(0).defined(), name,

@@ -157,8 +157,8 @@ struct Place {
 // log(1 + e^x) and its slope. e^-|x| with the rounding of the argument's product
 // put right, the logarithm of 1 + e with that sum's: within 4 + |x| / 4 times
 // 2^-24 of the result, where the second part is log2(e)'s own rounding and
-// counts for x < 0 alone. Past the exponent's range the remainder is infinite or NaN and e
-// is 0: the bound keeps their product 0.
+// counts for x < 0 alone. Past the exponent's range the remainder is infinite or
+// NaN and e is 0: the bound keeps their product 0.
 __device__ __forceinline__ float softplus_s(float x, float& slope) {
     const float a = -fabsf(x), hi = a * LOG2E, lo = fminf(fmaf(a, LOG2E, -hi), 1.f);
     float e = __builtin_amdgcn_exp2f(hi);
@@ -1118,10 +1118,10 @@ extern "C" ScanPlan scan_plan(const ScanParams& p, int is_f32, int back) {
     // Segments of at least 4 chunks where that brings the waves towards four per
     // SIMD, in the backward two: what the kernels of 9 states and more have
     // registers for (those of 8 and fewer have some for more: up to 8 forward, 4
-    // backward, which is not used). They cost a second pass
-    // over the recurrence, so fewer than 3 do not pay. Measured, forward and
-    // backward of 8192 x 1536: 378 us against 397 with four in the backward too;
-    // prompt of 16384 x 2048: 262 us against 290 with two.
+    // backward, which is not used). They cost a second pass over the recurrence,
+    // so fewer than 3 do not pay. Measured, forward and backward of 8192 x 1536:
+    // 378 us against 397 with four in the backward too; prompt of 16384 x 2048:
+    // 262 us against 290 with two.
     const long tasks = l.groups * p.G * l.cb, same = (long)p.G * l.cb;
     long nseg = tasks ? (back ? 2048 : 4096) / tasks : 1;
     // Two chunks where four would leave less than two waves a SIMD: 2 x 1024 x
